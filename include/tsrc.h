@@ -10,7 +10,8 @@
 //
 // Numerics: every result is the reference's bit for bit (the spec's f32 rules: DAZ inputs, RNE,
 // flush of subnormal results, canonical NaN 0x7FC00000; QACT A32 / A256; the 16-partial row dot of
-// sw/sim/tsr_ref.c:592-635), for any input bytes.
+// sw/sim/tsr_ref.c:592-635), for any input bytes. The q4_0 cache section below, which has no counterpart
+// there, states its own.
 //
 // Errors: every function returns TSRC_OK (0) or a negative TSRC_E_* code and then sets a message
 // that tsrc_last_error() returns (per thread). Nothing aborts and no C++ exception crosses the ABI.
@@ -265,6 +266,89 @@ typedef struct tsrc_fa_cfg {
 TSRC_API int tsrc_flash_attn(tsrc_ctx * ctx, const tsrc_kv * kv, const float * q, uint32_t T, uint32_t n_head,
                              uint32_t n_kv, const uint16_t * mask, uint32_t mask_stride, float scale,
                              uint32_t new_lo, uint32_t new_hi, const tsrc_fa_cfg * cfg, float * out, void * stream);
+
+// ---- q4_0 KV cache, the attention that reads it, and beam search's step ------------------------------
+// No counterpart in the reference, whose cache is q8_0 only and whose outputs end at the logits. The cache
+// holds ggml's q4_0 blocks (llama.cpp's q4_0 cache type): per 32 values {fp16 d; 32 codes n of 4 bits}, each
+// value standing for d (n - 8). Values in device memory are f32, f16 or bf16, named by ggml's type numbers.
+// Arithmetic is in f32 or better with rounding to nearest, not the reference's flushing f32 rules. Nothing here
+// allocates device memory after tsrc_kv4_create (set_bytes / get_bytes stage through a temporary buffer) or
+// synchronises, except where noted, so every queued call may be captured into a CUDA graph; workspaces are the
+// caller's, and calls (or graphs) that may run at the same time need one each. The calling thread's current
+// device is left as it was.
+#define TSRC_TYPE_F32   0u
+#define TSRC_TYPE_F16   1u
+#define TSRC_TYPE_BF16 30u
+
+typedef struct tsrc_kv4 tsrc_kv4;
+
+// Allocates a zeroed cache of n_cells cells of E = n_head_kv * head_dim values for K and for V (head_dim 64, 128,
+// 256 or 512; E / 64 <= 511; n_cells 1..2^30): 2 * n_cells * E * 18 / 32 bytes, the cells rounded up to 64.
+TSRC_API int tsrc_kv4_create(tsrc_ctx * ctx, uint32_t n_head_kv, uint32_t head_dim, uint32_t n_cells, tsrc_kv4 ** out);
+// Synchronises the device, then frees the cache.
+TSRC_API int tsrc_kv4_free(tsrc_kv4 * kv);
+// Quantizes rows i < n of E values (k and v: device memory, row_stride values apart, 0 = E; either may be NULL)
+// and stores them at cells cells[i] (device int64) or, with cells = NULL, at cell0 + i. A block's codes and scale
+// are ggml's: m = the first value of largest magnitude, d = m / -8, n = min(15, trunc(x * (1 / d) + 8.5)), each
+// step rounded to f32, d stored as fp16; a NaN is stored as code 8 and does not become m, and a block with an
+// infinity reads back NaN. A cell outside the cache is not stored and makes the next tsrc_sync return TSRC_E_ARG.
+// Cells must differ: of rows that name the same cell, which one's values a block keeps is not defined. On `stream`.
+TSRC_API int tsrc_kv4_set_rows(tsrc_ctx * ctx, tsrc_kv4 * kv, uint32_t type, const void * k, const void * v, uint32_t n,
+                               uint32_t row_stride, const int64_t * cells, uint32_t cell0, void * stream);
+// The inverse: the values d (n - 8) of cells cells[i] (any order, repeats allowed) or cell0 + i, rounded to `type`,
+// into rows of k and / or v. A cell outside the cache leaves its row unwritten and makes the next tsrc_sync return
+// TSRC_E_ARG. On `stream`.
+TSRC_API int tsrc_kv4_get_rows(tsrc_ctx * ctx, const tsrc_kv4 * kv, uint32_t type, void * k, void * v, uint32_t n,
+                               uint32_t row_stride, const int64_t * cells, uint32_t cell0, void * stream);
+// The ggml q4_0 image of cells [cell0, cell0 + n): rows of E / 32 blocks of 18 bytes, in host or device memory
+// (byte 2 + j of a block: the codes of values j, low bits, and j + 16). Synchronous.
+TSRC_API int tsrc_kv4_set_bytes(tsrc_kv4 * kv, uint32_t which, const void * ggml_rows, uint32_t cell0, uint32_t n);
+TSRC_API int tsrc_kv4_get_bytes(const tsrc_kv4 * kv, uint32_t which, void * ggml_rows, uint32_t cell0, uint32_t n);
+// Beam search's reordering of its states: n_group groups of n_beam (1..32) sequences, sequence s = g * n_beam + b
+// holding cells [cell0 + s * seq_stride, + n). Afterwards sequence (g, b) holds what (g, parent[g * n_beam + b])
+// held before, K and V, in place (parent: device int32, any values in [0, n_beam), as tsrc_beam_select writes
+// them; -1: the sequence keeps its cells). Another parent keeps them too and makes the next tsrc_sync return
+// TSRC_E_ARG. seq_stride >= n. On `stream`.
+TSRC_API int tsrc_kv4_reorder(tsrc_ctx * ctx, tsrc_kv4 * kv, const int32_t * parent, uint32_t n_group, uint32_t n_beam,
+                              uint32_t cell0, uint32_t seq_stride, uint32_t n, void * stream);
+
+// Attention over the cache. For token t < T and query head h < n_head (a multiple of n_head_kv; head h reads KV
+// head h / (n_head / n_head_kv)), over the cells c that t sees:
+//   out[t][h][:] = sum_c p_c V[c] / sum_c p_c,   p_c = exp(s_c - max_c s_c),   s_c = scale * q[t][h] . K[c] + mask[t][c]
+// with K and V the values the codes stand for, products and sums in f32 or better, and one rounding to `type` (of
+// q and out) at the end. Token t sees cells [ranges[2t], ranges[2t + 1]) (device int32, cut to [0, n_kv); NULL: all
+// n_kv) whose mask (device f16 [T][mask_stride], cells from 0; NULL: none) is not -inf; what other cells hold, NaN
+// or infinities included, has no effect. A token that sees no cell gets zeros. A NaN score makes its row NaN.
+// So a decode step of many sequences, a causal or windowed prompt and a drafted tree are one call each; the ranges
+// may be rewritten on the device between replays of a captured call.
+// group (0 = T): consecutive tokens that read about the same cells (a sequence's); T must be a multiple of it.
+// max_len (0 = n_kv): about how many cells one group's tokens span. Both choose how the work is split, never what
+// is computed. q and out: device, token rows q_stride / out_stride values apart (0 = n_head * head_dim), heads dense.
+// ws: ws_bytes of device memory (256-byte aligned), at least tsrc_flash_attn_q4_workspace's (NULL when that is 0);
+// its content needs no initialisation. out must not overlap q. On `stream`.
+TSRC_API int tsrc_flash_attn_q4(tsrc_ctx * ctx, const tsrc_kv4 * kv, uint32_t type, const void * q, uint32_t q_stride,
+                                uint32_t T, uint32_t n_head, uint32_t n_kv, const int32_t * ranges, uint32_t group,
+                                uint32_t max_len, const uint16_t * mask, uint32_t mask_stride, float scale, void * out,
+                                uint32_t out_stride, void * ws, size_t ws_bytes, void * stream);
+// Workspace bytes of such a call (host only, no device needed; the arguments of the call).
+TSRC_API size_t tsrc_flash_attn_q4_workspace(uint32_t type, uint32_t n_head_kv, uint32_t head_dim, uint32_t T, uint32_t n_head,
+                                             uint32_t n_kv, uint32_t group, uint32_t max_len);
+// Why such a call could not run (NULL if it can); host only.
+TSRC_API const char * tsrc_flash_attn_q4_unsupported(uint32_t type, uint32_t n_head_kv, uint32_t head_dim, uint32_t n_head);
+
+// One step of beam search: for each of n_group groups of n_beam rows of n_vocab logits (device, `type`, rows
+// `stride` values apart, 0 = n_vocab; row g * n_beam + b),
+//   s[b][v] = scores[g][b] + x[b][v] - log(sum_u exp(x[b][u]))       (scores: device f32, NULL = zeros)
+// and the n_out largest over all (b, v) of the group, in descending order, equal ones by ascending (b, v):
+// out_scores (f32), out_beam and out_token (int32), each [n_group][n_out]. Comparisons are on s in f64. A candidate
+// whose s is -inf or NaN is never chosen (banned tokens, dead beams; a row with a NaN or +inf logit loses every
+// candidate); where too few are left the rest of the row is (-inf, -1, -1). n_out 1..64, n_beam 1..64.
+// ws as above, tsrc_beam_select_workspace bytes. On `stream`.
+TSRC_API int tsrc_beam_select(tsrc_ctx * ctx, uint32_t type, const void * logits, uint32_t stride, const float * scores,
+                              uint32_t n_group, uint32_t n_beam, uint32_t n_vocab, uint32_t n_out, float * out_scores,
+                              int32_t * out_beam, int32_t * out_token, void * ws, size_t ws_bytes, void * stream);
+TSRC_API size_t tsrc_beam_select_workspace(uint32_t n_group, uint32_t n_beam, uint32_t n_vocab, uint32_t n_out);
+TSRC_API const char * tsrc_beam_select_unsupported(uint32_t type, uint32_t n_beam, uint32_t n_vocab, uint32_t n_out);
 
 // ---- the decoder layer's vector kinds (VU ops of the reference's kinds) ----------------------------
 // Every f32 result follows the reference's vector-unit rules (DAZ inputs, RNE, FTZ results,

@@ -117,6 +117,8 @@ struct tsrc_ctx {
     size_t fa_scratch_bytes = 0;
     std::set<tsrc_weight*> weights;
     std::set<tsrc_kv*> kvs;
+    std::set<tsrc_kv4*> kv4s;
+    bool kv4_used = false;           // tsrc_sync reads the q4_0 cache's error word only where one was made
 };
 
 namespace {
@@ -212,6 +214,13 @@ bool kv_geometry_ok(uint32_t n_head_kv, uint32_t D) {
 namespace tsrc {
 
 int set_error(int code, const char* msg) { return fail(code, "%s", msg); }
+
+// The q4_0 caches a context owns (tsrc_close drops them).
+void ctx_add_kv4(tsrc_ctx* ctx, tsrc_kv4* kv) {
+    ctx->kv4s.insert(kv);
+    ctx->kv4_used = true;
+}
+void ctx_remove_kv4(tsrc_ctx* ctx, tsrc_kv4* kv) { ctx->kv4s.erase(kv); }
 
 // Makes the context's device current (for translation units that do not see tsrc_ctx) and returns
 // its ordinal in *dev.
@@ -388,6 +397,7 @@ int tsrc_close(tsrc_ctx* ctx) {
     cudaDeviceSynchronize();
     while (!ctx->weights.empty()) drop_weight(*ctx->weights.begin());
     while (!ctx->kvs.empty()) drop_kv(*ctx->kvs.begin());
+    while (!ctx->kv4s.empty()) tsrc::kv4_drop(*ctx->kv4s.begin());
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->fa_scratch) cudaFree(ctx->fa_scratch);
     delete ctx;
@@ -416,6 +426,13 @@ int tsrc_sync(tsrc_ctx* ctx, void* stream) {
     e = tsrc::vu_error(&code, true);
     if (e != cudaSuccess) return cuda_fail(e, "reading the vector-kind error flag");
     if (code) return fail(TSRC_E_ARG, "tsrc_get_rows: a token id outside the weight (that row was not written)");
+    if (!ctx->kv4_used) return TSRC_OK;
+    e = tsrc::kv4_error(&code, true);
+    if (e != cudaSuccess) return cuda_fail(e, "reading the q4_0 cache error word");
+    if (code & tsrc::kKv4ErrSet) return fail(TSRC_E_ARG, "tsrc_kv4_set_rows: a cell index outside the cache (those rows were not stored)");
+    if (code & tsrc::kKv4ErrGet) return fail(TSRC_E_ARG, "tsrc_kv4_get_rows: a cell index outside the cache (those rows were not written)");
+    if (code & tsrc::kKv4ErrParent) return fail(TSRC_E_ARG, "tsrc_kv4_reorder: a parent outside [0, n_beam) (those sequences kept their cells)");
+    if (code) return fail(TSRC_E_DEVICE, "a q4_0 attention kernel gave up a bounded wait (code %u)", code);
     return TSRC_OK;
 }
 

@@ -7,6 +7,7 @@
 
 struct tsrc_ctx;
 struct tsrc_kv;
+struct tsrc_kv4;
 struct tsrc_fa_cfg;
 
 namespace tsrc {
@@ -240,5 +241,16 @@ cudaError_t launch_kv_to_ggml(const int8_t* q, const uint16_t* d, uint32_t n, ui
 // The first error a KVST launch recorded on the current device (0 = none, 1 = a cell index
 // outside the cache).
 cudaError_t kv_error(uint32_t* code, bool clear);
+
+
+// ---- q4_0 cache, its attention, beam selection (tsrc_kv4.cu, tsrc_fa4.cu, tsrc_beam.cu) ----
+int set_error(int code, const char* msg);
+int ctx_device(const tsrc_ctx* ctx, int* dev);
+void ctx_add_kv4(tsrc_ctx* ctx, tsrc_kv4* kv);
+void ctx_remove_kv4(tsrc_ctx* ctx, tsrc_kv4* kv);
+void kv4_drop(tsrc_kv4* kv);
+// bits of the q4_0 kernels' error word, cleared when read with clear = true
+constexpr uint32_t kKv4ErrSet = 1u, kKv4ErrGet = 2u, kKv4ErrParent = 4u, kKv4ErrWait = 8u;
+cudaError_t kv4_error(uint32_t* code, bool clear);
 
 }  // namespace tsrc

@@ -94,6 +94,20 @@ _SIGS = {
     "tsrc_kv_set_rows": (_i, [_p, _p, _u32, _p, _u32, _u32, _p, _u32, _p]),
     "tsrc_kv_set_bytes": (_i, [_p, _u32, _p, _u32, _u32]),
     "tsrc_kv_get_bytes": (_i, [_p, _u32, _p, _u32, _u32]),
+    "tsrc_kv4_create": (_i, [_p, _u32, _u32, _u32, ct.POINTER(_p)]),
+    "tsrc_kv4_free": (_i, [_p]),
+    "tsrc_kv4_set_rows": (_i, [_p, _p, _u32, _p, _p, _u32, _u32, _p, _u32, _p]),
+    "tsrc_kv4_get_rows": (_i, [_p, _p, _u32, _p, _p, _u32, _u32, _p, _u32, _p]),
+    "tsrc_kv4_set_bytes": (_i, [_p, _u32, _p, _u32, _u32]),
+    "tsrc_kv4_get_bytes": (_i, [_p, _u32, _p, _u32, _u32]),
+    "tsrc_kv4_reorder": (_i, [_p, _p, _p, _u32, _u32, _u32, _u32, _u32, _p]),
+    "tsrc_flash_attn_q4": (_i, [_p, _p, _u32, _p, _u32, _u32, _u32, _u32, _p, _u32, _u32, _p, _u32, _f32, _p, _u32,
+                                _p, ct.c_size_t, _p]),
+    "tsrc_flash_attn_q4_workspace": (ct.c_size_t, [_u32] * 8),
+    "tsrc_flash_attn_q4_unsupported": (ct.c_char_p, [_u32] * 4),
+    "tsrc_beam_select": (_i, [_p, _u32, _p, _u32, _p, _u32, _u32, _u32, _u32, _p, _p, _p, _p, ct.c_size_t, _p]),
+    "tsrc_beam_select_workspace": (ct.c_size_t, [_u32] * 4),
+    "tsrc_beam_select_unsupported": (ct.c_char_p, [_u32] * 4),
     "tsrc_flash_attn": (_i, [_p, _p, _p, _u32, _u32, _u32, _p, _u32, _f32, _u32, _u32, _p, _p, _p]),
 }
 
@@ -115,6 +129,8 @@ MODEL_GLOBAL = 0xFFFFFFFF
 KV_K, KV_V = 0, 1
 TEAM_HANDLE_BYTES = 64
 Q8_0_BLOCK_BYTES = 34
+Q4_0_BLOCK_BYTES = 18
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30
 
 
 def declared_symbols() -> list[str]:
@@ -168,6 +184,45 @@ def _stream(stream) -> int | None:
     if isinstance(stream, int):
         return stream or None
     return stream.cuda_stream or None
+
+
+def _type_of(*tensors) -> int:
+    """The TSRC_TYPE_* that the given torch tensors (None left out) share."""
+    names = {str(t.dtype) for t in tensors if t is not None}
+    kind = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16, "torch.bfloat16": TYPE_BF16}.get(names.pop() if len(names) == 1 else "")
+    if kind is None:
+        raise TsrcError(E_ARG, "tensors must be of one type among float32, float16 and bfloat16")
+    return kind
+
+
+def _expect(t, dtype: str, what: str):
+    """t's address after a check of its element type and density (None and raw addresses pass)."""
+    if t is not None and not isinstance(t, int):
+        if str(t.dtype) != "torch." + dtype or not t.is_contiguous() or not t.is_cuda:
+            raise TsrcError(E_ARG, f"{what} must be a contiguous CUDA tensor of {dtype}")
+    return _addr(t)
+
+
+def _workspace(like, nbytes: int, stream):
+    """(tensor kept alive for the call, address): torch's allocator orders its reuse by stream."""
+    if nbytes == 0:
+        return None, None
+    import torch
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    if stream is not None:
+        ws.record_stream(torch.cuda.ExternalStream(stream, device=like.device) if isinstance(stream, int) else stream)
+    return ws, ws.data_ptr()
+
+
+def flash_attn_q4_unsupported(type_: int, n_head_kv: int, head_dim: int, n_head: int) -> str | None:
+    """Why an attention over a q4_0 cache of this shape could not run (None if it can)."""
+    why = lib().tsrc_flash_attn_q4_unsupported(type_, n_head_kv, head_dim, n_head)
+    return None if why is None else why.decode()
+
+
+def beam_select_unsupported(type_: int, n_beam: int, n_vocab: int, n_out: int) -> str | None:
+    why = lib().tsrc_beam_select_unsupported(type_, n_beam, n_vocab, n_out)
+    return None if why is None else why.decode()
 
 
 def ggml_row_bytes(fmt: int, K: int) -> int:
@@ -383,6 +438,41 @@ class Device:
                                      new[0], new[1], None if c is None else ct.byref(c), _addr(out),
                                      _stream(stream)))
 
+    # ---- q4_0 cache, the attention over it, beam search ----
+    def kv4_create(self, n_head_kv: int, head_dim: int, n_cells: int) -> "Kv4Cache":
+        h = _p()
+        _check(lib().tsrc_kv4_create(self.handle, n_head_kv, head_dim, n_cells, ct.byref(h)))
+        return Kv4Cache(self, h, n_head_kv, head_dim, n_cells)
+
+    def flash_attn_q4(self, kv: "Kv4Cache", q, out, T: int, n_head: int, n_kv: int, scale: float, ranges=None,
+                      group: int = 0, max_len: int = 0, mask=None, mask_stride: int = 0, q_stride: int = 0,
+                      out_stride: int = 0, workspace=None, stream=None) -> None:
+        """out[t][h] = attention of q[t][h] over the cells of kv that token t sees (tsrc_flash_attn_q4).
+        q / out: device f32, f16 or bf16 tensors of one type; ranges: device int32 [T][2]; mask: device f16
+        [T][mask_stride]; workspace: a device buffer of flash_attn_q4_workspace bytes, or None to take one from
+        torch's allocator."""
+        kind = _type_of(q, out)
+        if mask is not None and not isinstance(mask, int) and mask_stride == 0:
+            mask_stride = mask.shape[-1]
+        nbytes = lib().tsrc_flash_attn_q4_workspace(kind, kv.n_head_kv, kv.head_dim, T, n_head, n_kv, group, max_len)
+        ws, ptr = (workspace, _addr(workspace)) if workspace is not None else _workspace(q, nbytes, stream)
+        size = nbytes if ws is None or isinstance(ws, int) else ws.numel() * ws.element_size()
+        _check(lib().tsrc_flash_attn_q4(self.handle, kv.handle, kind, _addr(q), q_stride, T, n_head, n_kv,
+                                        _expect(ranges, "int32", "ranges"), group, max_len, _expect(mask, "float16", "mask"),
+                                        mask_stride, scale, _addr(out), out_stride, ptr, size, _stream(stream)))
+
+    def beam_select(self, logits, scores, out_scores, out_beam, out_token, n_group: int, n_beam: int, n_vocab: int,
+                    n_out: int, stride: int = 0, workspace=None, stream=None) -> None:
+        """The n_out best continuations of each group's beams (tsrc_beam_select)."""
+        kind = _type_of(logits)
+        nbytes = lib().tsrc_beam_select_workspace(n_group, n_beam, n_vocab, n_out)
+        ws, ptr = (workspace, _addr(workspace)) if workspace is not None else _workspace(logits, nbytes, stream)
+        size = nbytes if ws is None or isinstance(ws, int) else ws.numel() * ws.element_size()
+        _check(lib().tsrc_beam_select(self.handle, kind, _addr(logits), stride, _expect(scores, "float32", "scores"), n_group,
+                                      n_beam, n_vocab, n_out, _expect(out_scores, "float32", "out_scores"),
+                                      _expect(out_beam, "int32", "out_beam"), _expect(out_token, "int32", "out_token"),
+                                      ptr, size, _stream(stream)))
+
 
 class Weight:
     """A weight shard resident in device memory."""
@@ -511,6 +601,68 @@ class KvCache:
     def free(self) -> None:
         if self.handle and self.dev.handle:
             _check(lib().tsrc_kv_free(self.handle))
+        self.handle = None
+
+
+class Kv4Cache:
+    """One layer's q4_0 K and V cache resident in device memory."""
+
+    def __init__(self, dev: Device, handle, n_head_kv: int, head_dim: int, n_cells: int):
+        self.dev, self.handle = dev, handle
+        self.n_head_kv, self.head_dim, self.n_cells = n_head_kv, head_dim, n_cells
+        self.E = n_head_kv * head_dim
+
+    @property
+    def row_bytes(self) -> int:
+        return self.E // 32 * Q4_0_BLOCK_BYTES
+
+    def set_bytes(self, which: int, ggml_rows, cell0: int = 0) -> None:
+        """ggml q4_0 rows (uint8 [n, row_bytes], a numpy array or a CUDA tensor) -> cells [cell0, cell0 + n)."""
+        import numpy as np
+        if hasattr(ggml_rows, "data_ptr"):
+            a = ggml_rows.contiguous()
+            if str(a.dtype) != "torch.uint8" or a.numel() % self.row_bytes:
+                raise TsrcError(E_ARG, "set_bytes: uint8 rows of row_bytes are wanted")
+            addr, n = a.data_ptr(), a.numel() // self.row_bytes
+        else:
+            a = np.ascontiguousarray(ggml_rows, dtype=np.uint8).reshape(-1, self.row_bytes)
+            addr, n = a.ctypes.data, a.shape[0]
+        _check(lib().tsrc_kv4_set_bytes(self.handle, which, addr, cell0, n))
+
+    def get_bytes(self, which: int, cell0: int = 0, n: int | None = None):
+        import numpy as np
+        n = self.n_cells - cell0 if n is None else n
+        out = np.zeros((n, self.row_bytes), np.uint8)
+        _check(lib().tsrc_kv4_get_bytes(self.handle, which, out.ctypes.data, cell0, n))
+        return out
+
+    def set_rows(self, k, v, n: int | None = None, cells=None, cell0: int = 0, row_stride: int = 0, stream=None) -> None:
+        """Quantizes device rows [n][E] of k and v (f32, f16 or bf16; either may be None) into cells (device int64)
+        or cell0 + i."""
+        n = self._rows(k, v) if n is None else n
+        _check(lib().tsrc_kv4_set_rows(self.dev.handle, self.handle, _type_of(k, v), _addr(k), _addr(v), n, row_stride,
+                                       _expect(cells, "int64", "cells"), cell0, _stream(stream)))
+
+    def get_rows(self, k, v, n: int | None = None, cells=None, cell0: int = 0, row_stride: int = 0, stream=None) -> None:
+        """The values of cells (device int64) or cell0 + i into device rows of k and v (either may be None)."""
+        n = self._rows(k, v) if n is None else n
+        _check(lib().tsrc_kv4_get_rows(self.dev.handle, self.handle, _type_of(k, v), _addr(k), _addr(v), n, row_stride,
+                                       _expect(cells, "int64", "cells"), cell0, _stream(stream)))
+
+    @staticmethod
+    def _rows(k, v) -> int:
+        if k is None and v is None:
+            raise TsrcError(E_ARG, "neither k nor v rows")
+        return (v if k is None else k).shape[0]
+
+    def reorder(self, parent, n_group: int, n_beam: int, seq_stride: int, n: int, cell0: int = 0, stream=None) -> None:
+        """Sequence (g, b) takes the first n cells of (g, parent[g][b]) (device int32), in place."""
+        _check(lib().tsrc_kv4_reorder(self.dev.handle, self.handle, _expect(parent, "int32", "parent"), n_group, n_beam, cell0,
+                                      seq_stride, n, _stream(stream)))
+
+    def free(self) -> None:
+        if self.handle and self.dev.handle:
+            _check(lib().tsrc_kv4_free(self.handle))
         self.handle = None
 
 
