@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const T* __restrict__ k,
         return;
     }
     const size_t hc = (size_t)u.head * p.n_alloc + (size_t)cell;
-    uint8_t* q = p.q[which] + hc * (p.D / 2u) + u.group * (NB * 16u) + u.g * (NB * 2u);
+    uint8_t* q = p.q[which] + hc * (p.D / 2u) + u.group * (NB * 16u) + kv4_place(u.g, (size_t)cell) * (NB * 2u);
     if constexpr (NB == 4) *reinterpret_cast<uint2*>(q) = make_uint2(code[0] | (code[1] << 16), code[2] | (code[3] << 16));
     else *reinterpret_cast<uint32_t*>(q) = code[0] | (code[1] << 16);
     if (u.g < NB) {
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(T* __restrict__ k, T* __r
         return;
     }
     const size_t hc = (size_t)u.head * p.n_alloc + (size_t)cell;
-    const uint8_t* q = p.q[which] + hc * (p.D / 2u) + u.group * (NB * 16u) + u.g * (NB * 2u);
+    const uint8_t* q = p.q[which] + hc * (p.D / 2u) + u.group * (NB * 16u) + kv4_place(u.g, (size_t)cell) * (NB * 2u);
     const __half* ds = p.d[which] + hc * (p.D / 32u) + u.group * NB;
     uint32_t w[NB / 2], s[NB / 2];
     if constexpr (NB == 4) {
@@ -182,7 +182,7 @@ __global__ void kv4_from_ggml_kernel(const uint8_t* ggml, uint32_t n, uint32_t c
             const uint32_t e = 4u * g + j;
             c |= (e < 16u ? src[2 + e] & 15u : src[2 + e - 16u] >> 4) << (4u * j);
         }
-        *reinterpret_cast<uint16_t*>(row + g * NB * 2u) = (uint16_t)c;
+        *reinterpret_cast<uint16_t*>(row + kv4_place(g, (size_t)cell0 + i) * NB * 2u) = (uint16_t)c;
     }
 }
 
@@ -199,51 +199,57 @@ __global__ void kv4_to_ggml_kernel(uint8_t* ggml, uint32_t n, uint32_t cell0, ui
     dst[1] = (uint8_t)(d >> 8);
     const uint8_t* row = p.q[which] + hc * (p.D / 2u) + (b / NB) * (NB * 16u) + (b % NB) * 2u;
     for (uint32_t g = 0; g < 4; ++g) {
-        const uint32_t lo = *reinterpret_cast<const uint16_t*>(row + g * NB * 2u);
-        const uint32_t hi = *reinterpret_cast<const uint16_t*>(row + (g + 4u) * NB * 2u);
+        const uint32_t lo = *reinterpret_cast<const uint16_t*>(row + kv4_place(g, (size_t)cell0 + i) * NB * 2u);
+        const uint32_t hi = *reinterpret_cast<const uint16_t*>(row + kv4_place(g + 4u, (size_t)cell0 + i) * NB * 2u);
         for (uint32_t j = 0; j < 4; ++j)
             dst[2 + 4u * g + j] = (uint8_t)(((lo >> (4u * j)) & 15u) | (((hi >> (4u * j)) & 15u) << 4));
     }
 }
 
-// Reordering in place: the same thread owns the same bytes of every sequence of a group, reads those that move
+// Reordering in place: the same thread owns the same values of every sequence of a group, reads those that move
 // and then writes them, so no copy overtakes another. U: the unit of bytes (16 for codes; the scales of a cell
-// need not be 16-byte aligned where a sequence starts).
+// need not be 16-byte aligned where a sequence starts). swap: the bit of a unit's index that the chunks' places
+// flip (kv4_place) where the cell has its bit 2 set: half a group's units for codes, 0 for scales.
 template <class U, uint32_t NBEAM>
-__global__ void __launch_bounds__(256) kv4_reorder_kernel(U* a, U* b, uint32_t units_cell, uint32_t n_alloc, const int32_t* parent,
-                                                          uint32_t n_beam, uint32_t cell0, uint32_t seq_stride, uint32_t n) {
+__global__ void __launch_bounds__(256) kv4_reorder_kernel(U* a, U* b, uint32_t units_cell, uint32_t swap, uint32_t n_alloc,
+                                                          const int32_t* parent, uint32_t n_beam, uint32_t cell0, uint32_t seq_stride,
+                                                          uint32_t n) {
     const uint32_t group = blockIdx.y, head = blockIdx.z >> 1;
-    U* plane = (blockIdx.z & 1u) ? b : a;
+    U* plane = ((blockIdx.z & 1u) ? b : a) + (size_t)head * n_alloc * units_cell;
     const size_t j = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
     const int32_t* par = parent + (size_t)group * n_beam;
     if (j >= (size_t)n * units_cell) return;
-    U* base = plane + ((size_t)head * n_alloc + cell0 + (size_t)group * n_beam * seq_stride) * units_cell + j;
-    const size_t step = (size_t)seq_stride * units_cell;
+    const uint32_t i = (uint32_t)(j / units_cell), unit = (uint32_t)(j - (size_t)i * units_cell);
+    const size_t first = (size_t)cell0 + (size_t)group * n_beam * seq_stride + i;
+    auto at = [&](uint32_t s) {
+        const size_t cell = first + (size_t)s * seq_stride;
+        return plane + cell * units_cell + (unit ^ ((cell & 4u) ? swap : 0u));
+    };
     U w[NBEAM];
 #pragma unroll
     for (uint32_t s = 0; s < NBEAM; ++s) {
         if (s >= n_beam) break;
         const int32_t from = par[s];
-        if (from >= 0 && from < (int32_t)n_beam && from != (int32_t)s) w[s] = base[(size_t)from * step];
+        if (from >= 0 && from < (int32_t)n_beam && from != (int32_t)s) w[s] = *at((uint32_t)from);
         else if ((from < -1 || from >= (int32_t)n_beam) && j == 0) atomicOr(&g_kv4_error, kKv4ErrParent);
     }
 #pragma unroll
     for (uint32_t s = 0; s < NBEAM; ++s) {
         if (s >= n_beam) break;
         const int32_t from = par[s];
-        if (from >= 0 && from < (int32_t)n_beam && from != (int32_t)s) base[(size_t)s * step] = w[s];
+        if (from >= 0 && from < (int32_t)n_beam && from != (int32_t)s) *at(s) = w[s];
     }
 }
 
 template <class U>
-cudaError_t launch_reorder(U* a, U* b, uint32_t units_cell, const tsrc_kv4* kv, const int32_t* parent, uint32_t n_group,
+cudaError_t launch_reorder(U* a, U* b, uint32_t units_cell, uint32_t swap, const tsrc_kv4* kv, const int32_t* parent, uint32_t n_group,
                            uint32_t n_beam, uint32_t cell0, uint32_t seq_stride, uint32_t n, cudaStream_t st) {
     const size_t units = (size_t)n * units_cell;
     const dim3 grid((unsigned)((units + 255u) / 256u), n_group, 2u * kv->n_head_kv);
     if (n_beam <= 8u)
-        kv4_reorder_kernel<U, 8><<<grid, 256, 0, st>>>(a, b, units_cell, kv->n_alloc, parent, n_beam, cell0, seq_stride, n);
+        kv4_reorder_kernel<U, 8><<<grid, 256, 0, st>>>(a, b, units_cell, swap, kv->n_alloc, parent, n_beam, cell0, seq_stride, n);
     else
-        kv4_reorder_kernel<U, 32><<<grid, 256, 0, st>>>(a, b, units_cell, kv->n_alloc, parent, n_beam, cell0, seq_stride, n);
+        kv4_reorder_kernel<U, 32><<<grid, 256, 0, st>>>(a, b, units_cell, swap, kv->n_alloc, parent, n_beam, cell0, seq_stride, n);
     return cudaGetLastError();
 }
 
@@ -451,10 +457,11 @@ int tsrc_kv4_reorder(tsrc_ctx* ctx, tsrc_kv4* kv, const int32_t* parent, uint32_
     DeviceScope scope(ctx);
     if (scope.rc) return scope.rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t e = launch_reorder(reinterpret_cast<uint4*>(kv->q[0]), reinterpret_cast<uint4*>(kv->q[1]), kv->D / 32u, kv, parent,
+    cudaError_t e = launch_reorder(reinterpret_cast<uint4*>(kv->q[0]), reinterpret_cast<uint4*>(kv->q[1]), kv->D / 32u,
+                                   kv->D == 64u ? 1u : 2u, kv, parent,
                                    n_group, n_beam, cell0, seq_stride, n, st);
     if (e == cudaSuccess)
-        e = launch_reorder(reinterpret_cast<uint32_t*>(kv->d[0]), reinterpret_cast<uint32_t*>(kv->d[1]), kv->D / 64u, kv, parent,
+        e = launch_reorder(reinterpret_cast<uint32_t*>(kv->d[0]), reinterpret_cast<uint32_t*>(kv->d[1]), kv->D / 64u, 0u, kv, parent,
                            n_group, n_beam, cell0, seq_stride, n, st);
     return e == cudaSuccess ? TSRC_OK : cuda_refuse(e, "tsrc_kv4_reorder");
 }

@@ -11,6 +11,8 @@
 // one chunk (8 bytes; 4 for D = 64) with four values of every block, and two neighbouring chunks (16 bytes) are
 // the eight values of every block that a lane feeds to the four k indices it owns: K and V are both read in the
 // fragment layout with wide loads and no shuffles, and K and V planes look alike.
+// In every second run of four cells chunk g lies in place g ^ 4: the lanes that read one chunk of four or eight
+// cells of a tile in shared memory then meet no bank twice.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -32,6 +34,9 @@ struct tsrc_kv4 {
 namespace tsrc {
 
 constexpr uint32_t kKv4Pad = 64;
+
+// where chunk g of a cell's row lies
+__host__ __device__ __forceinline__ uint32_t kv4_place(uint32_t g, size_t cell) { return g ^ ((uint32_t)cell & 4u); }
 
 // Restores the calling thread's current device when it leaves an entry point.
 class DeviceScope {

@@ -186,32 +186,60 @@ def _stream(stream) -> int | None:
     return stream.cuda_stream or None
 
 
-def _type_of(*tensors) -> int:
-    """The TSRC_TYPE_* that the given torch tensors (None left out) share."""
-    names = {str(t.dtype) for t in tensors if t is not None}
-    kind = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16, "torch.bfloat16": TYPE_BF16}.get(names.pop() if len(names) == 1 else "")
-    if kind is None:
+_torch = None        # torch, its element types and its stream lookup: set by the first call that needs them
+_kinds: dict = {}
+_raw_stream = None
+
+
+def _load_torch():
+    global _torch, _raw_stream
+    import torch
+    _kinds.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16})
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    _torch = torch
+    return torch
+
+
+def _type_of(a, b=None) -> int:
+    """The TSRC_TYPE_* that one or two torch tensors (None left out) share."""
+    _torch or _load_torch()
+    if a is None:
+        a, b = b, None
+    kind = None if a is None else _kinds.get(a.dtype)
+    if kind is None or (b is not None and b.dtype != a.dtype):
         raise TsrcError(E_ARG, "tensors must be of one type among float32, float16 and bfloat16")
     return kind
 
 
 def _expect(t, dtype: str, what: str):
     """t's address after a check of its element type and density (None and raw addresses pass)."""
-    if t is not None and not isinstance(t, int):
-        if str(t.dtype) != "torch." + dtype or not t.is_contiguous() or not t.is_cuda:
-            raise TsrcError(E_ARG, f"{what} must be a contiguous CUDA tensor of {dtype}")
-    return _addr(t)
+    if t is None or isinstance(t, int):
+        return t
+    if t.dtype is not getattr(_torch or _load_torch(), dtype) or not t.is_contiguous() or not t.is_cuda:
+        raise TsrcError(E_ARG, f"{what} must be a contiguous CUDA tensor of {dtype}")
+    return t.data_ptr()
 
 
-def _workspace(like, nbytes: int, stream):
-    """(tensor kept alive for the call, address): torch's allocator orders its reuse by stream."""
+def _stream_on(index: int, stream):
+    """The stream's handle; None: the device's current stream (not the current device's)."""
+    if stream is None:
+        _torch or _load_torch()
+        return _raw_stream(index) or None
+    return _stream(stream)
+
+
+def _workspace(like, nbytes: int, given, stream):
+    """(tensor kept alive for the call, address, bytes) of a call's workspace: the caller's, or one from torch's
+    allocator, which orders its reuse by stream."""
+    if given is not None:
+        return given, _addr(given), nbytes if isinstance(given, int) else given.numel() * given.element_size()
     if nbytes == 0:
-        return None, None
-    import torch
+        return None, None, 0
+    torch = _torch or _load_torch()
     ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
     if stream is not None:
         ws.record_stream(torch.cuda.ExternalStream(stream, device=like.device) if isinstance(stream, int) else stream)
-    return ws, ws.data_ptr()
+    return ws, ws.data_ptr(), nbytes
 
 
 def flash_attn_q4_unsupported(type_: int, n_head_kv: int, head_dim: int, n_head: int) -> str | None:
@@ -455,23 +483,21 @@ class Device:
         if mask is not None and not isinstance(mask, int) and mask_stride == 0:
             mask_stride = mask.shape[-1]
         nbytes = lib().tsrc_flash_attn_q4_workspace(kind, kv.n_head_kv, kv.head_dim, T, n_head, n_kv, group, max_len)
-        ws, ptr = (workspace, _addr(workspace)) if workspace is not None else _workspace(q, nbytes, stream)
-        size = nbytes if ws is None or isinstance(ws, int) else ws.numel() * ws.element_size()
+        ws, ptr, size = _workspace(q, nbytes, workspace, stream)
         _check(lib().tsrc_flash_attn_q4(self.handle, kv.handle, kind, _addr(q), q_stride, T, n_head, n_kv,
                                         _expect(ranges, "int32", "ranges"), group, max_len, _expect(mask, "float16", "mask"),
-                                        mask_stride, scale, _addr(out), out_stride, ptr, size, _stream(stream)))
+                                        mask_stride, scale, _addr(out), out_stride, ptr, size, _stream_on(self.index, stream)))
 
     def beam_select(self, logits, scores, out_scores, out_beam, out_token, n_group: int, n_beam: int, n_vocab: int,
                     n_out: int, stride: int = 0, workspace=None, stream=None) -> None:
         """The n_out best continuations of each group's beams (tsrc_beam_select)."""
         kind = _type_of(logits)
         nbytes = lib().tsrc_beam_select_workspace(n_group, n_beam, n_vocab, n_out)
-        ws, ptr = (workspace, _addr(workspace)) if workspace is not None else _workspace(logits, nbytes, stream)
-        size = nbytes if ws is None or isinstance(ws, int) else ws.numel() * ws.element_size()
+        ws, ptr, size = _workspace(logits, nbytes, workspace, stream)
         _check(lib().tsrc_beam_select(self.handle, kind, _addr(logits), stride, _expect(scores, "float32", "scores"), n_group,
                                       n_beam, n_vocab, n_out, _expect(out_scores, "float32", "out_scores"),
                                       _expect(out_beam, "int32", "out_beam"), _expect(out_token, "int32", "out_token"),
-                                      ptr, size, _stream(stream)))
+                                      ptr, size, _stream_on(self.index, stream)))
 
 
 class Weight:
@@ -641,13 +667,13 @@ class Kv4Cache:
         or cell0 + i."""
         n = self._rows(k, v) if n is None else n
         _check(lib().tsrc_kv4_set_rows(self.dev.handle, self.handle, _type_of(k, v), _addr(k), _addr(v), n, row_stride,
-                                       _expect(cells, "int64", "cells"), cell0, _stream(stream)))
+                                       _expect(cells, "int64", "cells"), cell0, _stream_on(self.dev.index, stream)))
 
     def get_rows(self, k, v, n: int | None = None, cells=None, cell0: int = 0, row_stride: int = 0, stream=None) -> None:
         """The values of cells (device int64) or cell0 + i into device rows of k and v (either may be None)."""
         n = self._rows(k, v) if n is None else n
         _check(lib().tsrc_kv4_get_rows(self.dev.handle, self.handle, _type_of(k, v), _addr(k), _addr(v), n, row_stride,
-                                       _expect(cells, "int64", "cells"), cell0, _stream(stream)))
+                                       _expect(cells, "int64", "cells"), cell0, _stream_on(self.dev.index, stream)))
 
     @staticmethod
     def _rows(k, v) -> int:
@@ -658,7 +684,7 @@ class Kv4Cache:
     def reorder(self, parent, n_group: int, n_beam: int, seq_stride: int, n: int, cell0: int = 0, stream=None) -> None:
         """Sequence (g, b) takes the first n cells of (g, parent[g][b]) (device int32), in place."""
         _check(lib().tsrc_kv4_reorder(self.dev.handle, self.handle, _expect(parent, "int32", "parent"), n_group, n_beam, cell0,
-                                      seq_stride, n, _stream(stream)))
+                                      seq_stride, n, _stream_on(self.dev.index, stream)))
 
     def free(self) -> None:
         if self.handle and self.dev.handle:

@@ -6,7 +6,11 @@ Tolerance of an output value, from the arithmetic (e = 2^-24, u = the rounding o
            the blocks' scales: |ds| <= (3 D / 16 + 16) e A, A = scale * max_c sum |q||k|, plus e times the mask
            value's size where a mask is added and 2 e |s| for the change of base;
   weights  dp / p <= |ds| + |ds of the maximum| + 2^-21 (the exponential);
-  output   sum p v / sum p: (2 |ds| + 2^-20 + 64 e) * sum p |v|, and u |out| for the last rounding (fp16: at least
+  output   sum p v / sum p: (2 |ds| + 2^-20 + 64 e) * sum p |v|; values enter the products as d n, n = 0..15, and
+           8 sum p d is taken off at the end, so a rounding is relative to 16 sum p |d| also where v = d (n - 8) is
+           near 0. A tensor-core step adds 16 products and the sum so far, each cut at a unit (2 e) of the largest;
+           a warp takes a step for 16 cells of its share (a quarter, and a tile's rest) of the n cells, and four
+           f32 steps follow: (34 (n / 64 + 2) + 4) e * 16 sum p |d| more; and u |out| for the last rounding (fp16: at least
            2^-25, half the step of its subnormal numbers).
 bf16 outputs allow the kernels one fp16 rounding (2^-11) of each weight, each key and each value: 2^-10 (A + 1) sum p |v| more.
 """
@@ -26,6 +30,10 @@ def _tolerance(q, kb, vb, Hk, scale, ranges, mask, dtype, want):
     n = len(kb)
     k, v = (np.abs(P.unpack(b).reshape(n, Hk, D)) for b in (kb, vb))
     tol = np.zeros_like(want)
+
+    def scales(rows):
+        return np.abs(np.ascontiguousarray(rows.reshape(n, -1, 18)[..., :2]).view(np.float16).astype(np.float64)).reshape(n, Hk, D // 32)
+
     e = 2.0 ** -24
     for t in range(T):
         lo, hi = (0, n) if ranges is None else (max(int(ranges[t][0]), 0), min(int(ranges[t][1]), n))
@@ -48,7 +56,8 @@ def _tolerance(q, kb, vb, Hk, scale, ranges, mask, dtype, want):
                 s = s + mask[t, :n][seen].astype(np.float64)
             p = np.exp(s - s.max())
             pv = (p @ vv) / p.sum()
-            tol[t, h] = (2 * ds + 2.0 ** -20 + 64 * e) * pv + np.maximum(HALF[dtype] * np.abs(want[t, h]), 2.0 ** -25 if dtype == "float16" else 0.0)
+            pd = np.repeat((p @ scales(vb)[seen, h // (H // Hk)]) / p.sum(), 32)
+            tol[t, h] = (2 * ds + 2.0 ** -20 + 64 * e) * pv + (34 * (n / 64 + 2) + 4) * e * 16 * pd + np.maximum(HALF[dtype] * np.abs(want[t, h]), 2.0 ** -25 if dtype == "float16" else 0.0)
             if dtype == "bfloat16":
                 tol[t, h] += 2.0 ** -10 * (A + 1) * pv
     return tol + 1e-30
