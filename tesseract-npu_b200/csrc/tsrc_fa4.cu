@@ -8,8 +8,9 @@ namespace tsrc {
 
 namespace {
 
-constexpr uint32_t kDecWarps = 4, kDecTile = 32;
-constexpr uint32_t kDecCtas = 3 * 148;         // CTAs that fill a B200 once, three to an SM
+constexpr uint32_t kDecWarps = 4, kDecTile = 32, kDecStages = 3;
+constexpr uint32_t kSms = 148, kDecCtas = 4 * kSms;      // the CTAs that a B200 holds at once, four to an SM
+constexpr uint32_t kMaxCluster = 16;
 
 struct Fa4Args {
     const void* q;
@@ -23,8 +24,10 @@ struct Fa4Args {
     size_t mask_stride;
     float scale;
     uint32_t group, row_tiles, splits;         // tokens a group, row tiles a group and KV head, splits of the cells
-    float *part_o, *part_ml;                   // splits > 1: [unit][split][R][D], [unit][split][R][4]
+    float *part_o, *part_ml;                   // splits joined by the merge kernel: [unit][split][R][D], [unit][split][R][4]
 };
+
+constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -40,23 +43,37 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// d = a b + c of a 16 x 16 by 16 x 8 tile
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                         float c0, float c1, float c2, float c3) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {      // of an 8 x 8 tile of fp16, two neighbours a lane
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 __device__ __forceinline__ __half2 as_h2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) { return as_u32(__floats2half2_rn(lo, hi)); }
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float remote_f32(const float* p, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
+}
 
-// how a warp's sixteen mma rows are used
+// how a warp's columns of eight query rows are used
 enum : int {
-    kRows8Split = 0,       // eight query rows; rows 8..15 carry the second fp16 term of q and of the weights
-    kRows8 = 1,            // eight query rows, one fp16 term (bf16 outputs)
-    kRows16 = 2,           // sixteen query rows, one fp16 term (bf16 outputs)
+    kRows8Split = 0,       // eight rows; q and the weights in two fp16 terms each
+    kRows8 = 1,            // eight rows, one term (bf16 outputs)
+    kRows16 = 2,           // sixteen rows, one term (bf16 outputs)
 };
 template <int MODE> constexpr uint32_t kRowsOf = MODE == kRows16 ? 16u : 8u;
 
@@ -68,332 +85,301 @@ template <int D> struct DecShape {
     static constexpr uint32_t ROW = W / 2, DS = NB * 2;         // bytes of a cell's codes and scales in a group
     static constexpr uint32_t V_AT = kDecTile * ROW, KD_AT = 2 * kDecTile * ROW, VD_AT = KD_AT + kDecTile * DS;
     static constexpr uint32_t STAGE = VD_AT + kDecTile * DS;
-    static constexpr uint32_t STAGES = NG > 1 ? 3 : 4;          // three CTAs' rings fit an SM
-    static constexpr uint32_t RING = STAGE * STAGES;
+    static constexpr uint32_t RING = STAGE * kDecStages;
 };
+// ring (later the warps' results), the warps' and the CTA's maxima and sums, the score exchange of teams (two turns)
+// or the factors of a cluster's CTAs
+constexpr uint32_t kRedBytes = (kDecWarps + 1u) * 16u * 3u * 4u;
 template <int D, int MODE> __host__ __device__ constexpr uint32_t dec_smem() {
     using S = DecShape<D>;
-    // ring (later the warps' results), score exchange of teams (two turns), maxima and sums of the warps
-    return kDecWarps * S::RING + (S::NG > 1 ? 2u * kDecWarps * 32u * (MODE == kRows16 ? 16u : 8u) * 4u : 0u) + kDecWarps * 16u * 3u * 4u;
+    return kDecWarps * S::RING + kRedBytes + (S::NG > 1 ? 2u * kDecWarps * 32u : kMaxCluster + 1u) * kRowsOf<MODE> * 4u;
 }
+
+// The weights' scale, by the exponent field v of the largest |dV| met: p is taken times 2^weight_exp(v) and, where
+// all dV are tiny, dV times 2^10, so that w = p dV stays below 2^15 and keeps its digits above fp16's last, 2^-24.
+__device__ __forceinline__ int weight_exp(uint32_t v) { return v >= 15u ? 29 - (int)v : 15; }
+__device__ __forceinline__ int value_exp(uint32_t v) { return v < 5u ? 10 : 0; }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // Decode attention, one pass over the cells.
 //   A CTA takes up to 8 (16) query rows -- the (token, head) pairs of a group that share a KV head -- and one split
-// of the cells they span, its warps tiles of 32 cells in turn (D > 128: teams of D / 128 warps, each with 128 values
-// of the head, which add up their partial scores through shared memory). Tiles come by cp.async, four deep.
+// of the cells they span; its warps take tiles of 32 cells in turn (D > 128: teams of D / 128 warps, each with 128
+// values of the head, which add up their partial scores through shared memory). Tiles come by cp.async, three deep.
+// The splits of a row are the CTAs of one cluster, which join their results through shared memory, or, where more
+// than sixteen are wanted, separate CTAs and a merge kernel.
+//   Both products run transposed, scores = K q^T and outputs = V^T w^T, so that the eight columns of an mma are the
+// query rows and its sixteen rows are cells (values): with few query rows nothing of a tile is idle, and an output
+// takes half the registers. The weights change from the first product's layout to the second's by movmatrix.
 //   Codes go to the tensor cores as they are: a code n in the low four bits of an fp16 is the subnormal number
-// n 2^-24, in the next four n 2^-20 (q's values that meet those carry 2^-4), so an operand register of two codes
-// is one AND of a word of eight (and a shift for every second pair). What is missing, sum q (n - 8) = sum q n -
-// 8 sum q, is the accumulator's start value for K; for V the weights' sum comes from one more mma per block with
-// 8 2^-24 in every column. The blocks' scales stay out of the products: K's multiply the four (two) partial
-// sums of a score in f32; V's multiply the weights: w = p dV, one set of weights per block.
-//   Precision: q and w are two fp16 terms each, 22 bits (q scaled by a power of two per row, the weights by 2^14
-// and by a power of two that follows the largest |dV| seen, so that neither term leaves fp16's range); for bf16
-// outputs one term, 11 bits. Running maximum, sum and outputs are f32.
+// n 2^-24, in the next four n 2^-20 (q's values that meet those carry 2^-4; outputs from those are scaled at the
+// end), so an operand register of two codes is one AND of a word of eight, and a shift for every second pair. What
+// is missing, sum q (n - 8) = sum q n - 8 sum q, is the accumulator's start value for K; for V the weights' sum
+// comes from one more mma per block with 8 2^-24 in every row. The blocks' scales stay out of the products: K's
+// multiply the four (two) partial sums of a score in f32; V's multiply the weights: w = p dV, a set for each block.
+//   Precision: q and w are two fp16 terms each, 22 bits (q scaled by a power of two per row); for bf16 outputs one
+// term, 11 bits. Running maximum, sum and outputs are f32.
 template <class T, int D, int MODE, bool MASK>
-__global__ void __launch_bounds__(kDecWarps * 32, 3) fa4_dec_kernel(Fa4Args a) {
+__global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_dec_kernel(Fa4Args a) {
     using S = DecShape<D>;
-    constexpr uint32_t NB = S::NB, R = kRowsOf<MODE>, RS = MODE == kRows16 ? 2 : 1;   // RS: rows of a lane
+    constexpr uint32_t NB = S::NB, R = kRowsOf<MODE>, NT = R / 8;        // NT: columns of eight rows
+    constexpr bool SPLIT = MODE == kRows8Split;
     extern __shared__ __align__(128) uint8_t sm[];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t = lane & 3u;
     const uint32_t team = warp / S::NG, sub = warp % S::NG;
-    const uint32_t unit = blockIdx.x, split = blockIdx.y;
+    const uint32_t unit = blockIdx.x / a.splits, split = blockIdx.x - unit * a.splits;
     const uint32_t hk = unit % a.n_head_kv, rt = unit / a.n_head_kv % a.row_tiles, grp = unit / (a.n_head_kv * a.row_tiles);
     const uint32_t rows = a.group * a.G;
-    const uint32_t ring = smem_u32(sm) + warp * S::RING;
     uint8_t* ringp = sm + warp * S::RING;
-    float* xch = reinterpret_cast<float*>(sm + kDecWarps * S::RING);
-    float* red = reinterpret_cast<float*>(sm + dec_smem<D, MODE>() - kDecWarps * 16u * 3u * 4u);      // [warp][16][3]
+    const uint32_t ring = smem_u32(ringp);
+    float* red = reinterpret_cast<float*>(sm + kDecWarps * S::RING);     // [warps + 1][16][3]
+    float* xch = red + kRedBytes / 4u;
 
-    // the rows' cells, and the hull of them
-    int32_t lo[RS], hi[RS], first = 0x7FFFFFFF, last = 0;
-    const T* qrow[RS];
-    const __half* mrow[RS];
+    // the cells of this lane's rows (8 n + 2 t + i), and the hull of all rows
+    int32_t lo[NT][2], hi[NT][2], first = 0x7FFFFFFF, last = 0, all_lo = 0, all_hi = 0x7FFFFFFF;
+    const __half* mrow[NT][2];
 #pragma unroll
-    for (uint32_t r = 0; r < RS; ++r) {
-        const uint32_t row = rt * R + g + 8u * r;
-        lo[r] = hi[r] = 0;
-        qrow[r] = nullptr;
-        mrow[r] = a.mask;
-        if (row < rows) {
-            const uint32_t tok = grp * a.group + row / a.G, h = hk * a.G + row % a.G;
-            hi[r] = (int32_t)a.n_kv;
-            if (a.ranges) {
-                lo[r] = max(a.ranges[2u * (size_t)tok], 0);
-                hi[r] = min(a.ranges[2u * (size_t)tok + 1u], (int32_t)a.n_kv);
+    for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            const uint32_t row = rt * R + 8u * n + 2u * t + i;
+            lo[n][i] = hi[n][i] = 0;
+            mrow[n][i] = a.mask;
+            if (row < rows) {
+                const uint32_t tok = grp * a.group + row / a.G;
+                int32_t x = 0, y = (int32_t)a.n_kv;
+                if (a.ranges) {
+                    x = max(a.ranges[2u * (size_t)tok], 0);
+                    y = min(a.ranges[2u * (size_t)tok + 1u], y);
+                }
+                if (x < y) {
+                    lo[n][i] = x;
+                    hi[n][i] = y;
+                    first = min(first, x);
+                    last = max(last, y);
+                }
+                // the cells that every row sees; a column without a row has nothing to lose
+                all_lo = max(all_lo, lo[n][i]);
+                all_hi = min(all_hi, hi[n][i]);
+                if (MASK) mrow[n][i] = a.mask + (size_t)tok * a.mask_stride;
             }
-            if (lo[r] >= hi[r]) lo[r] = hi[r] = 0;
-            else {
-                first = min(first, lo[r]);
-                last = max(last, hi[r]);
-            }
-            qrow[r] = static_cast<const T*>(a.q) + (size_t)tok * a.q_stride + (size_t)h * D + sub * S::W;
-            if (MASK) mrow[r] = a.mask + (size_t)tok * a.mask_stride;
         }
-    }
     first = __reduce_min_sync(0xFFFFFFFFu, first);
     last = __reduce_max_sync(0xFFFFFFFFu, last);
-    // the cells that every row sees (an unused row must not stop the shortcut: it has no cells to lose)
-    int32_t all_lo = 0, all_hi = 0x7FFFFFFF;
-#pragma unroll
-    for (uint32_t r = 0; r < RS; ++r)
-        if (qrow[r]) {
-            all_lo = max(all_lo, lo[r]);
-            all_hi = min(all_hi, hi[r]);
-        }
     all_lo = __reduce_max_sync(0xFFFFFFFFu, all_lo);
     all_hi = __reduce_min_sync(0xFFFFFFFFu, all_hi);
     const uint32_t tile0 = (uint32_t)min(first, last) / kDecTile, tiles = last > first ? ((uint32_t)last + kDecTile - 1u) / kDecTile - tile0 : 0u;
     const uint32_t from = tile0 + (uint32_t)((uint64_t)tiles * split / a.splits) + team;
     const uint32_t to = tile0 + (uint32_t)((uint64_t)tiles * (split + 1u) / a.splits);
 
-    const uint8_t* kq = a.kq + (size_t)hk * a.n_alloc * (D / 2) + sub * S::ROW;
-    const uint8_t* vq = a.vq + (size_t)hk * a.n_alloc * (D / 2) + sub * S::ROW;
-    const __half* kd = a.kd + (size_t)hk * a.n_alloc * (D / 32) + sub * NB;
-    const __half* vd = a.vd + (size_t)hk * a.n_alloc * (D / 32) + sub * NB;
+    // this lane's pieces of a tile: codes at rows lane / PER + 32 / PER i, the scales as one run or cell by cell
+    constexpr uint32_t PER = S::ROW / 16;                       // 16-byte pieces of a cell's codes
+    const size_t plane = (size_t)hk * a.n_alloc;
+    const uint8_t* kq = a.kq + (plane + lane / PER) * (D / 2) + sub * S::ROW + 16u * (lane % PER);
+    const uint8_t* vq = a.vq + (plane + lane / PER) * (D / 2) + sub * S::ROW + 16u * (lane % PER);
+    constexpr uint32_t DP = kDecTile * S::DS / 16;              // 16-byte pieces of a tile's scales
+    const uint8_t* ds = S::NG > 1 ? reinterpret_cast<const uint8_t*>(a.kd + (plane + lane) * (D / 32) + sub * NB)
+                                  : reinterpret_cast<const uint8_t*>((lane < DP ? a.kd : a.vd) + plane * NB) + 16u * (lane % DP);
+    const uint8_t* ds2 = S::NG > 1 ? reinterpret_cast<const uint8_t*>(a.vd + (plane + lane) * (D / 32) + sub * NB) : nullptr;
     auto fetch = [&](uint32_t tile, uint32_t stage) {
         const size_t c0 = (size_t)tile * kDecTile;
-        const uint32_t at = ring + stage * S::STAGE;
-        constexpr uint32_t PER = S::ROW / 16;                  // 16-byte pieces of a cell's codes
+        const uint32_t at = ring + stage * S::STAGE + 16u * lane;
+        const uint8_t *k = kq + c0 * (D / 2), *v = vq + c0 * (D / 2);
 #pragma unroll
         for (uint32_t i = 0; i < PER; ++i) {
-            const uint32_t p = lane + 32u * i, c = p / PER, w = p % PER;
-            cp16(at + c * S::ROW + 16u * w, kq + (c0 + c) * (D / 2) + 16u * w);
-            cp16(at + S::V_AT + c * S::ROW + 16u * w, vq + (c0 + c) * (D / 2) + 16u * w);
+            cp16(at + 512u * i, k + i * (32u / PER) * (D / 2));
+            cp16(at + S::V_AT + 512u * i, v + i * (32u / PER) * (D / 2));
         }
-        if constexpr (S::NG == 1) {                             // a tile's scales are one run
-            constexpr uint32_t P = kDecTile * S::DS / 16;       // 16 pieces (8 for D = 64)
-            if (lane < P) cp16(at + S::KD_AT + 16u * lane, reinterpret_cast<const uint8_t*>(kd + c0 * NB) + 16u * lane);
-            else if (lane < 2u * P) cp16(at + S::VD_AT + 16u * (lane - P), reinterpret_cast<const uint8_t*>(vd + c0 * NB) + 16u * (lane - P));
+        if constexpr (S::NG == 1) {
+            if (lane < 2u * DP) cp16(at + S::KD_AT, ds + c0 * S::DS);
         } else {
-            cp8(at + S::KD_AT + 8u * lane, kd + (c0 + lane) * (D / 32));
-            cp8(at + S::VD_AT + 8u * lane, vd + (c0 + lane) * (D / 32));
+            cp8(at + S::KD_AT - 8u * lane, ds + c0 * (D / 16));
+            cp8(at + S::VD_AT - 8u * lane, ds2 + c0 * (D / 16));
         }
     };
 #pragma unroll
-    for (uint32_t s = 0; s < S::STAGES - 1; ++s) {
+    for (uint32_t s = 0; s < kDecStages - 1; ++s) {
         if (from + s * S::TEAMS < to) fetch(from + s * S::TEAMS, s);
         cp_commit();
     }
 
-    // q's fragments: lane (g, t) owns values 8t .. 8t + 7 of each block of row g (and g + 8)
-    uint32_t qa[NB][2][4];
-    float start[NB][2], rs[RS];
-    {
-        float x[2][NB][8];
+    // q's fragments: lane (g, t) owns values 8t .. 8t + 7 of each block of row g (8 n + g)
+    uint32_t qb[NT][SPLIT ? 2 : 1][NB][2][2];
+    float start[NT][NB][2], rs[NT][2];
 #pragma unroll
-        for (uint32_t r = 0; r < 2; ++r)
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b)
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) x[r][b][i] = r < RS && qrow[r < RS ? r : 0] ? to_f32(qrow[r < RS ? r : 0][32u * b + 8u * t + i]) : 0.0f;
-#pragma unroll
-        for (uint32_t r = 0; r < RS; ++r) {
-            float top = 0.0f;
+    for (uint32_t n = 0; n < NT; ++n) {
+        const uint32_t row = rt * R + 8u * n + g;
+        float x[NB][8], top = 0.0f;
+        if (row < rows) {
+            const T* q = static_cast<const T*>(a.q) + (size_t)(grp * a.group + row / a.G) * a.q_stride +
+                         (size_t)(hk * a.G + row % a.G) * D + sub * S::W + 8u * t;
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[r][b][i]));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            // the row's largest value to [2^12, 2^13); rows of tiny values by 2^100 at most
-            const int e = min(12 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
-            const float f = __uint_as_float((uint32_t)(e + 127) << 23), inv = __uint_as_float((uint32_t)(127 - e) << 23);
-            rs[r] = a.scale * 1.4426950408889634f * (inv * 16777216.0f);
+                for (uint32_t i = 0; i < 8; ++i) x[b][i] = to_f32(q[32u * b + i]);
+        } else {
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) x[r][b][i] *= f;
+                for (uint32_t i = 0; i < 8; ++i) x[b][i] = 0.0f;
         }
 #pragma unroll
+        for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[b][i]));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        // the row's largest value to [2^12, 2^13); rows of tiny values by 2^100 at most
+        const int e = min(12 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
+        const float f = pow2(e), mine = a.scale * kLog2e * (pow2(-e) * 16777216.0f);
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) rs[n][i] = __shfl_sync(0xFFFFFFFFu, mine, 8u * t + 4u * i);
+#pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
-            float sum[2] = {};
-            float y[2][8];                                       // what rows 0..7 and 8..15 of the operand hold
+            float sum = 0.0f;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                y[0][i] = __half2float(__float2half_rn(x[0][b][i]));
-                if (MODE == kRows8Split) y[1][i] = __half2float(__float2half_rn(x[0][b][i] - y[0][i]));
-                else if (MODE == kRows16) y[1][i] = __half2float(__float2half_rn(x[1][b][i]));
-                else y[1][i] = 0.0f;
-                sum[0] += y[0][i];
-                sum[1] += y[1][i];
-            }
+            for (uint32_t k = 0; k < (SPLIT ? 2u : 1u); ++k) {
+                float y[8];
 #pragma unroll
-            for (uint32_t r = 0; r < 2; ++r) {
-                sum[r] += __shfl_xor_sync(0xFFFFFFFFu, sum[r], 1);
-                sum[r] += __shfl_xor_sync(0xFFFFFFFFu, sum[r], 2);
-                start[b][r] = sum[r] * (-8.0f / 16777216.0f);
+                for (uint32_t i = 0; i < 8; ++i) {
+                    if (k == 0) x[b][i] *= f;
+                    y[i] = __half2float(__float2half_rn(x[b][i]));
+                    x[b][i] -= y[i];
+                    sum += y[i];
+                }
 #pragma unroll
                 for (uint32_t j = 0; j < 2; ++j) {
-                    qa[b][j][r] = pack2(y[r][2 * j], y[r][2 * j + 4]);
-                    qa[b][j][2 + r] = pack2(y[r][2 * j + 1] * 0.0625f, y[r][2 * j + 5] * 0.0625f);
+                    qb[n][k][b][j][0] = pack2(y[2 * j], y[2 * j + 4]);
+                    qb[n][k][b][j][1] = pack2(y[2 * j + 1] * 0.0625f, y[2 * j + 5] * 0.0625f);
                 }
             }
+            sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+            sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+            sum *= -8.0f / 16777216.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) start[n][b][i] = __shfl_sync(0xFFFFFFFFu, sum, 8u * t + 4u * i);
         }
     }
 
-    float o[NB * 4][4] = {}, wsum[NB][2] = {}, m[RS], l[RS], off[RS];
-    uint32_t vexp = 1;                                           // exponent field that the weights' scale follows
+    float o[NT][NB][2][4] = {}, wsum[NT][NB][2] = {}, m[NT][2], l[NT][2], off[NT][2];
+    uint32_t vexp = 1;
 #pragma unroll
-    for (uint32_t r = 0; r < RS; ++r) {
-        m[r] = off[r] = -INFINITY;
-        l[r] = 0.0f;
-    }
-    const uint32_t pg = g ^ ((g >> 1) & 1u);                      // the cell (of eight) whose scores column g holds
-    const uint32_t c_a = (2u * t) ^ (t & 1u), c_b = c_a ^ 1u;     // the cells of this lane's columns 2t, 2t + 1
+    for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            m[n][i] = off[n][i] = -INFINITY;
+            l[n][i] = 0.0f;
+        }
+    // Cells of an eight in the order 0 1 3 2 4 5 7 6: with kv4_place, the four cells that the lanes of a column
+    // meet in V then lie in different banks, and so do the two of a K load.
+    const uint32_t pg = g ^ ((g >> 1) & 1u);                      // the cell of this lane's row of K's operand
+    const uint32_t c_a = (2u * t) ^ (t & 1u), c_b = c_a ^ 1u;     // the cells of the pair 2t, 2t + 1
+    const uint32_t k_at = pg * S::ROW + (t ^ ((pg >> 1) & 2u)) * (S::ROW / 4);
+    const uint32_t v_at = S::V_AT + c_a * S::ROW + (g ^ ((t >> 1) * 4u)) * (S::ROW / 8);
+    const int32_t v_step = c_b > c_a ? (int32_t)S::ROW : -(int32_t)S::ROW;
 
     uint32_t stage = 0, turn = 0;
     for (uint32_t tile = from; tile < to; tile += S::TEAMS) {
         {
-            const uint32_t next = tile + (S::STAGES - 1) * S::TEAMS;
-            if (next < to) fetch(next, (stage + S::STAGES - 1) % S::STAGES);
+            const uint32_t next = tile + (kDecStages - 1) * S::TEAMS;
+            if (next < to) fetch(next, stage == 0 ? kDecStages - 1 : stage - 1);
             cp_commit();
         }
         const uint32_t c0 = tile * kDecTile;
-        float mk[RS][8];
+        const bool open = !MASK && (int32_t)c0 >= all_lo && (int32_t)(c0 + kDecTile) <= all_hi;
+        // scores: index j of a lane's four cells pg + 8 j
+        float mk[NT][2][4];
         if (MASK) {
 #pragma unroll
-            for (uint32_t r = 0; r < RS; ++r)
+            for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    const uint32_t c = c0 + 8u * (j / 2) + (j & 1u ? c_b : c_a);
-                    mk[r][j] = (int32_t)c >= lo[r] && (int32_t)c < hi[r] ? __half2float(mrow[r][c]) : -INFINITY;
-                }
+                for (uint32_t i = 0; i < 2; ++i)
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const int32_t c = (int32_t)(c0 + pg + 8u * j);
+                        mk[n][i][j] = c >= lo[n][i] && c < hi[n][i] ? __half2float(mrow[n][i][c]) : -INFINITY;
+                    }
         }
-        cp_wait<S::STAGES - 1>();
+        cp_wait<kDecStages - 1>();
         __syncwarp();
         const uint8_t* sk = ringp + stage * S::STAGE;
-        float s[RS][8];
+        float s[NT][2][4];
 #pragma unroll
-        for (uint32_t nt = 0; nt < 4; ++nt) {
-            uint32_t w[4];
-            const uint8_t* p = sk + (8u * nt + pg) * S::ROW + (t ^ ((pg >> 1) & 2u)) * (S::ROW / 4);
-            if constexpr (NB == 4) {
-                const uint4 v = *reinterpret_cast<const uint4*>(p);
-                w[0] = __byte_perm(v.x, v.z, 0x5410);
-                w[1] = __byte_perm(v.x, v.z, 0x7632);
-                w[2] = __byte_perm(v.y, v.w, 0x5410);
-                w[3] = __byte_perm(v.y, v.w, 0x7632);
-            } else {
-                const uint2 v = *reinterpret_cast<const uint2*>(p);
-                w[0] = __byte_perm(v.x, v.y, 0x5410);
-                w[1] = __byte_perm(v.x, v.y, 0x7632);
+        for (uint32_t mt = 0; mt < 2; ++mt) {
+            uint32_t w[2][NB], d[2][NB / 2];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint8_t* p = sk + k_at + (16u * mt + 8u * h) * S::ROW;
+                const uint8_t* pd = sk + S::KD_AT + (16u * mt + 8u * h + pg) * S::DS;
+                if constexpr (NB == 4) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(p);
+                    w[h][0] = __byte_perm(v.x, v.z, 0x5410);
+                    w[h][1] = __byte_perm(v.x, v.z, 0x7632);
+                    w[h][2] = __byte_perm(v.y, v.w, 0x5410);
+                    w[h][3] = __byte_perm(v.y, v.w, 0x7632);
+                    const uint2 u = *reinterpret_cast<const uint2*>(pd);
+                    d[h][0] = u.x;
+                    d[h][1] = u.y;
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2*>(p);
+                    w[h][0] = __byte_perm(v.x, v.y, 0x5410);
+                    w[h][1] = __byte_perm(v.x, v.y, 0x7632);
+                    d[h][0] = *reinterpret_cast<const uint32_t*>(pd);
+                }
             }
-            uint32_t da[NB / 2], db[NB / 2];
-            const uint8_t* pd = sk + S::KD_AT + 8u * nt * S::DS;
-            if constexpr (NB == 4) {
-                const uint2 x = *reinterpret_cast<const uint2*>(pd + c_a * 8u), y = *reinterpret_cast<const uint2*>(pd + c_b * 8u);
-                da[0] = x.x; da[1] = x.y; db[0] = y.x; db[1] = y.y;
-            } else {
-                da[0] = *reinterpret_cast<const uint32_t*>(pd + c_a * 4u);
-                db[0] = *reinterpret_cast<const uint32_t*>(pd + c_b * 4u);
-            }
-            float acc[RS][2] = {};
+            float acc[NT][4] = {};
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
-                const uint32_t x = w[b], y = x >> 8;
-                float c[4] = {start[b][0], start[b][0], start[b][1], start[b][1]};
-                mma16816(c, qa[b][0][0], qa[b][0][1], qa[b][0][2], qa[b][0][3], x & 0x000F000Fu, x & 0x00F000F0u);
-                mma16816(c, qa[b][1][0], qa[b][1][1], qa[b][1][2], qa[b][1][3], y & 0x000F000Fu, y & 0x00F000F0u);
-                const float2 fa = __half22float2(as_h2(da[b / 2])), fb = __half22float2(as_h2(db[b / 2]));
-                const float ka = b & 1u ? fa.y : fa.x, kb = b & 1u ? fb.y : fb.x;
-                if (MODE == kRows8Split) {
-                    acc[0][0] = fmaf(c[0] + c[2], ka, acc[0][0]);
-                    acc[0][1] = fmaf(c[1] + c[3], kb, acc[0][1]);
-                } else {
-                    acc[0][0] = fmaf(c[0], ka, acc[0][0]);
-                    acc[0][1] = fmaf(c[1], kb, acc[0][1]);
-                    if (RS == 2) {
-                        acc[RS - 1][0] = fmaf(c[2], ka, acc[RS - 1][0]);
-                        acc[RS - 1][1] = fmaf(c[3], kb, acc[RS - 1][1]);
+                const uint32_t x0 = w[0][b], x1 = w[1][b], y0 = x0 >> 8, y1 = x1 >> 8;
+                const float2 f0 = __half22float2(as_h2(d[0][b / 2])), f1 = __half22float2(as_h2(d[1][b / 2]));
+                const float d0 = b & 1u ? f0.y : f0.x, d1 = b & 1u ? f1.y : f1.x;
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n) {
+                    float c[4];
+                    mma16816(c, x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u, qb[n][0][b][0][0], qb[n][0][b][0][1],
+                             start[n][b][0], start[n][b][1], start[n][b][0], start[n][b][1]);
+                    mma16816(c, y0 & 0x000F000Fu, y1 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x00F000F0u, qb[n][0][b][1][0], qb[n][0][b][1][1],
+                             c[0], c[1], c[2], c[3]);
+                    if constexpr (SPLIT) {
+                        mma16816(c, x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u, qb[n][1][b][0][0], qb[n][1][b][0][1],
+                                 c[0], c[1], c[2], c[3]);
+                        mma16816(c, y0 & 0x000F000Fu, y1 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x00F000F0u, qb[n][1][b][1][0], qb[n][1][b][1][1],
+                                 c[0], c[1], c[2], c[3]);
                     }
+                    acc[n][0] = fmaf(c[0], d0, acc[n][0]);
+                    acc[n][1] = fmaf(c[1], d0, acc[n][1]);
+                    acc[n][2] = fmaf(c[2], d1, acc[n][2]);
+                    acc[n][3] = fmaf(c[3], d1, acc[n][3]);
                 }
             }
 #pragma unroll
-            for (uint32_t r = 0; r < RS; ++r) {
-                s[r][2 * nt] = acc[r][0] * rs[r];
-                s[r][2 * nt + 1] = acc[r][1] * rs[r];
-            }
+            for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) {
+                    s[n][i][2 * mt] = acc[n][i] * rs[n][i];
+                    s[n][i][2 * mt + 1] = acc[n][2 + i] * rs[n][i];
+                }
         }
         if constexpr (S::NG > 1) {
             // the team's partial scores, added in the order of the groups
-            float* mine = xch + ((turn * kDecWarps + warp) * RS * 8u) * 32u + lane;
+            float* mine = xch + (turn * kDecWarps + warp) * NT * 8u * 32u + lane;
 #pragma unroll
-            for (uint32_t r = 0; r < RS; ++r)
-#pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) mine[(r * 8u + j) * 32u] = s[r][j];
+            for (uint32_t k = 0; k < NT * 8u; ++k) mine[k * 32u] = s[k / 8u][k / 4u % 2u][k % 4u];
             asm volatile("bar.sync %0, %1;" ::"r"(1u + team), "n"(32 * S::NG) : "memory");
-            const float* all = xch + ((turn * kDecWarps + team * S::NG) * RS * 8u) * 32u + lane;
+            const float* all = xch + (turn * kDecWarps + team * S::NG) * NT * 8u * 32u + lane;
 #pragma unroll
-            for (uint32_t r = 0; r < RS; ++r)
+            for (uint32_t k = 0; k < NT * 8u; ++k) {
+                float x = all[k * 32u];
 #pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    float x = all[(r * 8u + j) * 32u];
-#pragma unroll
-                    for (uint32_t k = 1; k < S::NG; ++k) x += all[(k * RS * 8u + r * 8u + j) * 32u];
-                    s[r][j] = x;
-                }
+                for (uint32_t j = 1; j < S::NG; ++j) x += all[(j * NT * 8u + k) * 32u];
+                s[k / 8u][k / 4u % 2u][k % 4u] = x;
+            }
             turn ^= 1u;
         }
-        // what a row does not see: -inf here, and no scale of V below
-        const bool open = !MASK && (int32_t)c0 >= all_lo && (int32_t)(c0 + kDecTile) <= all_hi;
-        uint32_t seen[RS];
+        // V's scales as pairs of cells, and the largest of them
+        __half2 dv[4][NB], most = __float2half2_rn(0.0f);
 #pragma unroll
-        for (uint32_t r = 0; r < RS; ++r) {
-            seen[r] = 0xFFu;
-            if (!open) {
-#pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    const int32_t c = (int32_t)(c0 + 8u * (j / 2) + (j & 1u ? c_b : c_a));
-                    const bool in = c >= lo[r] && c < hi[r] && !(MASK && mk[r][j] == -INFINITY);
-                    if (!in) seen[r] &= ~(1u << j);
-                }
-            }
-        }
-        float alpha[RS];
-        bool moved = false;
-#pragma unroll
-        for (uint32_t r = 0; r < RS; ++r) {
-            float m_old = m[r];
-            if (MASK) {
-                // the mask's running maximum is taken out first: a row of the type's lowest value keeps its scores' digits
-                float top = -INFINITY;
-#pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) top = fmaxf(top, seen[r] >> j & 1u ? mk[r][j] : -INFINITY);
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                const float off_new = fmaxf(off[r], top), base = off_new == -INFINITY ? 0.0f : off_new;
-                if (off[r] != -INFINITY && off[r] != off_new) m_old += (off[r] - base) * 1.4426950408889634f;
-                off[r] = off_new;
-#pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) s[r][j] = fmaf(mk[r][j] - base, 1.4426950408889634f, s[r][j]);
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) {
-                if (!open) s[r][j] = seen[r] >> j & 1u ? s[r][j] : -INFINITY;
-                top = fmaxf(top, s[r][j]);
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            const float m_new = fmaxf(m_old, top);
-            const float base = m_new == -INFINITY ? 0.0f : m_new;
-            alpha[r] = ex2(m_old - base);
-            moved |= m_new > m[r] || m_old != m[r];
-            m[r] = m_new;
-            l[r] *= alpha[r];
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) {
-                s[r][j] = ex2(s[r][j] - (base - 14.0f));         // 2^14 p: l and o share the factor
-                l[r] += s[r][j];
-            }
-        }
-        // V's scales as pairs (cells 2t, 2t + 1 of each eight), the largest of them, and the weights
-        __half2 dv[4][NB];
-        __half2 most = __float2half2_rn(0.0f);
-#pragma unroll
-        for (uint32_t nt = 0; nt < 4; ++nt) {
-            const uint8_t* pd = sk + S::VD_AT + 8u * nt * S::DS;
+        for (uint32_t e = 0; e < 4; ++e) {
+            const uint8_t* pd = sk + S::VD_AT + 8u * e * S::DS;
             uint32_t x[NB / 2], y[NB / 2];
             if constexpr (NB == 4) {
                 const uint2 u = *reinterpret_cast<const uint2*>(pd + c_a * 8u), v = *reinterpret_cast<const uint2*>(pd + c_b * 8u);
@@ -404,77 +390,132 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) fa4_dec_kernel(Fa4Args a) {
             }
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
-                uint32_t v = __byte_perm(x[b / 2], y[b / 2], b & 1u ? 0x7632 : 0x5410);
+                dv[e][b] = as_h2(__byte_perm(x[b / 2], y[b / 2], b & 1u ? 0x7632 : 0x5410));
+                most = __hmax2(most, __habs2(dv[e][b]));          // a NaN is passed over
+            }
+        }
+        uint32_t big = __reduce_max_sync(0xFFFFFFFFu, max(as_u32(most) & 0xFFFFu, as_u32(most) >> 16));
+        if (big >= 0x7C00u) {                                     // an infinity among them (seldom): the largest finite one
+            uint32_t x = 0;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) {
+                    const uint32_t u = as_u32(dv[e][b]) & 0x7FFF7FFFu, u0 = u & 0xFFFFu, u1 = u >> 16;
+                    x = max(x, max(u0 < 0x7C00u ? u0 : 0u, u1 < 0x7C00u ? u1 : 0u));
+                }
+            big = __reduce_max_sync(0xFFFFFFFFu, x);
+        }
+        bool moved = false;
+        float rescale = 1.0f;
+        if ((big >> 10) > vexp) {                                 // the same for the whole warp
+            const uint32_t v = big >> 10;
+            const int p = weight_exp(v) - weight_exp(vexp);
+            rescale = pow2(p + value_exp(v) - value_exp(vexp));
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n) {
+                l[n][0] *= pow2(p);
+                l[n][1] *= pow2(p);
+            }
+            vexp = v;
+            moved = rescale != 1.0f;
+        }
+        const float pexp = (float)weight_exp(vexp);
+        // running maximum and sum; what a row does not see is -inf
+        float alpha[NT][2];
+#pragma unroll
+        for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+                float (&z)[4] = s[n][i];
+                float m_old = m[n][i];
+                bool seen[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const int32_t c = (int32_t)(c0 + pg + 8u * j);
+                    seen[j] = open || (MASK ? mk[n][i][j] != -INFINITY : c >= lo[n][i] && c < hi[n][i]);
+                }
+                if (MASK) {
+                    // the mask's running maximum is taken out first: a row of the type's lowest value keeps its scores' digits
+                    float top = fmaxf(fmaxf(mk[n][i][0], mk[n][i][1]), fmaxf(mk[n][i][2], mk[n][i][3]));
+#pragma unroll
+                    for (uint32_t x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+                    const float was = off[n][i], now = fmaxf(was, top), base = now == -INFINITY ? 0.0f : now;
+                    if (was != -INFINITY && was != now) m_old += (was - base) * kLog2e;
+                    off[n][i] = now;
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) z[j] = fmaf(mk[n][i][j] - base, kLog2e, z[j]);
+                }
                 if (!open) {
-                    uint32_t any = seen[0];
-                    if (RS == 2) any |= seen[RS - 1];
-                    v &= (any >> (2 * nt) & 1u ? 0x0000FFFFu : 0u) | (any >> (2 * nt) & 2u ? 0xFFFF0000u : 0u);
-                }
-                dv[nt][b] = as_h2(v);
-                most = __hmax2(most, __habs2(dv[nt][b]));
-            }
-        }
-        {
-            const uint32_t u = as_u32(most), x = max(u & 0xFFFFu, u >> 16);
-            const uint32_t e = __reduce_max_sync(0xFFFFFFFFu, x >= 0x7C00u ? 0u : x) >> 10;
-            if (e > vexp) {                                      // the same for the whole warp
-                const float f = __uint_as_float((127u + vexp - e) << 23);
-                vexp = e;
 #pragma unroll
-                for (uint32_t r = 0; r < RS; ++r) alpha[r] *= f;
-                moved = true;                                    // l does not have this factor
+                    for (uint32_t j = 0; j < 4; ++j) z[j] = seen[j] ? z[j] : -INFINITY;
+                }
+                float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+#pragma unroll
+                for (uint32_t x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+                const float m_new = fmaxf(m_old, top), base = m_new == -INFINITY ? 0.0f : m_new, up = pexp - base;
+                alpha[n][i] = ex2(m_old - base);
+                moved |= m_new > m[n][i] || m_old != m[n][i];
+                m[n][i] = m_new;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) z[j] = ex2(z[j] + up);
+                l[n][i] = fmaf(l[n][i], alpha[n][i], (z[0] + z[1]) + (z[2] + z[3]));
             }
-        }
         if (__any_sync(0xFFFFFFFFu, moved)) {
-            const float a0 = alpha[0], a1 = MODE == kRows16 ? alpha[RS - 1] : alpha[0];
 #pragma unroll
-            for (uint32_t i = 0; i < NB * 4; ++i) {
-                o[i][0] *= a0;
-                o[i][1] *= a0;
-                o[i][2] *= a1;
-                o[i][3] *= a1;
-            }
+            for (uint32_t n = 0; n < NT; ++n) {
+                const float a0 = alpha[n][0] * rescale, a1 = alpha[n][1] * rescale;
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                wsum[b][0] *= a0;
-                wsum[b][1] *= a1;
-            }
-        }
-        const __half2 vs = __half2half2(__ushort_as_half(vexp < 30u ? (unsigned short)((30u - vexp) << 10) : (unsigned short)0x0200u));   // 2^(15 - vexp)
-        uint32_t wa[4][NB][2];                                   // the weights' operand: rows 0..7, rows 8..15
+                for (uint32_t b = 0; b < NB; ++b) {
 #pragma unroll
-        for (uint32_t nt = 0; nt < 4; ++nt) {
-            const __half2 ph = __floats2half2_rn(s[0][2 * nt], s[0][2 * nt + 1]);
-            __half2 pl;
-            if (MODE == kRows8Split) {
-                const float2 back = __half22float2(ph);
-                pl = __floats2half2_rn(s[0][2 * nt] - back.x, s[0][2 * nt + 1] - back.y);
-            } else if (MODE == kRows16) {
-                pl = __floats2half2_rn(s[RS - 1][2 * nt], s[RS - 1][2 * nt + 1]);
-            }
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                const __half2 d2 = __hmul2(dv[nt][b], vs);
-                const __half2 h = __hmul2(ph, d2);
-                wa[nt][b][0] = as_u32(h);
-                if (MODE == kRows8Split) wa[nt][b][1] = as_u32(__hfma2(pl, d2, __hfma2(ph, d2, __hneg2(h))));
-                else if (MODE == kRows16) wa[nt][b][1] = as_u32(__hmul2(pl, d2));
-                else wa[nt][b][1] = 0u;
-                if (MODE == kRows16 && !open) {
-                    // the two rows of a lane may see different cells
-                    const uint32_t k0 = seen[0] >> (2 * nt), k1 = seen[RS - 1] >> (2 * nt);
-                    wa[nt][b][0] &= (k0 & 1u ? 0x0000FFFFu : 0u) | (k0 & 2u ? 0xFFFF0000u : 0u);
-                    wa[nt][b][1] &= (k1 & 1u ? 0x0000FFFFu : 0u) | (k1 & 2u ? 0xFFFF0000u : 0u);
+                    for (uint32_t k = 0; k < 2; ++k) {
+                        o[n][b][k][0] *= a0;
+                        o[n][b][k][1] *= a1;
+                        o[n][b][k][2] *= a0;
+                        o[n][b][k][3] *= a1;
+                    }
+                    wsum[n][b][0] *= a0;
+                    wsum[n][b][1] *= a1;
                 }
             }
         }
+        if (vexp < 5u) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) dv[e][b] = __hmul2(dv[e][b], __float2half2_rn(1024.0f));
+        }
+        // the weights of each block, cells now along the lane's pairs and row g in the column
+        uint32_t wb[NT][SPLIT ? 2 : 1][4][NB];
+#pragma unroll
+        for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                const __half2 h = __floats2half2_rn(s[n][0][e], s[n][1][e]);
+                __half2 ph = as_h2(transpose8(as_u32(h))), pl;
+                if (SPLIT) {
+                    const float2 back = __half22float2(h);
+                    pl = as_h2(transpose8(pack2(s[n][0][e] - back.x, s[n][1][e] - back.y)));
+                }
+                // a cell whose weight is 0 has no part in the outputs, whatever its scale is
+                const uint32_t keep = open ? 0xFFFFFFFFu : __hne2_mask(ph, __float2half2_rn(0.0f));
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) {
+                    const __half2 x = __hmul2(ph, dv[e][b]);
+                    wb[n][0][e][b] = as_u32(x);
+                    if (SPLIT) wb[n][SPLIT ? 1 : 0][e][b] = as_u32(__hfma2(pl, dv[e][b], __hfma2(ph, dv[e][b], __hneg2(x))));
+                    if (!open) {
+                        wb[n][0][e][b] &= keep;
+                        if (SPLIT) wb[n][SPLIT ? 1 : 0][e][b] &= keep;
+                    }
+                }
+            }
 #pragma unroll
         for (uint32_t ks = 0; ks < 2; ++ks) {
-            const uint8_t* pv = sk + S::V_AT + 16u * ks * S::ROW + (g ^ ((t >> 1) * 4u)) * (S::ROW / 8);
-            uint32_t v[4][2];
+            uint32_t v[4][NB / 2];
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
-                const uint8_t* p = pv + (8u * (j >> 1) + (j & 1u ? c_b : c_a)) * S::ROW;
+                const uint8_t* p = sk + v_at + (16u * ks + 8u * (j >> 1)) * S::ROW + (j & 1u ? v_step : 0);
                 if constexpr (NB == 4) {
                     const uint2 x = *reinterpret_cast<const uint2*>(p);
                     v[j][0] = x.x;
@@ -486,99 +527,170 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) fa4_dec_kernel(Fa4Args a) {
             for (uint32_t b = 0; b < NB; ++b) {
                 const uint32_t sel = b & 1u ? 0x7632 : 0x5410;
                 const uint32_t x0 = __byte_perm(v[0][b / 2], v[1][b / 2], sel), x1 = __byte_perm(v[2][b / 2], v[3][b / 2], sel);
-                const uint32_t a0 = wa[2 * ks][b][0], a1 = wa[2 * ks][b][1], a2 = wa[2 * ks + 1][b][0], a3 = wa[2 * ks + 1][b][1];
-                mma16816(o[4 * b], a0, a1, a2, a3, x0 & 0x000F000Fu, x1 & 0x000F000Fu);
-                mma16816(o[4 * b + 1], a0, a1, a2, a3, x0 & 0x00F000F0u, x1 & 0x00F000F0u);
-                mma16816(o[4 * b + 2], a0, a1, a2, a3, (x0 >> 8) & 0x000F000Fu, (x1 >> 8) & 0x000F000Fu);
-                mma16816(o[4 * b + 3], a0, a1, a2, a3, (x0 >> 8) & 0x00F000F0u, (x1 >> 8) & 0x00F000F0u);
+                const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                    for (uint32_t k = 0; k < (SPLIT ? 2u : 1u); ++k) {
+                        const uint32_t b0 = wb[n][k][2 * ks][b], b1 = wb[n][k][2 * ks + 1][b];
+                        float (&p)[4] = o[n][b][0];
+                        mma16816(p, x0 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x000F000Fu, x1 & 0x00F000F0u, b0, b1, p[0], p[1], p[2], p[3]);
+                        float (&q)[4] = o[n][b][1];
+                        mma16816(q, y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u, b0, b1, q[0], q[1], q[2], q[3]);
+                    }
             }
         }
 #pragma unroll
-        for (uint32_t b = 0; b < NB; ++b) {
-            float c[4] = {};
-            mma16816(c, wa[0][b][0], wa[0][b][1], wa[1][b][0], wa[1][b][1], 0x00080008u, 0x00080008u);
-            mma16816(c, wa[2][b][0], wa[2][b][1], wa[3][b][0], wa[3][b][1], 0x00080008u, 0x00080008u);
-            wsum[b][0] += c[0];
-            wsum[b][1] += c[2];
-        }
-        stage = (stage + 1u) % S::STAGES;
+        for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                constexpr uint32_t k8 = 0x00080008u;
+                float c[4];
+                mma16816(c, k8, k8, k8, k8, wb[n][0][0][b], wb[n][0][1][b], 0.0f, 0.0f, 0.0f, 0.0f);
+                mma16816(c, k8, k8, k8, k8, wb[n][0][2][b], wb[n][0][3][b], c[0], c[1], c[2], c[3]);
+                if constexpr (SPLIT) {
+                    mma16816(c, k8, k8, k8, k8, wb[n][1][0][b], wb[n][1][1][b], c[0], c[1], c[2], c[3]);
+                    mma16816(c, k8, k8, k8, k8, wb[n][1][2][b], wb[n][1][3][b], c[0], c[1], c[2], c[3]);
+                }
+                wsum[n][b][0] += c[0];
+                wsum[n][b][1] += c[1];
+            }
+        stage = stage + 1u == kDecStages ? 0u : stage + 1u;
         __syncwarp();                                            // the tile is read: its stage may be filled
     }
     cp_wait<0>();
     __syncwarp();
 
-    // the warp's results in its ring: [R][W] outputs; 2^14 and 2^(15 - vexp) and 2^-24 (2^-20) are undone here
+    // the warp's results in its ring: [R][W] outputs without their scales; maxima and sums beside the rings
     float* wo = reinterpret_cast<float*>(ringp);
-    const float unscale = __uint_as_float((127u + 24u + vexp - 15u) << 23);
+    const float unscale = pow2(24 - value_exp(vexp)), pinv = pow2(-weight_exp(vexp));
 #pragma unroll
-    for (uint32_t b = 0; b < NB; ++b)
+    for (uint32_t n = 0; n < NT; ++n) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            const float f = i & 1u ? unscale * 0.0625f : unscale, k = i & 1u ? 16.0f : 1.0f;
-            const float* c = o[4 * b + i];
-            const uint32_t d0 = 32u * b + 8u * t + i;             // columns 2t, 2t + 1: chunks 2t, 2t + 1
-            if (MODE == kRows8Split) {
-                const float ws = (wsum[b][0] + wsum[b][1]) * k;
-                wo[g * S::W + d0] = ((c[0] + c[2]) - ws) * f;
-                wo[g * S::W + d0 + 4] = ((c[1] + c[3]) - ws) * f;
-            } else {
-                wo[g * S::W + d0] = (c[0] - wsum[b][0] * k) * f;
-                wo[g * S::W + d0 + 4] = (c[1] - wsum[b][0] * k) * f;
-                if (MODE == kRows16) {
-                    wo[(g + 8u) * S::W + d0] = (c[2] - wsum[b][1] * k) * f;
-                    wo[(g + 8u) * S::W + d0 + 4] = (c[3] - wsum[b][1] * k) * f;
+        for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+            for (uint32_t k = 0; k < 2; ++k)
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) {
+                    float* p = wo + (8u * n + 2u * t + i) * S::W + 32u * b + 4u * g + 2u * k;
+                    p[0] = (o[n][b][k][i] - wsum[n][b][i]) * (unscale * pinv);
+                    p[1] = (o[n][b][k][2 + i] * 0.0625f - wsum[n][b][i]) * (unscale * pinv);
                 }
-            }
-        }
 #pragma unroll
-    for (uint32_t r = 0; r < RS; ++r) {
-        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
-        if (t == 0) {
-            float* p = red + (warp * 16u + g + 8u * r) * 3u;
-            p[0] = MASK ? off[r] : 0.0f;
-            p[1] = m[r];
-            p[2] = l[r];
+        for (uint32_t i = 0; i < 2; ++i) {
+            float x = l[n][i] * pinv;
+#pragma unroll
+            for (uint32_t k = 4; k < 32; k <<= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, k);
+            if (g == 0) {
+                float* p = red + (warp * 16u + 8u * n + 2u * t + i) * 3u;
+                p[0] = MASK ? off[n][i] : 0.0f;
+                p[1] = m[n][i];
+                p[2] = x;
+            }
         }
     }
     __syncthreads();
-    // the CTA's teams, added in order; then the output, or the split's share of it
+    // the CTA's teams, added in order, into the first team's place
+    auto result = [&](uint32_t j, uint32_t r, uint32_t d) {
+        return reinterpret_cast<float*>(sm + (j * S::NG + d / S::W) * S::RING) + r * S::W + d % S::W;
+    };
+    float* fin = red + kDecWarps * 16u * 3u;
     for (uint32_t e = tid; e < R * D; e += kDecWarps * 32u) {
-        const uint32_t r = e / D, d = e % D, row = rt * R + r;
-        if (row >= rows) continue;
-        float ot = -INFINITY, mt = -INFINITY, lt = 0.0f, acc = 0.0f;
+        const uint32_t r = e / D, d = e % D;
+        float ot = -INFINITY, mt = -INFINITY, lt = 0.0f, acc = 0.0f, sh[S::TEAMS];
 #pragma unroll
         for (uint32_t j = 0; j < S::TEAMS; ++j) ot = fmaxf(ot, red[(j * S::NG * 16u + r) * 3u]);
-        float sh[S::TEAMS];
 #pragma unroll
         for (uint32_t j = 0; j < S::TEAMS; ++j) {
             const float* p = red + (j * S::NG * 16u + r) * 3u;
-            sh[j] = p[1] == -INFINITY ? -INFINITY : MASK ? p[1] + (p[0] - ot) * 1.4426950408889634f : p[1];
+            sh[j] = !MASK || p[0] == ot || p[1] == -INFINITY ? p[1] : p[1] + (p[0] - ot) * kLog2e;
             mt = fmaxf(mt, sh[j]);
         }
         const float base = mt == -INFINITY ? 0.0f : mt;
 #pragma unroll
         for (uint32_t j = 0; j < S::TEAMS; ++j) {
-            const float* p = red + (j * S::NG * 16u + r) * 3u;
+            const float lj = red[(j * S::NG * 16u + r) * 3u + 2u];
+            if (lj == 0.0f) continue;                            // a team that saw nothing of the row
             const float f = ex2(sh[j] - base);
-            if (p[2] == 0.0f) continue;                          // a team that saw nothing of the row
-            lt += f * p[2];
-            acc += f * reinterpret_cast<const float*>(sm + (j * S::NG + d / S::W) * S::RING)[r * S::W + d % S::W];
+            lt += f * lj;
+            acc += f * *result(j, r, d);
         }
-        if (a.splits == 1u) {
-            const uint32_t tok = grp * a.group + row / a.G, h = hk * a.G + row % a.G;
-            static_cast<T*>(a.out)[(size_t)tok * a.out_stride + (size_t)h * D + d] = from_f32<T>(lt == 0.0f ? 0.0f : acc / lt);
-        } else {
-            const size_t at = ((size_t)unit * a.splits + split) * R + r;
-            a.part_o[at * D + d] = acc;
-            if (d == 0) *reinterpret_cast<float4*>(a.part_ml + at * 4u) = make_float4(ot, mt, lt, 0.0f);
+        *result(0, r, d) = acc;
+        if (d == 0) {
+            fin[r * 3u] = ot;
+            fin[r * 3u + 1u] = mt;
+            fin[r * 3u + 2u] = lt;
         }
     }
+    __syncthreads();
+    if (a.splits > 1u && a.part_o) {                             // joined by the merge kernel
+        for (uint32_t e = tid; e < R * D; e += kDecWarps * 32u) {
+            const uint32_t r = e / D, d = e % D;
+            if (rt * R + r >= rows) break;
+            const size_t at = ((size_t)unit * a.splits + split) * R + r;
+            a.part_o[at * D + d] = *result(0, r, d);
+            if (d == 0) *reinterpret_cast<float4*>(a.part_ml + at * 4u) = make_float4(fin[r * 3u], fin[r * 3u + 1u], fin[r * 3u + 2u], 0.0f);
+        }
+        return;
+    }
+    // the cluster's CTAs, added in order: each finishes its share of the outputs
+    const uint32_t used = min(R, rows - rt * R);
+    float* share = xch;                                          // [R][splits + 1]: each CTA's factor, then 1 / sum
+    if (a.splits > 1u) {
+        cluster_sync();
+        // a half warp per row, a lane per CTA
+        for (uint32_t e = tid; e < R * kMaxCluster; e += kDecWarps * 32u) {
+            const uint32_t r = e / kMaxCluster, k = e % kMaxCluster;
+            float ot = -INFINITY, mt = -INFINITY, lt = 0.0f;
+            if (k < a.splits) {
+                if (MASK) ot = remote_f32(fin + r * 3u, k);
+                mt = remote_f32(fin + r * 3u + 1u, k);
+                lt = remote_f32(fin + r * 3u + 2u, k);
+            }
+            if (MASK) {
+                float top = ot;
+#pragma unroll
+                for (uint32_t x = 1; x < kMaxCluster; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+                if (ot != top && mt != -INFINITY) mt += (ot - top) * kLog2e;
+            }
+            float top = mt;
+#pragma unroll
+            for (uint32_t x = 1; x < kMaxCluster; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+            const float f = lt == 0.0f ? 0.0f : ex2(mt - (top == -INFINITY ? 0.0f : top));
+            float sum = lt == 0.0f ? 0.0f : f * lt;
+#pragma unroll
+            for (uint32_t x = 1; x < kMaxCluster; x <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+            share[r * (kMaxCluster + 1u) + k] = f;
+            if (k == 0) share[r * (kMaxCluster + 1u) + kMaxCluster] = sum;
+        }
+        __syncthreads();
+    }
+    for (uint32_t e = split * kDecWarps * 32u + tid; e < used * D; e += a.splits * kDecWarps * 32u) {
+        const uint32_t r = e / D, d = e % D, row = rt * R + r;
+        float lt, acc;
+        if (a.splits == 1u) {
+            lt = fin[r * 3u + 2u];
+            acc = *result(0, r, d);
+        } else {
+            const float* f = share + r * (kMaxCluster + 1u);
+            float x[kMaxCluster];
+#pragma unroll
+            for (uint32_t k = 0; k < kMaxCluster; ++k) x[k] = k < a.splits ? remote_f32(result(0, r, d), k) : 0.0f;
+            lt = f[kMaxCluster];
+            acc = 0.0f;
+#pragma unroll
+            for (uint32_t k = 0; k < kMaxCluster; ++k) acc += f[k] == 0.0f ? 0.0f : f[k] * x[k];
+        }
+        const uint32_t tok = grp * a.group + row / a.G, h = hk * a.G + row % a.G;
+        static_cast<T*>(a.out)[(size_t)tok * a.out_stride + (size_t)h * D + d] = from_f32<T>(lt == 0.0f ? 0.0f : acc / lt);
+    }
+    if (a.splits > 1u) cluster_sync();                           // nobody's shared memory goes while it is read
 }
 
 // Adds up the splits of each row in order. One CTA per row of a unit.
 template <class T, int D, uint32_t R>
 __global__ void __launch_bounds__(128) fa4_merge_kernel(Fa4Args a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t unit = blockIdx.x, r = blockIdx.y;
     const uint32_t hk = unit % a.n_head_kv, rt = unit / a.n_head_kv % a.row_tiles, grp = unit / (a.n_head_kv * a.row_tiles);
     const uint32_t row = rt * R + r;
@@ -586,22 +698,25 @@ __global__ void __launch_bounds__(128) fa4_merge_kernel(Fa4Args a) {
     const float4* ml = reinterpret_cast<const float4*>(a.part_ml) + (size_t)unit * a.splits * R + r;
     const float* po = a.part_o + ((size_t)unit * a.splits * R + r) * D;
     float ot = -INFINITY, mt = -INFINITY, lt = 0.0f;
-    for (uint32_t s = 0; s < a.splits; ++s) ot = fmaxf(ot, ml[(size_t)s * R].x);
-    for (uint32_t s = 0; s < a.splits; ++s) {
-        const float4 p = ml[(size_t)s * R];
-        if (p.y != -INFINITY) mt = fmaxf(mt, p.x == ot ? p.y : p.y + (p.x - ot) * 1.4426950408889634f);
-    }
+    for (uint32_t s = threadIdx.x & 31u; s < a.splits; s += 32u) ot = fmaxf(ot, ml[(size_t)s * R].x);
+    for (int x = 16; x; x >>= 1) ot = fmaxf(ot, __shfl_xor_sync(0xFFFFFFFFu, ot, x));
+    auto level = [&](const float4& p) { return p.x == ot || p.y == -INFINITY ? p.y : p.y + (p.x - ot) * kLog2e; };
+    for (uint32_t s = threadIdx.x & 31u; s < a.splits; s += 32u) mt = fmaxf(mt, level(ml[(size_t)s * R]));
+    for (int x = 16; x; x >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, x));
     const float base = mt == -INFINITY ? 0.0f : mt;
     constexpr uint32_t N = D / 128 ? D / 128 : 1;
     float acc[N] = {};
+#pragma unroll 8
     for (uint32_t s = 0; s < a.splits; ++s) {
         const float4 p = ml[(size_t)s * R];
-        if (p.z == 0.0f) continue;
-        const float f = ex2((p.x == ot ? p.y : p.y + (p.x - ot) * 1.4426950408889634f) - base);
-        lt += f * p.z;
+        const float f = p.z == 0.0f ? 0.0f : ex2(level(p) - base);
+        if (p.z != 0.0f) lt += f * p.z;
 #pragma unroll
         for (uint32_t k = 0; k < N; ++k)
-            if (threadIdx.x + 128u * k < D) acc[k] += f * po[(size_t)s * R * D + threadIdx.x + 128u * k];
+            if (threadIdx.x + 128u * k < D) {
+                const float x = po[(size_t)s * R * D + threadIdx.x + 128u * k];
+                if (p.z != 0.0f) acc[k] += f * x;
+            }
     }
     const uint32_t tok = grp * a.group + row / a.G, h = hk * a.G + row % a.G;
     T* out = static_cast<T*>(a.out) + (size_t)tok * a.out_stride + (size_t)h * D;
@@ -614,7 +729,7 @@ __global__ void __launch_bounds__(128) fa4_merge_kernel(Fa4Args a) {
 struct Fa4Plan {
     int mode;
     uint32_t group, row_tiles, units, splits;
-    size_t o_bytes, ml_bytes;
+    size_t o_bytes, ml_bytes;                  // of the workspace, where a merge kernel joins the splits
 };
 
 Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint32_t n_head, uint32_t n_kv, uint32_t group, uint32_t max_len) {
@@ -627,12 +742,14 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
     p.units = (T / p.group) * n_head_kv * p.row_tiles;
     const uint32_t len = max_len && max_len < n_kv ? max_len : n_kv;
     const uint32_t teams = D <= 128u ? kDecWarps : kDecWarps * 128u / D;
-    // split until the CTAs fill the GPU once, each warp keeping at least two tiles
-    const uint32_t most = (len / kDecTile + 1u + 2u * teams - 1u) / (2u * teams);
-    p.splits = p.units ? kDecCtas / p.units : 1u;
-    if (p.splits > most) p.splits = most;
-    if (p.splits < 1u) p.splits = 1u;
-    if (p.splits > 1u) {
+    // Splits until the CTAs fill the GPU twice over, in powers of two up to a cluster's CTAs, each warp keeping a
+    // tile at least; where even clusters of sixteen leave most SMs empty and the cells are many, more splits and
+    // a merge kernel.
+    const uint32_t most = (len / kDecTile + 1u) / teams;
+    p.splits = 1;
+    while (p.splits < kMaxCluster && p.splits * 2u <= most && p.units * p.splits < 2u * kDecCtas) p.splits *= 2u;
+    if (p.units * kMaxCluster < kSms && most >= 8u * kMaxCluster) {
+        p.splits = 2u * kSms / p.units;
         p.o_bytes = (size_t)p.units * p.splits * R * D * 4u;
         p.ml_bytes = (size_t)p.units * p.splits * R * 16u;
     }
@@ -642,13 +759,38 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
 template <class T, int D, int MODE, bool MASK>
 cudaError_t dec_launch_m(const Fa4Args& a, uint32_t units, cudaStream_t st) {
     constexpr uint32_t smem = dec_smem<D, MODE>();
-    cudaError_t e = cudaFuncSetAttribute(fa4_dec_kernel<T, D, MODE, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static bool done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    fa4_dec_kernel<T, D, MODE, MASK><<<dim3(units, a.splits), kDecWarps * 32, smem, st>>>(a);
-    e = cudaGetLastError();
-    if (e != cudaSuccess || a.splits == 1u) return e;
-    fa4_merge_kernel<T, D, kRowsOf<MODE>><<<dim3(units, kRowsOf<MODE>), 128, 0, st>>>(a);
-    return cudaGetLastError();
+    if (dev >= 64 || !done[dev]) {             // the kernel's attributes, set once per device
+        e = cudaFuncSetAttribute(fa4_dec_kernel<T, D, MODE, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(fa4_dec_kernel<T, D, MODE, MASK>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) done[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(units * a.splits);
+    cfg.blockDim = dim3(kDecWarps * 32u);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    if (a.splits > 1u && !a.part_o) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = a.splits;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.numAttrs = 1;
+    }
+    e = cudaLaunchKernelEx(&cfg, fa4_dec_kernel<T, D, MODE, MASK>, a);
+    if (e != cudaSuccess || !a.part_o) return e;
+    cfg.gridDim = dim3(units, kRowsOf<MODE>);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fa4_merge_kernel<T, D, kRowsOf<MODE>>, a);
 }
 template <class T, int D, int MODE>
 cudaError_t dec_launch(const Fa4Args& a, uint32_t units, cudaStream_t st) {
@@ -744,8 +886,10 @@ int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const v
     a.group = p.group;
     a.row_tiles = p.row_tiles;
     a.splits = p.splits;
-    a.part_o = static_cast<float*>(ws);
-    a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.o_bytes);
+    if (p.o_bytes) {
+        a.part_o = static_cast<float*>(ws);
+        a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.o_bytes);
+    }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (type == TSRC_TYPE_F32) e = dec_launch_d<float, kRows8Split>(a, kv->D, p.units, st);

@@ -31,11 +31,11 @@ Kv4Planes planes_of(const tsrc_kv4* kv) {
     return p;
 }
 
-// The unit of storing and reading is a chunk: lane g of eight owns values 4g .. 4g + 3 of each of NB blocks (NB = 4
-// for a 128-value group, 2 where D = 64), so the eight lanes of a unit cover NB x 32 neighbouring values, read or
-// write whole 64 / 128-byte lines of the rows and leave NB x 2 bytes of codes each.
+// The unit of storing and reading is a lane t of four that share NB blocks (NB = 4 for a 128-value group, 2 where
+// D = 64): values 8t .. 8t + 7 of each, the two neighbouring chunks 2t and 2t + 1 of the codes. The four lanes read
+// or write whole 64 / 128-byte lines of the rows and 16 (8) bytes of codes each.
 struct Kv4Unit {
-    uint32_t head, group, g;    // group: of NB * 32 values inside the head
+    uint32_t head, group, t;    // group: of NB * 32 values inside the head
     uint32_t value;             // the unit's first value in the row of E, + 32 b for block b
 };
 
@@ -43,11 +43,11 @@ template <uint32_t NB>
 __device__ __forceinline__ Kv4Unit unit_of(uint32_t u, uint32_t D) {
     Kv4Unit r;
     const uint32_t per_head = D / (NB * 32u);
-    r.g = u & 7u;
-    const uint32_t grp = u >> 3;
+    r.t = u & 3u;
+    const uint32_t grp = u >> 2;
     r.head = grp / per_head;
     r.group = grp - r.head * per_head;
-    r.value = grp * NB * 32u + 4u * r.g;
+    r.value = grp * NB * 32u + 8u * r.t;
     return r;
 }
 
@@ -55,58 +55,114 @@ __device__ __forceinline__ int64_t cell_of(const int64_t* cells, uint32_t cell0,
     return cells ? cells[i] : (int64_t)cell0 + i;
 }
 
-// Rows -> blocks. The largest magnitude of a block is an unsigned maximum of the magnitudes' bits over its eight
-// lanes (a NaN counts as 0); its sign is that of the first value that has it, found by a ballot.
+// Where chunks 2t and 2t + 1 of a group lie, in bytes from the group's row (kv4_place keeps such pairs together).
+template <uint32_t NB>
+__device__ __forceinline__ uint32_t pair_at(uint32_t t, size_t cell) { return kv4_place(2u * t, cell) * (NB * 2u); }
+
+// The codes of eight values of a block by the format's own steps, whatever they are (zeros, NaN, infinities, scales
+// below f32's normal numbers, largest values of either sign): every lane of the warp comes here together.
+__device__ __forceinline__ void kv4_block_any(const float (&x)[8], uint32_t& lo, uint32_t& hi, float& d) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t mag[8], top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        mag[j] = __float_as_uint(x[j]) & 0x7FFFFFFFu;
+        if (mag[j] > 0x7F800000u) mag[j] = 0u;                   // a NaN does not count
+        top = max(top, mag[j]);
+    }
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    uint32_t sign = 0;
+    bool has = false;
+#pragma unroll
+    for (int j = 7; j >= 0; --j)
+        if (mag[j] == top && x[j] == x[j]) {
+            has = true;
+            sign = __float_as_uint(x[j]) & 0x80000000u;
+        }
+    const uint32_t first = __ffs((__ballot_sync(0xFFFFFFFFu, has) >> (lane & 28u)) & 0xFu);
+    sign = __shfl_sync(0xFFFFFFFFu, sign, (lane & 28u) | ((first - 1u) & 3u));
+    d = (top ? __uint_as_float(top | sign) : 0.0f) * -0.125f;
+    const float id = d != 0.0f ? __frcp_rn(d) : 0.0f;
+    lo = hi = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float z = __fadd_rn(__fmul_rn(x[j], id), 8.5f);
+        const uint32_t c = z == z ? (uint32_t)fminf(fmaxf(z, 0.0f), 15.0f) : 8u;
+        if (j < 4) lo |= c << (4 * j);
+        else hi |= c << (4 * (j - 4));
+    }
+}
+
+// max and min that keep a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Four codes z = x id + 8.5 (0.5 <= z < 17) cut to 0..15: z + 2^23 rounded down has the code in its last bits, and
+// four such words, weighted 1, 16, 256, 4096, add up to the 16 bits and a constant.
+__device__ __forceinline__ uint32_t pack4(const float* x, float id) {
+    uint32_t acc = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float z = fminf(__fadd_rn(__fmul_rn(x[j], id), 8.5f), 15.5f);
+        acc += __float_as_uint(__fadd_rd(z, 8388608.0f)) << (4 * j);
+    }
+    return acc - 0x4B000000u * 0x1111u;
+}
+
+// Rows -> blocks. The block's first value of largest magnitude is its maximum or its minimum, so two maxima over
+// the eight values and two shuffles each find it; where they tie in magnitude (the first decides), or the block
+// has no ordinary scale, the warp takes the general steps.
+// 8192 rows of 1024 bf16 values, K and V (33.6 MB in, 9.4 out): 24.8 us with eight lanes a block, magnitudes and
+// signs by value and 64-bit divisions; 13.7 us so.
 template <class T, uint32_t NB, bool VEC>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const T* __restrict__ k, const T* __restrict__ v, uint32_t n, size_t row_stride,
                                                         const int64_t* cells, uint32_t cell0, Kv4Planes p) {
-    const uint32_t per_row = p.n_head_kv * p.D / (NB * 4u);
-    const size_t t = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const uint32_t i0 = (uint32_t)(t / per_row);
-    const bool live = i0 < n;                                   // whole groups of eight lanes live or not
+    const uint32_t per_row = p.n_head_kv * p.D / (NB * 8u);
+    const uint32_t t = blockIdx.x * blockDim.x + threadIdx.x;
+    const uint32_t i0 = t / per_row;
+    const bool live = i0 < n;                                   // whole groups of four lanes live or not
     const uint32_t i = live ? i0 : n - 1u;
     const uint32_t which = blockIdx.y + (k ? 0u : 1u);
-    const Kv4Unit u = unit_of<NB>((uint32_t)(t - (size_t)i0 * per_row), p.D);
+    const Kv4Unit u = unit_of<NB>(t - i0 * per_row, p.D);
     const int64_t cell = cell_of(cells, cell0, i);
     const bool inside = cell >= 0 && cell < (int64_t)p.n_cells;
     const T* row = (which ? v : k) + (size_t)i * row_stride + u.value;
-    float x[NB][4];
+    float x[NB][8];
 #pragma unroll
-    for (uint32_t b = 0; b < NB; ++b) load4<T, VEC>(row + 32u * b, x[b]);
-    uint32_t code[NB];
+    for (uint32_t b = 0; b < NB; ++b) load8<T, VEC>(row + 32u * b, x[b]);
+    uint32_t lo[NB], hi[NB];
     float d[NB];
-    const uint32_t lane = threadIdx.x & 31u;
 #pragma unroll
     for (uint32_t b = 0; b < NB; ++b) {
-        uint32_t mag[4], top = 0;
+        float up = x[b][0], down = x[b][0];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            mag[j] = __float_as_uint(x[b][j]) & 0x7FFFFFFFu;
-            if (mag[j] > 0x7F800000u) mag[j] = 0u;
-            top = max(top, mag[j]);
+        for (int j = 1; j < 8; ++j) {
+            up = max_nan(up, x[b][j]);
+            down = min_nan(down, x[b][j]);
         }
 #pragma unroll
-        for (int s = 1; s < 8; s <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
-        uint32_t sign = 0;
-        bool has = false;
-#pragma unroll
-        for (int j = 3; j >= 0; --j)
-            if (mag[j] == top && x[b][j] == x[b][j]) {
-                has = true;
-                sign = __float_as_uint(x[b][j]) & 0x80000000u;
-            }
-        const uint32_t first = __ffs((__ballot_sync(0xFFFFFFFFu, has) >> (lane & 24u)) & 0xFFu);
-        sign = __shfl_sync(0xFFFFFFFFu, sign, (lane & 24u) | ((first - 1u) & 7u));
-        const float m = top ? __uint_as_float(top | sign) : 0.0f;
-        d[b] = m * -0.125f;                                     // m / -8: a power of two
-        const float id = d[b] != 0.0f ? __frcp_rn(d[b]) : 0.0f;
-        code[b] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float z = __fadd_rn(__fmul_rn(x[b][j], id), 8.5f);
-            const uint32_t c = z == z ? (uint32_t)fminf(fmaxf(z, 0.0f), 15.0f) : 8u;
-            code[b] |= c << (4 * j);
+        for (int s = 1; s < 4; s <<= 1) {
+            up = max_nan(up, __shfl_xor_sync(0xFFFFFFFFu, up, s));
+            down = min_nan(down, __shfl_xor_sync(0xFFFFFFFFu, down, s));
         }
+        const float big = fabsf(up) > fabsf(down) ? up : down;
+        const bool plain = up + down != 0.0f && fabsf(big) >= 1e-30f && fabsf(big) < INFINITY;       // false for NaN
+        d[b] = big * -0.125f;                                   // m / -8: a power of two
+        if (__all_sync(0xFFFFFFFFu, plain)) {
+            const float id = __frcp_rn(d[b]);
+            lo[b] = pack4(x[b], id);
+            hi[b] = pack4(x[b] + 4, id);
+        } else
+            kv4_block_any(x[b], lo[b], hi[b], d[b]);
     }
     if (!live) return;
     if (!inside) {
@@ -114,54 +170,64 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const T* __restrict__ k,
         return;
     }
     const size_t hc = (size_t)u.head * p.n_alloc + (size_t)cell;
-    uint8_t* q = p.q[which] + hc * (p.D / 2u) + u.group * (NB * 16u) + kv4_place(u.g, (size_t)cell) * (NB * 2u);
-    if constexpr (NB == 4) *reinterpret_cast<uint2*>(q) = make_uint2(code[0] | (code[1] << 16), code[2] | (code[3] << 16));
-    else *reinterpret_cast<uint32_t*>(q) = code[0] | (code[1] << 16);
-    if (u.g < NB) {
+    uint8_t* q = p.q[which] + hc * (p.D / 2u) + u.group * (NB * 16u) + pair_at<NB>(u.t, (size_t)cell);
+    if constexpr (NB == 4)
+        *reinterpret_cast<uint4*>(q) = make_uint4(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16), hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
+    else *reinterpret_cast<uint2*>(q) = make_uint2(lo[0] | (lo[1] << 16), hi[0] | (hi[1] << 16));
+    if (u.t < NB) {
         float db = d[0];
 #pragma unroll
         for (uint32_t b = 1; b < NB; ++b)
-            if (u.g == b) db = d[b];
-        p.d[which][hc * (p.D / 32u) + u.group * NB + u.g] = __float2half_rn(db);
+            if (u.t == b) db = d[b];
+        p.d[which][hc * (p.D / 32u) + u.group * NB + u.t] = __float2half_rn(db);
     }
 }
 
-// Blocks -> rows. d (n - 8) has at most 15 significant bits: the f32 product is exact, so the result is rounded once.
+// Blocks -> rows. n - 8 comes from fp16 arithmetic without rounding (n + 1024 is an fp16 whose last bits are n).
+// d (n - 8) has at most 15 significant bits: the f32 product is exact, and so is an fp16 product before its one
+// rounding.
+// 131072 cells of 1024 values to fp16, K and V (151 MB in, 537 out): 181 us with eight lanes a group, 128 us so (5.4 TB/s).
 template <class T, uint32_t NB, bool VEC>
 __global__ void __launch_bounds__(256) kv4_read_kernel(T* __restrict__ k, T* __restrict__ v, uint32_t n, size_t row_stride,
                                                        const int64_t* cells, uint32_t cell0, Kv4Planes p) {
-    const uint32_t per_row = p.n_head_kv * p.D / (NB * 4u);
-    const size_t t = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const uint32_t i = (uint32_t)(t / per_row);
+    const uint32_t per_row = p.n_head_kv * p.D / (NB * 8u);
+    const uint32_t t = blockIdx.x * blockDim.x + threadIdx.x;
+    const uint32_t i = t / per_row;
     if (i >= n) return;
     const uint32_t which = blockIdx.y + (k ? 0u : 1u);
-    const Kv4Unit u = unit_of<NB>((uint32_t)(t - (size_t)i * per_row), p.D);
+    const Kv4Unit u = unit_of<NB>(t - i * per_row, p.D);
     const int64_t cell = cell_of(cells, cell0, i);
     if (cell < 0 || cell >= (int64_t)p.n_cells) {
         if (u.value == 0) atomicOr(&g_kv4_error, kKv4ErrGet);
         return;
     }
     const size_t hc = (size_t)u.head * p.n_alloc + (size_t)cell;
-    const uint8_t* q = p.q[which] + hc * (p.D / 2u) + u.group * (NB * 16u) + kv4_place(u.g, (size_t)cell) * (NB * 2u);
+    const uint8_t* q = p.q[which] + hc * (p.D / 2u) + u.group * (NB * 16u) + pair_at<NB>(u.t, (size_t)cell);
     const __half* ds = p.d[which] + hc * (p.D / 32u) + u.group * NB;
-    uint32_t w[NB / 2], s[NB / 2];
+    uint32_t w[NB], s[NB / 2];                                  // w: two blocks' values 8t .. + 3, then 8t + 4 .. + 7
     if constexpr (NB == 4) {
-        const uint2 a = *reinterpret_cast<const uint2*>(q), c = *reinterpret_cast<const uint2*>(ds);
-        w[0] = a.x; w[1] = a.y;
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(q));
+        const uint2 c = *reinterpret_cast<const uint2*>(ds);
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
         s[0] = c.x; s[1] = c.y;
     } else {
-        w[0] = *reinterpret_cast<const uint32_t*>(q);
+        const uint2 a = __ldcs(reinterpret_cast<const uint2*>(q));
+        w[0] = a.x; w[1] = a.y;
         s[0] = *reinterpret_cast<const uint32_t*>(ds);
     }
     T* row = (which ? v : k) + (size_t)i * row_stride + u.value;
 #pragma unroll
     for (uint32_t b = 0; b < NB; ++b) {
-        const uint32_t c = w[b / 2] >> (16u * (b & 1u));
-        const float d = __half2float(__ushort_as_half((unsigned short)(s[b / 2] >> (16u * (b & 1u)))));
-        float x[4];
+        // the block's halves side by side: codes i and i + 4 of the eight in the two halves of a word
+        const uint32_t c = __byte_perm(w[b / 2], w[NB / 2 + b / 2], b & 1u ? 0x7632 : 0x5410);
+        const __half d = __ushort_as_half((unsigned short)(s[b / 2] >> (16u * (b & 1u))));
+        __half2 x[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = d * (float)((int)((c >> (4 * j)) & 15u) - 8);
-        store4<T, VEC>(row + 32u * b, x);
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t bits = ((c >> (4 * j)) & 0x000F000Fu) | 0x64006400u;
+            x[j] = __hsub2(*reinterpret_cast<const __half2*>(&bits), __float2half2_rn(1032.0f));
+        }
+        store8<T, VEC>(row + 32u * b, x, d);
     }
 }
 
@@ -211,18 +277,11 @@ __global__ void kv4_to_ggml_kernel(uint8_t* ggml, uint32_t n, uint32_t cell0, ui
 // need not be 16-byte aligned where a sequence starts). swap: the bit of a unit's index that the chunks' places
 // flip (kv4_place) where the cell has its bit 2 set: half a group's units for codes, 0 for scales.
 template <class U, uint32_t NBEAM>
-__global__ void __launch_bounds__(256) kv4_reorder_kernel(U* a, U* b, uint32_t units_cell, uint32_t swap, uint32_t n_alloc,
-                                                          const int32_t* parent, uint32_t n_beam, uint32_t cell0, uint32_t seq_stride,
-                                                          uint32_t n) {
-    const uint32_t group = blockIdx.y, head = blockIdx.z >> 1;
-    U* plane = ((blockIdx.z & 1u) ? b : a) + (size_t)head * n_alloc * units_cell;
-    const size_t j = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int32_t* par = parent + (size_t)group * n_beam;
-    if (j >= (size_t)n * units_cell) return;
+__device__ __forceinline__ void reorder_unit(U* plane, size_t j, uint32_t units_cell, uint32_t swap, const int32_t* par, uint32_t n_beam,
+                                             size_t first, uint32_t seq_stride) {
     const uint32_t i = (uint32_t)(j / units_cell), unit = (uint32_t)(j - (size_t)i * units_cell);
-    const size_t first = (size_t)cell0 + (size_t)group * n_beam * seq_stride + i;
     auto at = [&](uint32_t s) {
-        const size_t cell = first + (size_t)s * seq_stride;
+        const size_t cell = first + i + (size_t)s * seq_stride;
         return plane + cell * units_cell + (unit ^ ((cell & 4u) ? swap : 0u));
     };
     U w[NBEAM];
@@ -241,34 +300,52 @@ __global__ void __launch_bounds__(256) kv4_reorder_kernel(U* a, U* b, uint32_t u
     }
 }
 
-template <class U>
-cudaError_t launch_reorder(U* a, U* b, uint32_t units_cell, uint32_t swap, const tsrc_kv4* kv, const int32_t* parent, uint32_t n_group,
-                           uint32_t n_beam, uint32_t cell0, uint32_t seq_stride, uint32_t n, cudaStream_t st) {
-    const size_t units = (size_t)n * units_cell;
-    const dim3 grid((unsigned)((units + 255u) / 256u), n_group, 2u * kv->n_head_kv);
-    if (n_beam <= 8u)
-        kv4_reorder_kernel<U, 8><<<grid, 256, 0, st>>>(a, b, units_cell, swap, kv->n_alloc, parent, n_beam, cell0, seq_stride, n);
-    else
-        kv4_reorder_kernel<U, 32><<<grid, 256, 0, st>>>(a, b, units_cell, swap, kv->n_alloc, parent, n_beam, cell0, seq_stride, n);
+// The first code_blocks CTAs of x take codes, the others scales. What is kept is neither read nor written.
+template <uint32_t NBEAM, class DU>
+__global__ void __launch_bounds__(256) kv4_reorder_kernel(Kv4Planes p, uint32_t code_blocks, const int32_t* parent, uint32_t n_beam,
+                                                          uint32_t cell0, uint32_t seq_stride, uint32_t n) {
+    const uint32_t group = blockIdx.y, head = blockIdx.z >> 1, which = blockIdx.z & 1u;
+    const int32_t* par = parent + (size_t)group * n_beam;
+    const size_t first = (size_t)cell0 + (size_t)group * n_beam * seq_stride;
+    if (blockIdx.x < code_blocks) {
+        const uint32_t per = p.D / 32u;
+        const size_t j = (size_t)blockIdx.x * 256u + threadIdx.x;
+        if (j >= (size_t)n * per) return;
+        reorder_unit<uint4, NBEAM>(reinterpret_cast<uint4*>(p.q[which]) + (size_t)head * p.n_alloc * per, j, per, p.D == 64u ? 1u : 2u,
+                                   par, n_beam, first, seq_stride);
+    } else {
+        const uint32_t per = p.D / 16u / (uint32_t)sizeof(DU);
+        const size_t j = (size_t)(blockIdx.x - code_blocks) * 256u + threadIdx.x;
+        if (j >= (size_t)n * per) return;
+        reorder_unit<DU, NBEAM>(reinterpret_cast<DU*>(p.d[which]) + (size_t)head * p.n_alloc * per, j, per, 0u, par, n_beam, first, seq_stride);
+    }
+}
+
+template <class DU>
+cudaError_t launch_reorder(const Kv4Planes& p, const int32_t* parent, uint32_t n_group, uint32_t n_beam, uint32_t cell0, uint32_t seq_stride,
+                           uint32_t n, cudaStream_t st) {
+    const size_t codes = ((size_t)n * (p.D / 32u) + 255u) / 256u, scales = ((size_t)n * (p.D / 16u / sizeof(DU)) + 255u) / 256u;
+    const dim3 grid((unsigned)(codes + scales), n_group, 2u * p.n_head_kv);
+    if (n_beam <= 8u) kv4_reorder_kernel<8, DU><<<grid, 256, 0, st>>>(p, (uint32_t)codes, parent, n_beam, cell0, seq_stride, n);
+    else kv4_reorder_kernel<32, DU><<<grid, 256, 0, st>>>(p, (uint32_t)codes, parent, n_beam, cell0, seq_stride, n);
     return cudaGetLastError();
 }
 
 template <class T, uint32_t NB, bool VEC>
 void launch_store(const T* k, const T* v, uint32_t n, size_t stride, const int64_t* cells, uint32_t cell0, const Kv4Planes& p, cudaStream_t st) {
-    const size_t threads = (size_t)n * (p.n_head_kv * p.D / (NB * 4u));
+    const size_t threads = (size_t)n * (p.n_head_kv * p.D / (NB * 8u));
     kv4_store_kernel<T, NB, VEC><<<dim3((unsigned)((threads + 255u) / 256u), k && v ? 2u : 1u), 256, 0, st>>>(k, v, n, stride, cells, cell0, p);
 }
 template <class T, uint32_t NB, bool VEC>
 void launch_read(T* k, T* v, uint32_t n, size_t stride, const int64_t* cells, uint32_t cell0, const Kv4Planes& p, cudaStream_t st) {
-    const size_t threads = (size_t)n * (p.n_head_kv * p.D / (NB * 4u));
+    const size_t threads = (size_t)n * (p.n_head_kv * p.D / (NB * 8u));
     kv4_read_kernel<T, NB, VEC><<<dim3((unsigned)((threads + 255u) / 256u), k && v ? 2u : 1u), 256, 0, st>>>(k, v, n, stride, cells, cell0, p);
 }
 
-// The variant by D, and by alignment: four values at once where rows and stride allow it.
+// The variant by D, and by alignment: eight values at once where rows and stride allow 16-byte accesses.
 template <class T>
 cudaError_t rows_io(bool store, void* k, void* v, uint32_t n, size_t stride, const int64_t* cells, uint32_t cell0, const Kv4Planes& p, cudaStream_t st) {
-    const size_t a = 4u * sizeof(T);
-    const bool vec = reinterpret_cast<uintptr_t>(k) % a == 0 && reinterpret_cast<uintptr_t>(v) % a == 0 && stride % 4u == 0;
+    const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 && stride * sizeof(T) % 16u == 0;
     T *kt = static_cast<T*>(k), *vt = static_cast<T*>(v);
     if (p.D == 64u) {
         if (store) vec ? launch_store<T, 2, true>(kt, vt, n, stride, cells, cell0, p, st) : launch_store<T, 2, false>(kt, vt, n, stride, cells, cell0, p, st);
@@ -306,7 +383,7 @@ int kv4_rows(const char* who, bool store, tsrc_ctx* ctx, const tsrc_kv4* kv, uin
     if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & m) || (reinterpret_cast<uintptr_t>(cells) & 7u))
         return refuse(TSRC_E_ARG, "%s: a pointer is not aligned to its elements", who);
     if (n == 0) return TSRC_OK;
-    if ((uint64_t)n * (E / 8u) > 256ull * 0x7FFFFFFFull) return refuse(TSRC_E_SHAPE, "%s: too many rows", who);
+    if ((uint64_t)n * (E / 16u) > 0xFFFF0000ull) return refuse(TSRC_E_SHAPE, "%s: n %u: more than 2^32 / (E / 16) rows in a call", who, n);
     DeviceScope scope(ctx);
     if (scope.rc) return scope.rc;
     const Kv4Planes p = planes_of(kv);
@@ -457,12 +534,9 @@ int tsrc_kv4_reorder(tsrc_ctx* ctx, tsrc_kv4* kv, const int32_t* parent, uint32_
     DeviceScope scope(ctx);
     if (scope.rc) return scope.rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t e = launch_reorder(reinterpret_cast<uint4*>(kv->q[0]), reinterpret_cast<uint4*>(kv->q[1]), kv->D / 32u,
-                                   kv->D == 64u ? 1u : 2u, kv, parent,
-                                   n_group, n_beam, cell0, seq_stride, n, st);
-    if (e == cudaSuccess)
-        e = launch_reorder(reinterpret_cast<uint32_t*>(kv->d[0]), reinterpret_cast<uint32_t*>(kv->d[1]), kv->D / 64u, 0u, kv, parent,
-                           n_group, n_beam, cell0, seq_stride, n, st);
+    const Kv4Planes p = planes_of(kv);
+    cudaError_t e = kv->D == 64u ? launch_reorder<uint32_t>(p, parent, n_group, n_beam, cell0, seq_stride, n, st)
+                                 : launch_reorder<uint2>(p, parent, n_group, n_beam, cell0, seq_stride, n, st);
     return e == cudaSuccess ? TSRC_OK : cuda_refuse(e, "tsrc_kv4_reorder");
 }
 

@@ -20,6 +20,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/tsrc.h"
 #include "tsrc_internal.h"
 
@@ -72,40 +74,73 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Four neighbouring values, loaded or stored at once where the address allows (VEC) or one by one.
+// Eight neighbouring values, loaded with 16-byte accesses where the address allows (VEC) or one by one.
 template <class T, bool VEC>
-__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
-    if constexpr (VEC) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 w = *reinterpret_cast<const float4*>(p);
-            v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
-        } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(p);
-            T t[4];
-            __builtin_memcpy(t, &w, 8);
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    if constexpr (VEC && sizeof(T) == 4) {
+        const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else if constexpr (VEC) {
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = to_f32(t[i]);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            } else {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = to_f32(p[i]);
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(p[i]);
     }
 }
+// d x of eight small whole numbers x, paired as (0, 4), (1, 5), (2, 6), (3, 7), rounded once to T and stored.
 template <class T, bool VEC>
-__device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
-    if constexpr (VEC) {
-        T t[4];
+__device__ __forceinline__ void store8(T* p, const __half2 (&x)[4], __half d) {
+    if constexpr (std::is_same_v<T, __half>) {
+        uint32_t y[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = from_f32<T>(v[i]);
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __hmul2(x[i], __half2half2(d));
+            y[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if constexpr (VEC)
+            __stcs(reinterpret_cast<uint4*>(p), make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410),
+                                                           __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632)));
         else {
-            uint2 w;
-            __builtin_memcpy(&w, t, 8);
-            *reinterpret_cast<uint2*>(p) = w;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = __ushort_as_half((unsigned short)(y[i & 3] >> (i & 4 ? 16 : 0)));
         }
     } else {
+        const float f = __half2float(d);
+        float y[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = from_f32<T>(v[i]);
+        for (int i = 0; i < 4; ++i) {
+            const float2 h = __half22float2(x[i]);
+            y[i] = f * h.x;
+            y[i + 4] = f * h.y;
+        }
+        if constexpr (VEC && sizeof(T) == 4) {
+            __stcs(reinterpret_cast<float4*>(p), make_float4(y[0], y[1], y[2], y[3]));
+            __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(y[4], y[5], y[6], y[7]));
+        } else if constexpr (VEC) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = from_f32<T>(y[i]);
+        }
     }
 }
 
