@@ -432,6 +432,8 @@ int tsrc_sync(tsrc_ctx* ctx, void* stream) {
     if (code & tsrc::kKv4ErrSet) return fail(TSRC_E_ARG, "tsrc_kv4_set_rows: a cell index outside the cache (those rows were not stored)");
     if (code & tsrc::kKv4ErrGet) return fail(TSRC_E_ARG, "tsrc_kv4_get_rows: a cell index outside the cache (those rows were not written)");
     if (code & tsrc::kKv4ErrParent) return fail(TSRC_E_ARG, "tsrc_kv4_reorder: a parent outside [0, n_beam) (those sequences kept their cells)");
+    e = tsrc::fa4_error(&code, true);
+    if (e != cudaSuccess) return cuda_fail(e, "reading the q4_0 attention error word");
     if (code) return fail(TSRC_E_DEVICE, "a q4_0 attention kernel gave up a bounded wait (code %u)", code);
     return TSRC_OK;
 }

@@ -2,7 +2,7 @@
 #include <cmath>
 #include <cstdio>
 
-#include "tsrc_kv4.cuh"
+#include "tsrc_fa4.cuh"
 
 namespace tsrc {
 
@@ -11,21 +11,6 @@ namespace {
 constexpr uint32_t kDecWarps = 4, kDecTile = 32, kDecStages = 3;
 constexpr uint32_t kSms = 148, kDecCtas = 4 * kSms;      // the CTAs that a B200 holds at once, four to an SM
 constexpr uint32_t kMaxCluster = 16;
-
-struct Fa4Args {
-    const void* q;
-    void* out;
-    size_t q_stride, out_stride;
-    const uint8_t *kq, *vq;
-    const __half *kd, *vd;
-    uint32_t T, n_head, n_head_kv, G, n_kv, n_alloc;
-    const int32_t* ranges;
-    const __half* mask;
-    size_t mask_stride;
-    float scale;
-    uint32_t group, row_tiles, splits;         // tokens a group, row tiles a group and KV head, splits of the cells
-    float *part_o, *part_ml;                   // splits joined by the merge kernel: [unit][split][R][D], [unit][split][R][4]
-};
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -74,6 +59,7 @@ enum : int {
     kRows8Split = 0,       // eight rows; q and the weights in two fp16 terms each
     kRows8 = 1,            // eight rows, one term (bf16 outputs)
     kRows16 = 2,           // sixteen rows, one term (bf16 outputs)
+    kRows128 = 3,          // the kernel for many rows
 };
 template <int MODE> constexpr uint32_t kRowsOf = MODE == kRows16 ? 16u : 8u;
 
@@ -732,10 +718,17 @@ struct Fa4Plan {
     size_t o_bytes, ml_bytes;                  // of the workspace, where a merge kernel joins the splits
 };
 
-Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint32_t n_head, uint32_t n_kv, uint32_t group, uint32_t max_len) {
+Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint32_t n_head, uint32_t n_kv, uint32_t group, uint32_t max_len, bool mask) {
     Fa4Plan p{};
     p.group = group ? group : T;
     const uint32_t rows = p.group * (n_head / n_head_kv);
+    p.splits = 1;
+    if (!mask && D <= 128u && rows >= 96u) {
+        p.mode = kRows128;
+        p.row_tiles = (rows + kFa4TcRows - 1u) / kFa4TcRows;
+        p.units = (T / p.group) * n_head_kv * p.row_tiles;
+        return p;
+    }
     p.mode = type != TSRC_TYPE_BF16 ? kRows8Split : rows <= 8u ? kRows8 : kRows16;
     const uint32_t R = p.mode == kRows16 ? 16u : 8u;
     p.row_tiles = (rows + R - 1u) / R;
@@ -746,7 +739,6 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
     // tile at least; where even clusters of sixteen leave most SMs empty and the cells are many, more splits and
     // a merge kernel.
     const uint32_t most = (len / kDecTile + 1u) / teams;
-    p.splits = 1;
     while (p.splits < kMaxCluster && p.splits * 2u <= most && p.units * p.splits < 2u * kDecCtas) p.splits *= 2u;
     if (p.units * kMaxCluster < kSms && most >= 8u * kMaxCluster) {
         p.splits = 2u * kSms / p.units;
@@ -832,7 +824,8 @@ const char* tsrc_flash_attn_q4_unsupported(uint32_t type, uint32_t n_head_kv, ui
 size_t tsrc_flash_attn_q4_workspace(uint32_t type, uint32_t n_head_kv, uint32_t head_dim, uint32_t T, uint32_t n_head,
                                     uint32_t n_kv, uint32_t group, uint32_t max_len) {
     if (T == 0 || tsrc_flash_attn_q4_unsupported(type, n_head_kv, head_dim, n_head)) return 0;
-    const Fa4Plan p = fa4_plan(type, n_head_kv, head_dim, T, n_head, n_kv, group, max_len);
+    // the largest a call of these sizes needs, with a mask or without
+    const Fa4Plan p = fa4_plan(type, n_head_kv, head_dim, T, n_head, n_kv, group, max_len, true);
     return p.o_bytes + p.ml_bytes;
 }
 
@@ -863,12 +856,15 @@ int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const v
     if (T == 0) return TSRC_OK;
     DeviceScope scope(ctx);
     if (scope.rc) return scope.rc;
-    const Fa4Plan p = fa4_plan(type, kv->n_head_kv, kv->D, T, n_head, n_kv, group, max_len);
+    const Fa4Plan p = fa4_plan(type, kv->n_head_kv, kv->D, T, n_head, n_kv, group, max_len, mask != nullptr);
     Fa4Args a{};
     a.q = q;
     a.out = out;
     a.q_stride = q_stride;
     a.out_stride = out_stride;
+    const uint32_t size = kv4_type_size(type);
+    a.q_wide = (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && (size_t)q_stride * size % 16u == 0;
+    a.out_wide = (reinterpret_cast<uintptr_t>(out) & (4u * size - 1u)) == 0 && out_stride % 4u == 0;
     a.kq = kv->q[0];
     a.vq = kv->q[1];
     a.kd = kv->d[0];
@@ -892,7 +888,8 @@ int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const v
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (type == TSRC_TYPE_F32) e = dec_launch_d<float, kRows8Split>(a, kv->D, p.units, st);
+    if (p.mode == kRows128) e = launch_fa4_tc(type, kv->D, a, p.units, st);
+    else if (type == TSRC_TYPE_F32) e = dec_launch_d<float, kRows8Split>(a, kv->D, p.units, st);
     else if (type == TSRC_TYPE_F16) e = dec_launch_d<__half, kRows8Split>(a, kv->D, p.units, st);
     else e = p.mode == kRows8 ? dec_launch_d<__nv_bfloat16, kRows8>(a, kv->D, p.units, st) : dec_launch_d<__nv_bfloat16, kRows16>(a, kv->D, p.units, st);
     if (e != cudaSuccess) return refuse(TSRC_E_CUDA, "tsrc_flash_attn_q4: %s (%s)", cudaGetErrorString(e), cudaGetErrorName(e));

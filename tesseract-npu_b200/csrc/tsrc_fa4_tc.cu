@@ -1,0 +1,684 @@
+// tsrc_fa4_tc.cu -- attention over the q4_0 KV cache with many query rows on one stretch of cells (prompts), on the
+// fifth-generation tensor cores. Layout of the cache: tsrc_kv4.cuh; the entry point and the rule that chooses
+// between this kernel and the one for few rows: tsrc_fa4.cu.
+//
+// A CTA takes 128 query rows -- the (token, head) pairs of a group that share a KV head -- and passes over the cells
+// they span in tiles of 64, with nine warps in three roles that hand over by mbarriers:
+//   dequant (4 warps)  codes and scales from global memory (a tile ahead, in registers) to fp16 operands in shared
+//                      memory: K as [8 values][cell][16 B], V transposed as [8 cells][value][16 B], the tensor
+//                      cores' unswizzled layout, every 16-byte store of a quarter warp side by side. Two buffers each.
+//   mma (1 thread)     S(i + 1) = Q K^T while the softmax of tile i runs, then O += P(i) V; S twice and O in tensor
+//                      memory, P written over its S.
+//   softmax (4 warps)  a thread per row: scores from tensor memory, running sum, weights back as fp16.
+// The reference that the weights' exponents are taken from follows the running maximum only when that has risen by
+// 8 (in log2): outputs in tensor memory are then rescaled, seldom after the first tiles; up to there weights reach
+// 2^8, which fp16 holds, and results do not depend on the reference.
+//   Range: q is scaled by a power of two per row, K's and V's scales by one per tile (V's follows the largest seen,
+// with O rescaled), so that all operands stay inside fp16. Scales of 32 and above, which no row of ordinary size
+// has, do not move these: such a cell gets a power of two of its own, which its scores and weights make good, so that
+// rows that do not see it keep their digits. Precision: bf16 outputs take one fp16 term (11 bits) of
+// q (exact), K, V and the weights. f32 and f16 outputs take two terms of each, 22 bits (d (n - 8) has 15, so K and V
+// are exact), and three products, the one of the two small terms left out: 2^-22 of the result.
+#include <type_traits>
+
+#include "tsrc_fa4.cuh"
+
+namespace tsrc {
+
+namespace {
+
+__device__ unsigned int g_fa4_error;                 // kKv4ErrWait once a wait ran out
+
+constexpr uint32_t kTile = 64, kRows = 128, kThreads = 288;
+constexpr long long kWaitCycles = 1ll << 31;         // a wait gives up after ~1 s of SM clock
+
+template <int D, bool PRECISE> struct TcShape {
+    static constexpr uint32_t NB = D / 32, TERMS = PRECISE ? 2 : 1;
+    static constexpr uint32_t Q_TERM = kRows * D * 2, KV_TERM = kTile * D * 2;      // bytes of one term of an operand
+    static constexpr uint32_t K_AT = Q_TERM * TERMS, V_AT = K_AT + 2 * KV_TERM * TERMS;
+    static constexpr uint32_t CTL_AT = V_AT + 2 * KV_TERM * TERMS;
+    // two CTAs an SM at most: tensor memory holds no more
+    static constexpr uint32_t BYTES = CTL_AT + 3072 < 100 * 1024 ? 100 * 1024 : CTL_AT + 3072;
+    static constexpr uint32_t MIN_CTAS = 2 * (BYTES + 1024) <= 227 * 1024 ? 2 : 1;
+    static constexpr uint32_t O_COL = 2 * kTile;                                    // tensor-memory columns: S, S, O
+};
+
+struct TileInfo {
+    float k_unscale;         // the tile's K operand times this is K
+    uint32_t v_exp;          // exponent field that V's scale follows from this tile on
+    uint32_t bad;            // a scale of V that is no number or infinite is in the tile (its block is 0 in the operand)
+    uint32_t far;            // a scale above the common one is in it: the cells' own powers of two count
+};
+constexpr uint32_t kFarExp = 19;     // exponent field of scales of 16 to 32, the largest that the common powers follow
+
+struct Control {                     // at most 3 KB
+    uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2];
+    TileInfo info[4];
+    // far tiles: what a cell's scores are times, and what the log2 of its weights is raised by. Of four tiles, as info:
+    // the dequant warps are up to two tiles ahead of the softmax when they write these.
+    float cell_k[4][kTile], cell_v[4][kTile];
+    uint32_t most[2][4][2];  // the dequant warps' largest |d| of K and V, by tile parity
+    uint32_t tmem, abort;
+    int32_t span[4][4];      // the softmax warps' first and last cell, and the cells that all their rows see
+};
+
+static_assert(sizeof(Control) <= 3072, "room behind the operands");
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory"); }
+// Waits for the phase of that parity; false when about a second passed or another role gave up.
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile uint32_t* abort) {
+    long long t0 = 0;
+    for (uint32_t it = 0;; ++it) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(smem_u32(b)), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((it & 63u) != 0u) continue;
+        if (*abort) return false;
+        if (it == 0) t0 = clock64();
+        else if (clock64() - t0 > kWaitCycles) break;
+    }
+    *abort = 1u;
+    atomicOr(&g_fa4_error, kKv4ErrWait);
+    return false;
+}
+__device__ __forceinline__ void commit(uint64_t* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// operand of `rows` rows in shared memory, 16-byte chunks of a row `rows` x 16 bytes apart, eight rows 128 bytes
+__device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t rows) {
+    return (uint64_t)((at >> 4) & 0x3FFFu) | ((uint64_t)rows << 16) | ((uint64_t)(128u >> 4) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+// f32 sums of fp16 products, 128 x n
+__host__ __device__ constexpr uint32_t instruction(uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((kRows >> 4) << 24); }
+
+#define TSRC_R8(v, o) "=r"((v)[o]), "=r"((v)[o + 1]), "=r"((v)[o + 2]), "=r"((v)[o + 3]), "=r"((v)[o + 4]), "=r"((v)[o + 5]), "=r"((v)[o + 6]), "=r"((v)[o + 7])
+#define TSRC_I8(v, o) "r"((v)[o]), "r"((v)[o + 1]), "r"((v)[o + 2]), "r"((v)[o + 3]), "r"((v)[o + 4]), "r"((v)[o + 5]), "r"((v)[o + 6]), "r"((v)[o + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : TSRC_R8(v, 0), TSRC_R8(v, 8), TSRC_R8(v, 16), TSRC_R8(v, 24) : "r"(at));
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t at, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : TSRC_R8(v, 0) : "r"(at));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+                 ::TSRC_I8(v, 0), TSRC_I8(v, 8), TSRC_I8(v, 16), TSRC_I8(v, 24), "r"(at) : "memory");
+}
+// Waits for the thread's loads; the registers go through it, so that nothing uses them before.
+#define TSRC_P8(v, o) "+r"((v)[o]), "+r"((v)[o + 1]), "+r"((v)[o + 2]), "+r"((v)[o + 3]), "+r"((v)[o + 4]), "+r"((v)[o + 5]), "+r"((v)[o + 6]), "+r"((v)[o + 7])
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : TSRC_P8(v, 0), TSRC_P8(v, 8) :: "memory");
+    asm volatile("" : TSRC_P8(v, 16), TSRC_P8(v, 24));
+}
+__device__ __forceinline__ void tmem_wait_ld64(uint32_t* v) {
+    tmem_wait_ld(v);
+    asm volatile("" : TSRC_P8(v, 32), TSRC_P8(v, 40), TSRC_P8(v, 48), TSRC_P8(v, 56));
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ __half2 as_h2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+// 2^(15 - e) in fp16: a scale with exponent field e goes to [1, 2)
+__device__ __forceinline__ __half2 to_one(uint32_t e) {
+    return __half2half2(__ushort_as_half(e < 30u ? (unsigned short)((30u - e) << 10) : (unsigned short)0x0200u));
+}
+// the largest finite magnitude among the four halves of two words
+__device__ __forceinline__ uint32_t finite_most(uint32_t u) {
+    u &= 0x7FFF7FFFu;
+    const uint32_t a = u & 0xFFFFu, b = u >> 16;
+    return max(a < 0x7C00u ? a : 0u, b < 0x7C00u ? b : 0u);
+}
+__device__ __forceinline__ uint32_t finite_only(uint32_t u) {
+    return ((u & 0x7C00u) == 0x7C00u ? 0u : u & 0xFFFFu) | ((u & 0x7C000000u) == 0x7C000000u ? 0u : u & 0xFFFF0000u);
+}
+template <class T>
+__device__ __forceinline__ void store4(T* p, const float (&x)[4], bool wide) {
+    if (wide) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        else {
+            T t[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = from_f32<T>(x[i]);
+            uint2 w;
+            w.x = (uint32_t)reinterpret_cast<const unsigned short&>(t[0]) | (uint32_t)reinterpret_cast<const unsigned short&>(t[1]) << 16;
+            w.y = (uint32_t)reinterpret_cast<const unsigned short&>(t[2]) | (uint32_t)reinterpret_cast<const unsigned short&>(t[3]) << 16;
+            *reinterpret_cast<uint2*>(p) = w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = from_f32<T>(x[i]);
+    }
+}
+// codes 4 j.. of two halves side by side, as n - 8
+__device__ __forceinline__ __half2 codes(uint32_t x, int j) {
+    const uint32_t u = ((x >> (4 * j)) & 0x000F000Fu) | 0x64006400u;
+    return __hsub2(as_h2(u), __float2half2_rn(1032.0f));
+}
+
+template <class T, int D, bool PRECISE>
+__global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_tc_kernel(Fa4Args a) {
+    using S = TcShape<D, PRECISE>;
+    constexpr uint32_t NB = S::NB, NBG = NB > 4 ? 4 : NB;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    Control& c = *reinterpret_cast<Control*>(sm + S::CTL_AT);
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    // the last rows first: in a causal prompt they see the most cells
+    const uint32_t hk = blockIdx.x % a.n_head_kv, rest = blockIdx.x / a.n_head_kv;
+    const uint32_t rt = a.row_tiles - 1u - rest % a.row_tiles, grp = rest / a.row_tiles;
+    const uint32_t rows = a.group * a.G, row = rt * kRows + tid;
+    const uint32_t tok = grp * a.group + row / a.G, head = hk * a.G + row % a.G;
+
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&c.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if (lane == 0) {
+            c.abort = 0;
+            for (int i = 0; i < 2; ++i) {
+                bar_init(&c.k_full[i], 4);
+                bar_init(&c.k_free[i], 1);
+                bar_init(&c.v_full[i], 4);
+                bar_init(&c.v_free[i], 1);
+                bar_init(&c.s_full[i], 2);           // the tensor cores, and the issuing thread for what it has seen
+                bar_init(&c.p_full[i], 4);
+            }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+    }
+    int32_t lo = 0, hi = 0;
+    float qs = 0.0f;                                 // this row's scale, for scores in log2
+    if (warp < 4) {
+        if (row < rows) {
+            hi = (int32_t)a.n_kv;
+            if (a.ranges) {
+                lo = max(a.ranges[2u * (size_t)tok], 0);
+                hi = min(a.ranges[2u * (size_t)tok + 1u], hi);
+            }
+            if (lo >= hi) lo = hi = 0;
+        }
+        const int32_t first = __reduce_min_sync(0xFFFFFFFFu, lo < hi ? lo : 0x7FFFFFFF), last = __reduce_max_sync(0xFFFFFFFFu, hi);
+        if (lane == 0) {
+            c.span[warp][0] = first;
+            c.span[warp][1] = last;
+        }
+        // q: the row's largest value to [2^12, 2^13), chunks of eight in the order 0 4 1 5 2 6 3 7 that K has
+        const T* q = static_cast<const T*>(a.q) + (size_t)tok * a.q_stride + (size_t)head * D;
+        float top = 0.0f;
+        if (row < rows) {
+#pragma unroll 4
+            for (uint32_t e = 0; e < D; e += 8) {
+                float x[8];
+                if (a.q_wide) load8<T, true>(q + e, x);
+                else load8<T, false>(q + e, x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+            }
+        }
+        const int e2 = min(12 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
+        const float f = pow2(e2);
+        qs = a.scale * 1.4426950408889634f * pow2(-e2);
+#pragma unroll 4
+        for (uint32_t e = 0; e < D; e += 8) {
+            float x[8] = {};
+            if (row < rows) {
+                if (a.q_wide) load8<T, true>(q + e, x);
+                else load8<T, false>(q + e, x);
+            }
+            uint32_t w[2][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = x[i] * f, v = x[i + 4] * f;
+                const __half2 h = __floats2half2_rn(u, v);
+                w[0][i] = as_u32(h);
+                if (PRECISE) {
+                    const float2 back = __half22float2(h);
+                    w[1][i] = as_u32(__floats2half2_rn(u - back.x, v - back.y));
+                }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < S::TERMS; ++k)
+                *reinterpret_cast<uint4*>(sm + k * S::Q_TERM + (e / 8u) * (kRows * 16u) + tid * 16u) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = c.tmem;
+    const int32_t first = min(min(c.span[0][0], c.span[1][0]), min(c.span[2][0], c.span[3][0]));
+    const int32_t last = max(max(c.span[0][1], c.span[1][1]), max(c.span[2][1], c.span[3][1]));
+    const uint32_t tile0 = last > first ? (uint32_t)first / kTile : 0u;
+    const uint32_t tiles = last > first ? ((uint32_t)last + kTile - 1u) / kTile - tile0 : 0u;
+
+    if (warp >= 4 && warp < 8) {
+        // ---- dequant
+        const uint32_t dw = warp - 4u;
+        // K: unit u is cell 16 dw + 8 u + lane % 8, values 8t .. 8t + 7 of every block, t = lane / 8
+        const uint32_t kt = lane >> 3, kc = 16u * dw + (lane & 7u);
+        const size_t plane = (size_t)hk * a.n_alloc + (size_t)tile0 * kTile;
+        // V: cells 8 vg .. + 7, chunk g, blocks 2 vb and 2 vb + 1
+        const uint32_t vg = 2u * dw + (lane >> 4), g = lane & 7u, vb = (lane >> 3) & 1u;
+        const bool v_live = 2u * vb < NB;
+        const uint8_t* kq = a.kq + (plane + kc) * (D / 2) + kv4_place(2u * kt, kc) * (NBG * 2u);
+        const __half* kd = a.kd + (plane + kc) * NB;
+        const uint8_t* vq = a.vq + (plane + 8u * vg) * (D / 2) + 4u * (v_live ? vb : 0u);
+        const __half* vd = a.vd + (plane + 8u * vg) * NB + 2u * (v_live ? vb : 0u);
+        uint32_t kw[2][NB], ks[2][NB / 2], vw[8], vs[8];
+        auto load = [&](uint32_t i) {
+            const size_t o = (size_t)i * kTile;
+#pragma unroll
+            for (uint32_t u = 0; u < 2; ++u) {
+                const uint8_t* p = kq + (o + 8u * u) * (D / 2);
+                const __half* d = kd + (o + 8u * u) * NB;
+                if constexpr (NB == 4) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(p);
+                    const uint2 y = *reinterpret_cast<const uint2*>(d);
+                    kw[u][0] = x.x; kw[u][1] = x.y; kw[u][2] = x.z; kw[u][3] = x.w;
+                    ks[u][0] = y.x; ks[u][1] = y.y;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(p);
+                    kw[u][0] = x.x; kw[u][1] = x.y;
+                    ks[u][0] = *reinterpret_cast<const uint32_t*>(d);
+                }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                vw[k] = *reinterpret_cast<const uint32_t*>(vq + (o + k) * (D / 2) + kv4_place(g, k) * (NBG * 2u));
+                vs[k] = *reinterpret_cast<const uint32_t*>(vd + (o + k) * NB);
+            }
+        };
+        uint32_t v_exp = 1;
+        bool ok = true;                              // after a wait that ran out the warps still meet at their barrier
+        if (tiles) load(0);
+        for (uint32_t i = 0; i < tiles; ++i) {
+            const uint32_t buf = i & 1u, round = i >> 1;
+            // the tile's largest scales, from what the four warps hold
+            __half2 mk = __float2half2_rn(0.0f), mv = mk;
+#pragma unroll
+            for (uint32_t u = 0; u < 2; ++u)
+#pragma unroll
+                for (uint32_t b = 0; b < NB / 2; ++b) mk = __hmax2_nan(mk, __habs2(as_h2(ks[u][b])));
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) mv = __hmax2_nan(mv, __habs2(as_h2(vs[k])));
+            uint32_t xk = max(as_u32(mk) & 0xFFFFu, as_u32(mk) >> 16), xv = max(as_u32(mv) & 0xFFFFu, as_u32(mv) >> 16);
+            xk = __reduce_max_sync(0xFFFFFFFFu, xk);
+            xv = __reduce_max_sync(0xFFFFFFFFu, xv);
+            if (xk >= 0x7C00u) {
+                uint32_t x = 0;
+#pragma unroll
+                for (uint32_t u = 0; u < 2; ++u)
+#pragma unroll
+                    for (uint32_t b = 0; b < NB / 2; ++b) x = max(x, finite_most(ks[u][b]));
+                xk = __reduce_max_sync(0xFFFFFFFFu, x);
+            }
+            if (xv >= 0x7C00u) {
+                uint32_t x = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) x = max(x, finite_most(vs[k]));
+                xv = __reduce_max_sync(0xFFFFFFFFu, x) | 0x8000u;
+            }
+            if (lane == 0) {
+                c.most[buf][dw][0] = xk;
+                c.most[buf][dw][1] = xv;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            uint32_t bad = 0;
+            xk = xv = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < 4; ++w) {
+                const uint32_t v = c.most[buf][w][1];
+                xk = max(xk, c.most[buf][w][0]);
+                xv = max(xv, v & 0x7FFFu);
+                bad |= v >> 15;
+            }
+            const uint32_t k_exp = min(max(xk >> 10, 1u), kFarExp);
+            v_exp = min(max(v_exp, xv >> 10), kFarExp);
+            const bool far = max(xk, xv) >> 10 > kFarExp;
+            if (tid == 128) c.info[i & 3u] = TileInfo{pow2((int)k_exp - 15), v_exp, bad, far};
+            uint32_t k_own[2] = {k_exp, k_exp};      // exponent field that each unit's operand follows
+            uint32_t v_own[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) v_own[k] = v_exp;
+            if (far) {
+#pragma unroll
+                for (uint32_t u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (uint32_t b = 0; b < NB / 2; ++b) k_own[u] = max(k_own[u], finite_most(ks[u][b]) >> 10);
+                    if (kt == 0) c.cell_k[i & 3u][kc + 8u * u] = pow2((int)(k_own[u] - k_exp));
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) {
+                    uint32_t x = finite_most(vs[k]);
+                    x = max(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8)) >> 10;
+                    v_own[k] = max(v_own[k], x);
+                    if (g == 0 && vb == 0) c.cell_v[i & 3u][8u * vg + k] = (float)(v_own[k] - v_exp);
+                }
+            }
+            if (bad) {
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) vs[k] = finite_only(vs[k]);
+            }
+            // K
+            uint32_t cw[8], cs[8];                   // V's words of this tile: the next tile's take their place
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                cw[k] = vw[k];
+                cs[k] = vs[k];
+            }
+            uint32_t ow[2][NB], os[2][NB / 2];
+#pragma unroll
+            for (uint32_t u = 0; u < 2; ++u) {
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) ow[u][b] = kw[u][b];
+#pragma unroll
+                for (uint32_t b = 0; b < NB / 2; ++b) os[u][b] = ks[u][b];
+            }
+            if (i + 1u < tiles) load(i + 1u);
+            if (i >= 2) ok = __all_sync(0xFFFFFFFFu, ok && bar_wait(&c.k_free[buf], (round - 1u) & 1u, &c.abort));
+            if (!ok) continue;
+            uint8_t* kb = sm + S::K_AT + buf * S::KV_TERM * S::TERMS;
+#pragma unroll
+            for (uint32_t u = 0; u < 2; ++u)
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) {
+                    const uint32_t x = __byte_perm(ow[u][b / 2], ow[u][NB / 2 + b / 2], b & 1u ? 0x7632 : 0x5410);
+                    const uint32_t s = os[u][b / 2];
+                    const __half2 d = __hmul2(as_h2(__byte_perm(s, s, b & 1u ? 0x3232 : 0x1010)), to_one(k_own[u]));
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const __half2 n = codes(x, j), y = __hmul2(n, d);
+                        h[j] = as_u32(y);
+                        if (PRECISE) l[j] = as_u32(__hfma2(n, d, __hneg2(y)));
+                    }
+                    uint8_t* p = kb + (4u * b + kt) * (kTile * 16u) + (kc + 8u * u) * 16u;
+                    *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
+                    if (PRECISE) *reinterpret_cast<uint4*>(p + S::KV_TERM) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(&c.k_full[buf]);
+            // V
+            if (i >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.v_free[buf], (round - 1u) & 1u, &c.abort));
+            if (!ok) continue;
+            if (v_live) {
+                uint8_t* vo = sm + S::V_AT + buf * S::KV_TERM * S::TERMS + vg * (D * 16u);
+                __half2 v_one[4];
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) v_one[k] = __lows2half2(to_one(v_own[2 * k]), to_one(v_own[2 * k + 1]));
+#pragma unroll
+                for (uint32_t b = 0; b < 2; ++b) {
+                    uint32_t x[4];
+                    __half2 d[4];
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        x[k] = __byte_perm(cw[2 * k], cw[2 * k + 1], b ? 0x7632 : 0x5410);
+                        d[k] = __hmul2(as_h2(__byte_perm(cs[2 * k], cs[2 * k + 1], b ? 0x7632 : 0x5410)), v_one[k]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t h[4], l[4];
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) {
+                            const __half2 n = codes(x[k], j), y = __hmul2(n, d[k]);
+                            h[k] = as_u32(y);
+                            if (PRECISE) l[k] = as_u32(__hfma2(n, d[k], __hneg2(y)));
+                        }
+                        // row j D / 4 + 8 (block) + g holds value 32 (block) + 4 g + j
+                        uint8_t* p = vo + ((uint32_t)j * (D / 4) + 8u * (2u * vb + b) + g) * 16u;
+                        *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
+                        if (PRECISE) *reinterpret_cast<uint4*>(p + S::KV_TERM) = make_uint4(l[0], l[1], l[2], l[3]);
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(&c.v_full[buf]);
+        }
+    } else if (warp == 8) {
+        // ---- mma
+        if (lane == 0) {
+            const uint32_t q_at = smem_u32(sm), k_at = q_at + S::K_AT, v_at = q_at + S::V_AT;
+            auto scores = [&](uint32_t i) {
+                const uint32_t buf = i & 1u;
+                if (!bar_wait(&c.k_full[buf], (i >> 1) & 1u, &c.abort)) return false;
+                fence_after();
+#pragma unroll
+                for (uint32_t k = 0; k < (PRECISE ? 3u : 1u); ++k) {       // q k, q_lo k, q k_lo
+                    const uint32_t qa = q_at + (k == 1 ? S::Q_TERM : 0u), kb = k_at + buf * S::KV_TERM * S::TERMS + (k == 2 ? S::KV_TERM : 0u);
+#pragma unroll
+                    for (uint32_t s = 0; s < D / 16; ++s)
+                        mma_ss(tmem + buf * kTile, operand(qa + s * 2u * kRows * 16u, kRows), operand(kb + s * 2u * kTile * 16u, kTile),
+                               instruction(kTile), k + s != 0u);
+                }
+                commit(&c.k_free[buf]);
+                commit(&c.s_full[buf]);
+                bar_arrive(&c.s_full[buf]);
+                return true;
+            };
+            bool ok = tiles == 0 || scores(0);
+            uint32_t done = 0;
+            for (uint32_t i = 0; ok && i < tiles; ++i) {
+                const uint32_t buf = i & 1u;
+                if (i + 1u < tiles) {
+                    // S(i + 1) takes the place of P(i - 1)
+                    if (i >= 1 && !bar_wait(&c.v_free[buf ^ 1u], ((i - 1u) >> 1) & 1u, &c.abort)) break;
+                    if (!scores(i + 1u)) break;
+                }
+                if (!bar_wait(&c.p_full[buf], (i >> 1) & 1u, &c.abort) || !bar_wait(&c.v_full[buf], (i >> 1) & 1u, &c.abort)) break;
+                fence_after();
+#pragma unroll
+                for (uint32_t k = 0; k < (PRECISE ? 3u : 1u); ++k) {       // p v, p_lo v, p v_lo
+                    const uint32_t pa = tmem + buf * kTile + (k == 1 ? kTile / 2u : 0u);
+                    const uint32_t vb = v_at + buf * S::KV_TERM * S::TERMS + (k == 2 ? S::KV_TERM : 0u);
+#pragma unroll
+                    for (uint32_t s = 0; s < kTile / 16; ++s)
+                        mma_ts(tmem + S::O_COL, pa + 8u * s, operand(vb + s * 2u * D * 16u, D), instruction(D), i + k + s != 0u);
+                }
+                commit(&c.v_free[buf]);
+                done = i + 1u;
+            }
+            // every product has ended before the tensor memory goes
+            if (done) bar_wait(&c.v_free[(done - 1u) & 1u], ((done - 1u) >> 1) & 1u, &c.abort);
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: this thread's row
+        const uint32_t mine = tmem + ((warp * 32u) << 16);
+        float m = -INFINITY, l = 0.0f;               // reference of the weights' exponents; running sum, both in units of 2^6 p
+        uint32_t v_exp = 1, lost = 0;                // lost: blocks of V in which the row sees a scale that is no number
+        bool ok = true;
+        // the cells that all rows of the warp see; rows behind the group's last lose nothing
+        const int32_t all_lo = __reduce_max_sync(0xFFFFFFFFu, row < rows ? lo : 0), all_hi = __reduce_min_sync(0xFFFFFFFFu, row < rows ? hi : 0x7FFFFFFF);
+        for (uint32_t i = 0; i < tiles; ++i) {
+            const uint32_t buf = i & 1u;
+            const int32_t c0 = (int32_t)((tile0 + i) * kTile);
+            ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.s_full[buf], (i >> 1) & 1u, &c.abort));
+            if (!ok) break;
+            fence_after();
+            uint32_t raw[64];
+            tmem_ld32(mine + buf * kTile, raw);
+            tmem_ld32(mine + buf * kTile + 32u, raw + 32);
+            const TileInfo info = c.info[i & 3u];
+            tmem_wait_ld64(raw);
+            const float f = qs * info.k_unscale;
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (c0 >= all_lo && c0 + (int32_t)kTile <= all_hi) {
+#pragma unroll
+                for (int j = 0; j < 64; ++j) {
+                    const float s = __uint_as_float(raw[j]) * f;
+                    raw[j] = __float_as_uint(s);
+                    top[j & 3] = fmaxf(top[j & 3], s);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 64; ++j) {
+                    const float s = c0 + j >= lo && c0 + j < hi ? __uint_as_float(raw[j]) * f : -INFINITY;
+                    raw[j] = __float_as_uint(s);
+                    top[j & 3] = fmaxf(top[j & 3], s);
+                }
+            }
+            if (info.far) {                          // seldom: the cells' own powers of two
+                top[0] = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 64; ++j) {
+                    const float s = fmaf(__uint_as_float(raw[j]), c.cell_k[i & 3u][j], c.cell_v[i & 3u][j]);
+                    raw[j] = __float_as_uint(s);
+                    top[0] = fmaxf(top[0], s);
+                }
+                top[1] = top[2] = top[3] = top[0];
+            }
+            const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            if (__any_sync(0xFFFFFFFFu, most > m + 8.0f || info.v_exp != v_exp)) {
+                const float now = fmaxf(m, most), base = now == -INFINITY ? 0.0f : now, down = ex2(m - base);
+                l *= down;
+                m = now;
+                if (i > 0) {
+                    // the products so far have to be there
+                    ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.v_free[buf ^ 1u], ((i - 1u) >> 1) & 1u, &c.abort));
+                    if (!ok) break;
+                    fence_after();
+                    const float both = down * pow2((int)v_exp - (int)info.v_exp);
+#pragma unroll
+                    for (uint32_t k = 0; k < D / 32; ++k) {
+                        uint32_t o[32];
+                        tmem_ld32(mine + S::O_COL + 32u * k, o);
+                        tmem_wait_ld(o);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * both);
+                        tmem_st32(mine + S::O_COL + 32u * k, o);
+                    }
+                }
+                v_exp = info.v_exp;
+            }
+            const float up = m == -INFINITY ? 0.0f : 6.0f - m;
+            float sum[4] = {};
+            uint32_t hw[32], lw[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const float p0 = ex2(__uint_as_float(raw[2 * j]) + up), p1 = ex2(__uint_as_float(raw[2 * j + 1]) + up);
+                if (!info.far) {
+                    sum[j & 1] += p0;
+                    sum[2 + (j & 1)] += p1;
+                } else {
+                    sum[0] += p0 * ex2(-c.cell_v[i & 3u][2 * j]);
+                    sum[2] += p1 * ex2(-c.cell_v[i & 3u][2 * j + 1]);
+                }
+                const __half2 h = __floats2half2_rn(p0, p1);
+                hw[j] = as_u32(h);
+                if (PRECISE) {
+                    const float2 back = __half22float2(h);
+                    lw[j] = as_u32(__floats2half2_rn(p0 - back.x, p1 - back.y));
+                }
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st32(mine + buf * kTile, hw);
+            if (PRECISE) tmem_st32(mine + buf * kTile + kTile / 2u, lw);
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&c.p_full[buf]);
+            if (info.bad) {                          // seldom: which of the blocks left out of V this row would have met
+                for (uint32_t j = 0; j < kTile; ++j) {
+                    if (c0 + (int32_t)j < lo || c0 + (int32_t)j >= hi) continue;
+                    const __half* d = a.vd + ((size_t)hk * a.n_alloc + (uint32_t)c0 + j) * NB;
+                    for (uint32_t b = 0; b < NB; ++b)
+                        if ((__half_as_ushort(d[b]) & 0x7C00u) == 0x7C00u) lost |= 1u << b;
+                }
+            }
+        }
+        if (ok && row < rows) {
+            const bool any = tiles != 0;
+            if (any) ok = bar_wait(&c.v_free[(tiles - 1u) & 1u], ((tiles - 1u) >> 1) & 1u, &c.abort);
+        }
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (ok) {
+            fence_after();
+            const float f = l == 0.0f ? 0.0f : pow2((int)v_exp - 15) / l;
+            T* out = static_cast<T*>(a.out) + (size_t)tok * a.out_stride + (size_t)head * D;
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                uint32_t o[32] = {};
+                if (tiles) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) tmem_ld8(mine + S::O_COL + j * (D / 4) + 8u * b, o + 8 * j);
+                    tmem_wait_ld(o);
+                }
+                if (row < rows) {
+#pragma unroll
+                    for (uint32_t g = 0; g < 8; ++g) {
+                        float x[4];
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j) {
+                            x[j] = l == 0.0f ? 0.0f : __uint_as_float(o[8 * j + g]) * f;
+                            if (lost >> b & 1u) x[j] = __int_as_float(0x7FC00000);
+                        }
+                        store4<T>(out + 32u * b + 4u * g, x, a.out_wide);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
+    }
+}
+
+template <class T, int D, bool PRECISE>
+cudaError_t launch(const Fa4Args& a, uint32_t units, cudaStream_t st) {
+    using S = TcShape<D, PRECISE>;
+    static bool done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !done[dev]) {
+        e = cudaFuncSetAttribute(fa4_tc_kernel<T, D, PRECISE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) done[dev] = true;
+    }
+    fa4_tc_kernel<T, D, PRECISE><<<units, kThreads, S::BYTES, st>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_fa4_tc(uint32_t type, uint32_t D, const Fa4Args& a, uint32_t units, cudaStream_t st) {
+    if (type == TSRC_TYPE_F32) return D == 64u ? launch<float, 64, true>(a, units, st) : launch<float, 128, true>(a, units, st);
+    if (type == TSRC_TYPE_F16) return D == 64u ? launch<__half, 64, true>(a, units, st) : launch<__half, 128, true>(a, units, st);
+    return D == 64u ? launch<__nv_bfloat16, 64, false>(a, units, st) : launch<__nv_bfloat16, 128, false>(a, units, st);
+}
+
+cudaError_t fa4_error(uint32_t* code, bool clear) {
+    cudaError_t e = cudaMemcpyFromSymbol(code, g_fa4_error, sizeof(uint32_t));
+    if (e == cudaSuccess && clear && *code) {
+        const uint32_t zero = 0;
+        e = cudaMemcpyToSymbol(g_fa4_error, &zero, sizeof(uint32_t));
+    }
+    return e;
+}
+
+}  // namespace tsrc

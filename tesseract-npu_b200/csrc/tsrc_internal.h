@@ -252,5 +252,6 @@ void kv4_drop(tsrc_kv4* kv);
 // bits of the q4_0 kernels' error word, cleared when read with clear = true
 constexpr uint32_t kKv4ErrSet = 1u, kKv4ErrGet = 2u, kKv4ErrParent = 4u, kKv4ErrWait = 8u;
 cudaError_t kv4_error(uint32_t* code, bool clear);
+cudaError_t fa4_error(uint32_t* code, bool clear);
 
 }  // namespace tsrc
