@@ -3,11 +3,12 @@
 // between this kernel and the one for few rows: tsrc_fa4.cu.
 //
 // A CTA takes 128 query rows -- the (token, head) pairs of a group that share a KV head -- and passes over the cells
-// they span in tiles of 64, with nine warps in three roles that hand over by mbarriers:
-//   dequant (4 warps)  codes and scales from global memory (a tile ahead, in registers) to fp16 operands in shared
-//                      memory: K as [8 values][cell][16 B], V transposed as [8 cells][value][16 B], the tensor
-//                      cores' unswizzled layout, every 16-byte store of a quarter warp side by side. Two buffers each.
-//   mma (1 thread)     S(i + 1) = Q K^T while the softmax of tile i runs, then O += P(i) V; S twice and O in tensor
+// they span in tiles of 64, its warps in three roles that hand over by mbarriers:
+//   dequant (4 or 8 warps)  codes and scales from global memory (a tile ahead, in registers) to fp16 operands in
+//                      shared memory: K as [8 values][cell][16 B], V transposed as [8 cells][value][16 B], the
+//                      tensor cores' unswizzled layout, every 16-byte store of a quarter warp side by side. Two buffers
+//                      each.
+//   products (1 thread)  S(i + 1) = Q K^T while the softmax of tile i runs, then O += P(i) V; S twice and O in tensor
 //                      memory, P written over its S.
 //   softmax (4 warps)  a thread per row: scores from tensor memory, running sum, weights back as fp16.
 // The reference that the weights' exponents are taken from follows the running maximum only when that has risen by
@@ -29,7 +30,7 @@ namespace {
 
 __device__ unsigned int g_fa4_error;                 // kKv4ErrWait once a wait ran out
 
-constexpr uint32_t kTile = 64, kRows = 128, kThreads = 288;
+constexpr uint32_t kTile = 64, kRows = 128;
 constexpr long long kWaitCycles = 1ll << 31;         // a wait gives up after ~1 s of SM clock
 
 template <int D, bool PRECISE> struct TcShape {
@@ -40,6 +41,8 @@ template <int D, bool PRECISE> struct TcShape {
     // two CTAs an SM at most: tensor memory holds no more
     static constexpr uint32_t BYTES = CTL_AT + 3072 < 100 * 1024 ? 100 * 1024 : CTL_AT + 3072;
     static constexpr uint32_t MIN_CTAS = 2 * (BYTES + 1024) <= 227 * 1024 ? 2 : 1;
+    static constexpr uint32_t DW = MIN_CTAS == 1 ? 8 : 4, THREADS = 160 + 32 * DW;   // dequant warps
+    static constexpr uint32_t KU = 8 / DW, BV = 8 / DW;                             // a lane's cells of K, blocks of V
     static constexpr uint32_t O_COL = 2 * kTile;                                    // tensor-memory columns: S, S, O
 };
 
@@ -57,7 +60,7 @@ struct Control {                     // at most 3 KB
     // far tiles: what a cell's scores are times, and what the log2 of its weights is raised by. Of four tiles, as info:
     // the dequant warps are up to two tiles ahead of the softmax when they write these.
     float cell_k[4][kTile], cell_v[4][kTile];
-    uint32_t most[2][4][2];  // the dequant warps' largest |d| of K and V, by tile parity
+    uint32_t most[2][8][2];  // the dequant warps' largest |d| of K and V, by tile parity
     uint32_t tmem, abort;
     int32_t span[4][4];      // the softmax warps' first and last cell, and the cells that all their rows see
 };
@@ -114,16 +117,17 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t* v) {
 __device__ __forceinline__ void tmem_ld8(uint32_t at, uint32_t* v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : TSRC_R8(v, 0) : "r"(at));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-                 ::TSRC_I8(v, 0), TSRC_I8(v, 8), TSRC_I8(v, 16), TSRC_I8(v, 24), "r"(at) : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::TSRC_I8(v, 0), "r"(at) : "memory");
 }
 // Waits for the thread's loads; the registers go through it, so that nothing uses them before.
 #define TSRC_P8(v, o) "+r"((v)[o]), "+r"((v)[o + 1]), "+r"((v)[o + 2]), "+r"((v)[o + 3]), "+r"((v)[o + 4]), "+r"((v)[o + 5]), "+r"((v)[o + 6]), "+r"((v)[o + 7])
 __device__ __forceinline__ void tmem_wait_ld(uint32_t* v) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : TSRC_P8(v, 0), TSRC_P8(v, 8) :: "memory");
     asm volatile("" : TSRC_P8(v, 16), TSRC_P8(v, 24));
+}
+__device__ __forceinline__ void tmem_wait_ld8(uint32_t* v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : TSRC_P8(v, 0) :: "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld64(uint32_t* v) {
     tmem_wait_ld(v);
@@ -177,9 +181,9 @@ __device__ __forceinline__ __half2 codes(uint32_t x, int j) {
 }
 
 template <class T, int D, bool PRECISE>
-__global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_tc_kernel(Fa4Args a) {
+__global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECISE>::MIN_CTAS) fa4_tc_kernel(Fa4Args a) {
     using S = TcShape<D, PRECISE>;
-    constexpr uint32_t NB = S::NB, NBG = NB > 4 ? 4 : NB;
+    constexpr uint32_t NB = S::NB;
     extern __shared__ __align__(1024) uint8_t sm[];
     Control& c = *reinterpret_cast<Control*>(sm + S::CTL_AT);
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
@@ -189,15 +193,15 @@ __global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_t
     const uint32_t rows = a.group * a.G, row = rt * kRows + tid;
     const uint32_t tok = grp * a.group + row / a.G, head = hk * a.G + row % a.G;
 
-    if (warp == 8) {
+    if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&c.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         if (lane == 0) {
             c.abort = 0;
             for (int i = 0; i < 2; ++i) {
-                bar_init(&c.k_full[i], 4);
+                bar_init(&c.k_full[i], S::DW);
                 bar_init(&c.k_free[i], 1);
-                bar_init(&c.v_full[i], 4);
+                bar_init(&c.v_full[i], S::DW);
                 bar_init(&c.v_free[i], 1);
                 bar_init(&c.s_full[i], 2);           // the tensor cores, and the issuing thread for what it has seen
                 bar_init(&c.p_full[i], 4);
@@ -225,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_t
         const T* q = static_cast<const T*>(a.q) + (size_t)tok * a.q_stride + (size_t)head * D;
         float top = 0.0f;
         if (row < rows) {
-#pragma unroll 4
+#pragma unroll 2
             for (uint32_t e = 0; e < D; e += 8) {
                 float x[8];
                 if (a.q_wide) load8<T, true>(q + e, x);
@@ -237,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_t
         const int e2 = min(12 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
         const float f = pow2(e2);
         qs = a.scale * 1.4426950408889634f * pow2(-e2);
-#pragma unroll 4
+#pragma unroll 2
         for (uint32_t e = 0; e < D; e += 8) {
             float x[8] = {};
             if (row < rows) {
@@ -270,197 +274,14 @@ __global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_t
     const uint32_t tile0 = last > first ? (uint32_t)first / kTile : 0u;
     const uint32_t tiles = last > first ? ((uint32_t)last + kTile - 1u) / kTile - tile0 : 0u;
 
-    if (warp >= 4 && warp < 8) {
-        // ---- dequant
-        const uint32_t dw = warp - 4u;
-        // K: unit u is cell 16 dw + 8 u + lane % 8, values 8t .. 8t + 7 of every block, t = lane / 8
-        const uint32_t kt = lane >> 3, kc = 16u * dw + (lane & 7u);
-        const size_t plane = (size_t)hk * a.n_alloc + (size_t)tile0 * kTile;
-        // V: cells 8 vg .. + 7, chunk g, blocks 2 vb and 2 vb + 1
-        const uint32_t vg = 2u * dw + (lane >> 4), g = lane & 7u, vb = (lane >> 3) & 1u;
-        const bool v_live = 2u * vb < NB;
-        const uint8_t* kq = a.kq + (plane + kc) * (D / 2) + kv4_place(2u * kt, kc) * (NBG * 2u);
-        const __half* kd = a.kd + (plane + kc) * NB;
-        const uint8_t* vq = a.vq + (plane + 8u * vg) * (D / 2) + 4u * (v_live ? vb : 0u);
-        const __half* vd = a.vd + (plane + 8u * vg) * NB + 2u * (v_live ? vb : 0u);
-        uint32_t kw[2][NB], ks[2][NB / 2], vw[8], vs[8];
-        auto load = [&](uint32_t i) {
-            const size_t o = (size_t)i * kTile;
-#pragma unroll
-            for (uint32_t u = 0; u < 2; ++u) {
-                const uint8_t* p = kq + (o + 8u * u) * (D / 2);
-                const __half* d = kd + (o + 8u * u) * NB;
-                if constexpr (NB == 4) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(p);
-                    const uint2 y = *reinterpret_cast<const uint2*>(d);
-                    kw[u][0] = x.x; kw[u][1] = x.y; kw[u][2] = x.z; kw[u][3] = x.w;
-                    ks[u][0] = y.x; ks[u][1] = y.y;
-                } else {
-                    const uint2 x = *reinterpret_cast<const uint2*>(p);
-                    kw[u][0] = x.x; kw[u][1] = x.y;
-                    ks[u][0] = *reinterpret_cast<const uint32_t*>(d);
-                }
-            }
-#pragma unroll
-            for (uint32_t k = 0; k < 8; ++k) {
-                vw[k] = *reinterpret_cast<const uint32_t*>(vq + (o + k) * (D / 2) + kv4_place(g, k) * (NBG * 2u));
-                vs[k] = *reinterpret_cast<const uint32_t*>(vd + (o + k) * NB);
-            }
-        };
-        uint32_t v_exp = 1;
-        bool ok = true;                              // after a wait that ran out the warps still meet at their barrier
-        if (tiles) load(0);
-        for (uint32_t i = 0; i < tiles; ++i) {
-            const uint32_t buf = i & 1u, round = i >> 1;
-            // the tile's largest scales, from what the four warps hold
-            __half2 mk = __float2half2_rn(0.0f), mv = mk;
-#pragma unroll
-            for (uint32_t u = 0; u < 2; ++u)
-#pragma unroll
-                for (uint32_t b = 0; b < NB / 2; ++b) mk = __hmax2_nan(mk, __habs2(as_h2(ks[u][b])));
-#pragma unroll
-            for (uint32_t k = 0; k < 8; ++k) mv = __hmax2_nan(mv, __habs2(as_h2(vs[k])));
-            uint32_t xk = max(as_u32(mk) & 0xFFFFu, as_u32(mk) >> 16), xv = max(as_u32(mv) & 0xFFFFu, as_u32(mv) >> 16);
-            xk = __reduce_max_sync(0xFFFFFFFFu, xk);
-            xv = __reduce_max_sync(0xFFFFFFFFu, xv);
-            if (xk >= 0x7C00u) {
-                uint32_t x = 0;
-#pragma unroll
-                for (uint32_t u = 0; u < 2; ++u)
-#pragma unroll
-                    for (uint32_t b = 0; b < NB / 2; ++b) x = max(x, finite_most(ks[u][b]));
-                xk = __reduce_max_sync(0xFFFFFFFFu, x);
-            }
-            if (xv >= 0x7C00u) {
-                uint32_t x = 0;
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) x = max(x, finite_most(vs[k]));
-                xv = __reduce_max_sync(0xFFFFFFFFu, x) | 0x8000u;
-            }
-            if (lane == 0) {
-                c.most[buf][dw][0] = xk;
-                c.most[buf][dw][1] = xv;
-            }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            uint32_t bad = 0;
-            xk = xv = 0;
-#pragma unroll
-            for (uint32_t w = 0; w < 4; ++w) {
-                const uint32_t v = c.most[buf][w][1];
-                xk = max(xk, c.most[buf][w][0]);
-                xv = max(xv, v & 0x7FFFu);
-                bad |= v >> 15;
-            }
-            const uint32_t k_exp = min(max(xk >> 10, 1u), kFarExp);
-            v_exp = min(max(v_exp, xv >> 10), kFarExp);
-            const bool far = max(xk, xv) >> 10 > kFarExp;
-            if (tid == 128) c.info[i & 3u] = TileInfo{pow2((int)k_exp - 15), v_exp, bad, far};
-            uint32_t k_own[2] = {k_exp, k_exp};      // exponent field that each unit's operand follows
-            uint32_t v_own[8];
-#pragma unroll
-            for (uint32_t k = 0; k < 8; ++k) v_own[k] = v_exp;
-            if (far) {
-#pragma unroll
-                for (uint32_t u = 0; u < 2; ++u) {
-#pragma unroll
-                    for (uint32_t b = 0; b < NB / 2; ++b) k_own[u] = max(k_own[u], finite_most(ks[u][b]) >> 10);
-                    if (kt == 0) c.cell_k[i & 3u][kc + 8u * u] = pow2((int)(k_own[u] - k_exp));
-                }
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                    uint32_t x = finite_most(vs[k]);
-                    x = max(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8)) >> 10;
-                    v_own[k] = max(v_own[k], x);
-                    if (g == 0 && vb == 0) c.cell_v[i & 3u][8u * vg + k] = (float)(v_own[k] - v_exp);
-                }
-            }
-            if (bad) {
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) vs[k] = finite_only(vs[k]);
-            }
-            // K
-            uint32_t cw[8], cs[8];                   // V's words of this tile: the next tile's take their place
-#pragma unroll
-            for (uint32_t k = 0; k < 8; ++k) {
-                cw[k] = vw[k];
-                cs[k] = vs[k];
-            }
-            uint32_t ow[2][NB], os[2][NB / 2];
-#pragma unroll
-            for (uint32_t u = 0; u < 2; ++u) {
-#pragma unroll
-                for (uint32_t b = 0; b < NB; ++b) ow[u][b] = kw[u][b];
-#pragma unroll
-                for (uint32_t b = 0; b < NB / 2; ++b) os[u][b] = ks[u][b];
-            }
-            if (i + 1u < tiles) load(i + 1u);
-            if (i >= 2) ok = __all_sync(0xFFFFFFFFu, ok && bar_wait(&c.k_free[buf], (round - 1u) & 1u, &c.abort));
-            if (!ok) continue;
-            uint8_t* kb = sm + S::K_AT + buf * S::KV_TERM * S::TERMS;
-#pragma unroll
-            for (uint32_t u = 0; u < 2; ++u)
-#pragma unroll
-                for (uint32_t b = 0; b < NB; ++b) {
-                    const uint32_t x = __byte_perm(ow[u][b / 2], ow[u][NB / 2 + b / 2], b & 1u ? 0x7632 : 0x5410);
-                    const uint32_t s = os[u][b / 2];
-                    const __half2 d = __hmul2(as_h2(__byte_perm(s, s, b & 1u ? 0x3232 : 0x1010)), to_one(k_own[u]));
-                    uint32_t h[4], l[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const __half2 n = codes(x, j), y = __hmul2(n, d);
-                        h[j] = as_u32(y);
-                        if (PRECISE) l[j] = as_u32(__hfma2(n, d, __hneg2(y)));
-                    }
-                    uint8_t* p = kb + (4u * b + kt) * (kTile * 16u) + (kc + 8u * u) * 16u;
-                    *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
-                    if (PRECISE) *reinterpret_cast<uint4*>(p + S::KV_TERM) = make_uint4(l[0], l[1], l[2], l[3]);
-                }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) bar_arrive(&c.k_full[buf]);
-            // V
-            if (i >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.v_free[buf], (round - 1u) & 1u, &c.abort));
-            if (!ok) continue;
-            if (v_live) {
-                uint8_t* vo = sm + S::V_AT + buf * S::KV_TERM * S::TERMS + vg * (D * 16u);
-                __half2 v_one[4];
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) v_one[k] = __lows2half2(to_one(v_own[2 * k]), to_one(v_own[2 * k + 1]));
-#pragma unroll
-                for (uint32_t b = 0; b < 2; ++b) {
-                    uint32_t x[4];
-                    __half2 d[4];
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) {
-                        x[k] = __byte_perm(cw[2 * k], cw[2 * k + 1], b ? 0x7632 : 0x5410);
-                        d[k] = __hmul2(as_h2(__byte_perm(cs[2 * k], cs[2 * k + 1], b ? 0x7632 : 0x5410)), v_one[k]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t h[4], l[4];
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            const __half2 n = codes(x[k], j), y = __hmul2(n, d[k]);
-                            h[k] = as_u32(y);
-                            if (PRECISE) l[k] = as_u32(__hfma2(n, d[k], __hneg2(y)));
-                        }
-                        // row j D / 4 + 8 (block) + g holds value 32 (block) + 4 g + j
-                        uint8_t* p = vo + ((uint32_t)j * (D / 4) + 8u * (2u * vb + b) + g) * 16u;
-                        *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
-                        if (PRECISE) *reinterpret_cast<uint4*>(p + S::KV_TERM) = make_uint4(l[0], l[1], l[2], l[3]);
-                    }
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) bar_arrive(&c.v_full[buf]);
-        }
-    } else if (warp == 8) {
-        // ---- mma
+    if (warp == 4u + S::DW) {
+        // ---- products, issued by one thread
         if (lane == 0) {
             const uint32_t q_at = smem_u32(sm), k_at = q_at + S::K_AT, v_at = q_at + S::V_AT;
-            auto scores = [&](uint32_t i) {
+            auto scores = [&](uint32_t i) {              // S(i)
                 const uint32_t buf = i & 1u;
+                // it takes the place of P(i - 2)
+                if (i >= 2 && !bar_wait(&c.v_free[buf], ((i - 2u) >> 1) & 1u, &c.abort)) return false;
                 if (!bar_wait(&c.k_full[buf], (i >> 1) & 1u, &c.abort)) return false;
                 fence_after();
 #pragma unroll
@@ -476,16 +297,9 @@ __global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_t
                 bar_arrive(&c.s_full[buf]);
                 return true;
             };
-            bool ok = tiles == 0 || scores(0);
-            uint32_t done = 0;
-            for (uint32_t i = 0; ok && i < tiles; ++i) {
+            auto outputs = [&](uint32_t i) {             // O += P(i) V
                 const uint32_t buf = i & 1u;
-                if (i + 1u < tiles) {
-                    // S(i + 1) takes the place of P(i - 1)
-                    if (i >= 1 && !bar_wait(&c.v_free[buf ^ 1u], ((i - 1u) >> 1) & 1u, &c.abort)) break;
-                    if (!scores(i + 1u)) break;
-                }
-                if (!bar_wait(&c.p_full[buf], (i >> 1) & 1u, &c.abort) || !bar_wait(&c.v_full[buf], (i >> 1) & 1u, &c.abort)) break;
+                if (!bar_wait(&c.v_full[buf], (i >> 1) & 1u, &c.abort) || !bar_wait(&c.p_full[buf], (i >> 1) & 1u, &c.abort)) return false;
                 fence_after();
 #pragma unroll
                 for (uint32_t k = 0; k < (PRECISE ? 3u : 1u); ++k) {       // p v, p_lo v, p v_lo
@@ -496,12 +310,202 @@ __global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_t
                         mma_ts(tmem + S::O_COL, pa + 8u * s, operand(vb + s * 2u * D * 16u, D), instruction(D), i + k + s != 0u);
                 }
                 commit(&c.v_free[buf]);
-                done = i + 1u;
-            }
-            // every product has ended before the tensor memory goes
-            if (done) bar_wait(&c.v_free[(done - 1u) & 1u], ((done - 1u) >> 1) & 1u, &c.abort);
+                return true;
+            };
+            bool ok = tiles == 0 || scores(0);
+            for (uint32_t i = 0; ok && i < tiles; ++i) ok = (i + 1u == tiles || scores(i + 1u)) && outputs(i);
         }
         __syncwarp();
+    } else if (warp >= 4) {
+        // ---- dequant
+        constexpr uint32_t KU = S::KU, BV = S::BV;
+        const uint32_t dw = warp - 4u;
+        // K: unit u is cell kc + 8 u, values 8t .. 8t + 7 of every block, t = lane / 8
+        const uint32_t kt = lane >> 3, kc = 8u * KU * dw + (lane & 7u);
+        const size_t plane = (size_t)hk * a.n_alloc + (size_t)tile0 * kTile;
+        // V: cells 8 vg .. + 7, chunk g, BV blocks from vb on
+        const uint32_t vg = BV == 2 ? 2u * dw + (lane >> 4) : dw, g = lane & 7u, vb = BV == 2 ? (lane >> 3 & 1u) * 2u : lane >> 3;
+        const bool v_live = vb < NB;
+        const uint8_t* kq = a.kq + (plane + kc) * (D / 2) + kv4_place(2u * kt, kc) * (NB * 2u);
+        const __half* kd = a.kd + (plane + kc) * NB;
+        const uint8_t* vq = a.vq + (plane + 8u * vg) * (D / 2) + 2u * (v_live ? vb : 0u);
+        const __half* vd = a.vd + (plane + 8u * vg) * NB + (v_live ? vb : 0u);
+        uint32_t kw[KU][NB], ks[KU][NB / 2], vw[8], vs[8];
+        auto load_k = [&](uint32_t i) {
+            const size_t o = (size_t)i * kTile;
+#pragma unroll
+            for (uint32_t u = 0; u < KU; ++u) {
+                const uint8_t* p = kq + (o + 8u * u) * (D / 2);
+                const __half* d = kd + (o + 8u * u) * NB;
+                if constexpr (NB == 4) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(p);
+                    const uint2 y = *reinterpret_cast<const uint2*>(d);
+                    kw[u][0] = x.x; kw[u][1] = x.y; kw[u][2] = x.z; kw[u][3] = x.w;
+                    ks[u][0] = y.x; ks[u][1] = y.y;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(p);
+                    kw[u][0] = x.x; kw[u][1] = x.y;
+                    ks[u][0] = *reinterpret_cast<const uint32_t*>(d);
+                }
+            }
+        };
+        auto load_v = [&](uint32_t i) {
+            const size_t o = (size_t)i * kTile;
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                const uint8_t* p = vq + (o + k) * (D / 2) + kv4_place(g, k) * (NB * 2u);
+                const __half* d = vd + (o + k) * NB;
+                if constexpr (BV == 2) {
+                    vw[k] = *reinterpret_cast<const uint32_t*>(p);
+                    vs[k] = *reinterpret_cast<const uint32_t*>(d);
+                } else {
+                    vw[k] = *reinterpret_cast<const uint16_t*>(p);
+                    vs[k] = *reinterpret_cast<const uint16_t*>(d);
+                }
+            }
+        };
+        uint32_t v_exp = 1;
+        bool ok = true;                              // after a wait that ran out the warps still meet at their barrier
+        if (tiles) {
+            load_k(0);
+            load_v(0);
+        }
+#pragma unroll 1
+        for (uint32_t i = 0; i < tiles; ++i) {
+            const uint32_t buf = i & 1u, round = i >> 1;
+            // the tile's largest scales, from what the warps hold
+            __half2 mk = __float2half2_rn(0.0f), mv = mk;
+#pragma unroll
+            for (uint32_t u = 0; u < KU; ++u)
+#pragma unroll
+                for (uint32_t b = 0; b < NB / 2; ++b) mk = __hmax2_nan(mk, __habs2(as_h2(ks[u][b])));
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) mv = __hmax2_nan(mv, __habs2(as_h2(vs[k])));
+            uint32_t xk = max(as_u32(mk) & 0xFFFFu, as_u32(mk) >> 16), xv = max(as_u32(mv) & 0xFFFFu, as_u32(mv) >> 16);
+            xk = __reduce_max_sync(0xFFFFFFFFu, xk);
+            xv = __reduce_max_sync(0xFFFFFFFFu, xv);
+            if (xk >= 0x7C00u) {
+                uint32_t x = 0;
+#pragma unroll
+                for (uint32_t u = 0; u < KU; ++u)
+#pragma unroll
+                    for (uint32_t b = 0; b < NB / 2; ++b) x = max(x, finite_most(ks[u][b]));
+                xk = __reduce_max_sync(0xFFFFFFFFu, x);
+            }
+            if (xv >= 0x7C00u) {
+                uint32_t x = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) x = max(x, finite_most(vs[k]));
+                xv = __reduce_max_sync(0xFFFFFFFFu, x) | 0x8000u;
+            }
+            if (lane == 0) {
+                c.most[buf][dw][0] = xk;
+                c.most[buf][dw][1] = xv;
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * S::DW) : "memory");
+            uint32_t bad = 0;
+            xk = xv = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < S::DW; ++w) {
+                const uint2 v = *reinterpret_cast<const uint2*>(c.most[buf][w]);
+                xk = max(xk, v.x);
+                xv = max(xv, v.y & 0x7FFFu);
+                bad |= v.y >> 15;
+            }
+            const uint32_t k_exp = min(max(xk >> 10, 1u), kFarExp);
+            v_exp = min(max(v_exp, xv >> 10), kFarExp);
+            const bool far = max(xk, xv) >> 10 > kFarExp;
+            if (tid == 128) c.info[i & 3u] = TileInfo{pow2((int)k_exp - 15), v_exp, bad, far};
+            __half2 k_one[KU], v_one[4];             // powers of two that take the scales to [1, 2) at most
+#pragma unroll
+            for (uint32_t u = 0; u < KU; ++u) k_one[u] = to_one(k_exp);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) v_one[k] = to_one(v_exp);
+            if (far) {
+#pragma unroll
+                for (uint32_t u = 0; u < KU; ++u) {
+                    uint32_t own = k_exp;
+#pragma unroll
+                    for (uint32_t b = 0; b < NB / 2; ++b) own = max(own, finite_most(ks[u][b]) >> 10);
+                    k_one[u] = to_one(own);
+                    if (kt == 0) c.cell_k[i & 3u][kc + 8u * u] = pow2((int)(own - k_exp));
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) {
+                    uint32_t x = finite_most(vs[k]);
+#pragma unroll
+                    for (uint32_t o = 8; o < (BV == 2 ? 16u : 32u); o <<= 1) x = max(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
+                    const uint32_t own = max(v_exp, x >> 10);
+                    if (g == 0 && vb == 0) c.cell_v[i & 3u][8u * vg + k] = (float)(own - v_exp);
+                    const __half2 one = to_one(own);
+                    v_one[k / 2] = k & 1u ? __lows2half2(v_one[k / 2], one) : __lows2half2(one, one);
+                }
+            }
+            if (bad) {
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) vs[k] = finite_only(vs[k]);
+            }
+            // K
+            if (i >= 2) ok = __all_sync(0xFFFFFFFFu, ok && bar_wait(&c.k_free[buf], (round - 1u) & 1u, &c.abort));
+            if (!ok) continue;
+            uint8_t* kb = sm + S::K_AT + buf * S::KV_TERM * S::TERMS;
+#pragma unroll
+            for (uint32_t u = 0; u < KU; ++u)
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) {
+                    const uint32_t x = __byte_perm(kw[u][b / 2], kw[u][NB / 2 + b / 2], b & 1u ? 0x7632 : 0x5410);
+                    const uint32_t s = ks[u][b / 2];
+                    const __half2 d = __hmul2(as_h2(__byte_perm(s, s, b & 1u ? 0x3232 : 0x1010)), k_one[u]);
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const __half2 n = codes(x, j), y = __hmul2(n, d);
+                        h[j] = as_u32(y);
+                        if (PRECISE) l[j] = as_u32(__hfma2(n, d, __hneg2(y)));
+                    }
+                    uint8_t* p = kb + (4u * b + kt) * (kTile * 16u) + (kc + 8u * u) * 16u;
+                    *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
+                    if (PRECISE) *reinterpret_cast<uint4*>(p + S::KV_TERM) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(&c.k_full[buf]);
+            if (i + 1u < tiles) load_k(i + 1u);
+            // V
+            if (i >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.v_free[buf], (round - 1u) & 1u, &c.abort));
+            if (!ok) continue;
+            if (v_live) {
+                uint8_t* vo = sm + S::V_AT + buf * S::KV_TERM * S::TERMS + vg * (D * 16u);
+#pragma unroll
+                for (uint32_t b = 0; b < BV; ++b) {
+                    uint32_t x[4];
+                    __half2 d[4];
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        x[k] = __byte_perm(vw[2 * k], vw[2 * k + 1], b ? 0x7632 : 0x5410);
+                        d[k] = __hmul2(as_h2(__byte_perm(vs[2 * k], vs[2 * k + 1], b ? 0x7632 : 0x5410)), v_one[k]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t h[4], l[4];
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) {
+                            const __half2 n = codes(x[k], j), y = __hmul2(n, d[k]);
+                            h[k] = as_u32(y);
+                            if (PRECISE) l[k] = as_u32(__hfma2(n, d[k], __hneg2(y)));
+                        }
+                        // row j D / 4 + 8 (block) + g holds value 32 (block) + 4 g + j
+                        uint8_t* p = vo + ((uint32_t)j * (D / 4) + 8u * (vb + b) + g) * 16u;
+                        *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
+                        if (PRECISE) *reinterpret_cast<uint4*>(p + S::KV_TERM) = make_uint4(l[0], l[1], l[2], l[3]);
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(&c.v_full[buf]);
+            if (i + 1u < tiles) load_v(i + 1u);
+        }
     } else {
         // ---- softmax: this thread's row
         const uint32_t mine = tmem + ((warp * 32u) << 16);
@@ -510,44 +514,48 @@ __global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_t
         bool ok = true;
         // the cells that all rows of the warp see; rows behind the group's last lose nothing
         const int32_t all_lo = __reduce_max_sync(0xFFFFFFFFu, row < rows ? lo : 0), all_hi = __reduce_min_sync(0xFFFFFFFFu, row < rows ? hi : 0x7FFFFFFF);
-        for (uint32_t i = 0; i < tiles; ++i) {
-            const uint32_t buf = i & 1u;
+#pragma unroll 1
+        for (uint32_t i = 0; ok && i < tiles; ++i) {
+            const uint32_t buf = i & 1u, at = mine + buf * kTile;
             const int32_t c0 = (int32_t)((tile0 + i) * kTile);
             ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.s_full[buf], (i >> 1) & 1u, &c.abort));
             if (!ok) break;
             fence_after();
-            uint32_t raw[64];
-            tmem_ld32(mine + buf * kTile, raw);
-            tmem_ld32(mine + buf * kTile + 32u, raw + 32);
             const TileInfo info = c.info[i & 3u];
+            const bool open = c0 >= all_lo && c0 + (int32_t)kTile <= all_hi;
+            float f = qs * info.k_unscale;
+            if (info.far) {                          // seldom: scores with the cells' own powers of two, put back for what follows
+#pragma unroll 1
+                for (uint32_t k = 0; k < kTile; k += 8) {
+                    uint32_t x[8];
+                    tmem_ld8(at + k, x);
+                    tmem_wait_ld8(x);
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; ++j) x[j] = __float_as_uint(fmaf(__uint_as_float(x[j]) * f, c.cell_k[i & 3u][k + j], c.cell_v[i & 3u][k + j]));
+                    tmem_st8(at + k, x);
+                }
+                tmem_wait_st();
+                f = 1.0f;
+            }
+            uint32_t raw[64];
+            tmem_ld32(at, raw);
+            tmem_ld32(at + 32u, raw + 32);
             tmem_wait_ld64(raw);
-            const float f = qs * info.k_unscale;
+#pragma unroll
+            for (int j = 0; j < 64; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * f);
+            if (!open) {                             // bit j of the words: the row sees cell c0 + j
+                const int32_t from = min(max(lo - c0, 0), 64), to = min(max(hi - c0, from), 64);
+                const unsigned long long bits = (to >= 64 ? ~0ull : (1ull << to) - 1ull) & ~(from >= 64 ? ~0ull : (1ull << from) - 1ull);
+                const uint32_t w0 = (uint32_t)bits, w1 = (uint32_t)(bits >> 32);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    raw[j] = w0 >> j & 1u ? raw[j] : 0xFF800000u;
+                    raw[32 + j] = w1 >> j & 1u ? raw[32 + j] : 0xFF800000u;
+                }
+            }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (c0 >= all_lo && c0 + (int32_t)kTile <= all_hi) {
 #pragma unroll
-                for (int j = 0; j < 64; ++j) {
-                    const float s = __uint_as_float(raw[j]) * f;
-                    raw[j] = __float_as_uint(s);
-                    top[j & 3] = fmaxf(top[j & 3], s);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 64; ++j) {
-                    const float s = c0 + j >= lo && c0 + j < hi ? __uint_as_float(raw[j]) * f : -INFINITY;
-                    raw[j] = __float_as_uint(s);
-                    top[j & 3] = fmaxf(top[j & 3], s);
-                }
-            }
-            if (info.far) {                          // seldom: the cells' own powers of two
-                top[0] = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 64; ++j) {
-                    const float s = fmaf(__uint_as_float(raw[j]), c.cell_k[i & 3u][j], c.cell_v[i & 3u][j]);
-                    raw[j] = __float_as_uint(s);
-                    top[0] = fmaxf(top[0], s);
-                }
-                top[1] = top[2] = top[3] = top[0];
-            }
+            for (int j = 0; j < 64; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(raw[j]));
             const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             if (__any_sync(0xFFFFFFFFu, most > m + 8.0f || info.v_exp != v_exp)) {
                 const float now = fmaxf(m, most), base = now == -INFINITY ? 0.0f : now, down = ex2(m - base);
@@ -559,46 +567,62 @@ __global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_t
                     if (!ok) break;
                     fence_after();
                     const float both = down * pow2((int)v_exp - (int)info.v_exp);
+#pragma unroll 1
+                    for (uint32_t k = 0; k < D; k += 16) {
+                        uint32_t o[16];
+                        tmem_ld8(mine + S::O_COL + k, o);
+                        tmem_ld8(mine + S::O_COL + k + 8u, o + 8);
+                        tmem_wait_ld8(o);
+                        tmem_wait_ld8(o + 8);
 #pragma unroll
-                    for (uint32_t k = 0; k < D / 32; ++k) {
-                        uint32_t o[32];
-                        tmem_ld32(mine + S::O_COL + 32u * k, o);
-                        tmem_wait_ld(o);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * both);
-                        tmem_st32(mine + S::O_COL + 32u * k, o);
+                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * both);
+                        tmem_st8(mine + S::O_COL + k, o);
+                        tmem_st8(mine + S::O_COL + k + 8u, o + 8);
                     }
                 }
                 v_exp = info.v_exp;
             }
             const float up = m == -INFINITY ? 0.0f : 6.0f - m;
-            float sum[4] = {};
-            uint32_t hw[32], lw[32];
+            float sum[4] = {}, far_sum = 0.0f;
+            if (info.far) {                          // the sum takes the weights without V's powers of two
+#pragma unroll 1
+                for (uint32_t k = 0; k < kTile; k += 8) {
+                    uint32_t x[8];
+                    tmem_ld8(at + k, x);
+                    tmem_wait_ld8(x);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const float p0 = ex2(__uint_as_float(raw[2 * j]) + up), p1 = ex2(__uint_as_float(raw[2 * j + 1]) + up);
-                if (!info.far) {
-                    sum[j & 1] += p0;
-                    sum[2 + (j & 1)] += p1;
-                } else {
-                    sum[0] += p0 * ex2(-c.cell_v[i & 3u][2 * j]);
-                    sum[2] += p1 * ex2(-c.cell_v[i & 3u][2 * j + 1]);
-                }
-                const __half2 h = __floats2half2_rn(p0, p1);
-                hw[j] = as_u32(h);
-                if (PRECISE) {
-                    const float2 back = __half22float2(h);
-                    lw[j] = as_u32(__floats2half2_rn(p0 - back.x, p1 - back.y));
+                    for (uint32_t j = 0; j < 8; ++j) {
+                        const int32_t cell = c0 + (int32_t)(k + j);
+                        if (cell >= lo && cell < hi) far_sum += ex2(__uint_as_float(x[j]) - c.cell_v[i & 3u][k + j] + up);
+                    }
+                    __syncwarp();
                 }
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_st32(mine + buf * kTile, hw);
-            if (PRECISE) tmem_st32(mine + buf * kTile + kTile / 2u, lw);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {            // sixteen cells at a time: eight words of each term
+                uint32_t hw[8], lw[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float p0 = ex2(__uint_as_float(raw[16 * k + 2 * j]) + up), p1 = ex2(__uint_as_float(raw[16 * k + 2 * j + 1]) + up);
+                    sum[j & 1] += p0;
+                    sum[2 + (j & 1)] += p1;
+                    const __half2 h = __floats2half2_rn(p0, p1);
+                    hw[j] = as_u32(h);
+                    if (PRECISE) {
+                        const float2 back = __half22float2(h);
+                        lw[j] = as_u32(__floats2half2_rn(p0 - back.x, p1 - back.y));
+                    }
+                }
+                tmem_st8(at + 8u * k, hw);
+                if (PRECISE) tmem_st8(at + kTile / 2u + 8u * k, lw);
+            }
+            l += info.far ? far_sum : (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_wait_st();
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(&c.p_full[buf]);
             if (info.bad) {                          // seldom: which of the blocks left out of V this row would have met
+#pragma unroll 1
                 for (uint32_t j = 0; j < kTile; ++j) {
                     if (c0 + (int32_t)j < lo || c0 + (int32_t)j >= hi) continue;
                     const __half* d = a.vd + ((size_t)hk * a.n_alloc + (uint32_t)c0 + j) * NB;
@@ -607,10 +631,8 @@ __global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_t
                 }
             }
         }
-        if (ok && row < rows) {
-            const bool any = tiles != 0;
-            if (any) ok = bar_wait(&c.v_free[(tiles - 1u) & 1u], ((tiles - 1u) >> 1) & 1u, &c.abort);
-        }
+        // every product has ended: the outputs are there, and the tensor memory may go
+        if (ok && tiles) ok = bar_wait(&c.v_free[(tiles - 1u) & 1u], ((tiles - 1u) >> 1) & 1u, &c.abort);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (ok) {
             fence_after();
@@ -642,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, TcShape<D, PRECISE>::MIN_CTAS) fa4_t
     }
     fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 0) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
     }
@@ -660,7 +682,7 @@ cudaError_t launch(const Fa4Args& a, uint32_t units, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         if (dev < 64) done[dev] = true;
     }
-    fa4_tc_kernel<T, D, PRECISE><<<units, kThreads, S::BYTES, st>>>(a);
+    fa4_tc_kernel<T, D, PRECISE><<<units, S::THREADS, S::BYTES, st>>>(a);
     return cudaGetLastError();
 }
 
