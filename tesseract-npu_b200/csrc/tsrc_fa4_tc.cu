@@ -275,40 +275,43 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
     const uint32_t tiles = last > first ? ((uint32_t)last + kTile - 1u) / kTile - tile0 : 0u;
 
     if (warp == 4u + S::DW) {
-        // ---- products, issued by one thread
-        if (lane == 0) {
-            const uint32_t q_at = smem_u32(sm), k_at = q_at + S::K_AT, v_at = q_at + S::V_AT;
-            auto scores = [&](uint32_t i) {              // S(i)
+        // ---- products, issued by one thread. Descriptors are made once and advanced by constants: made anew for every
+        // product they cost the issuing thread 90 cycles each, more than a 128 x 64 x 16 product takes (48).
+        uint32_t one;
+        asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+        if (one) {
+            const uint64_t q_op = operand(smem_u32(sm), kRows), k_op = operand(smem_u32(sm) + S::K_AT, kTile), v_op = operand(smem_u32(sm) + S::V_AT, D);
+            auto scores = [&](uint32_t i) {          // S(i)
                 const uint32_t buf = i & 1u;
                 // it takes the place of P(i - 2)
                 if (i >= 2 && !bar_wait(&c.v_free[buf], ((i - 2u) >> 1) & 1u, &c.abort)) return false;
                 if (!bar_wait(&c.k_full[buf], (i >> 1) & 1u, &c.abort)) return false;
                 fence_after();
+                const uint64_t kb = k_op + buf * (S::KV_TERM * S::TERMS >> 4);
+                const uint32_t to = tmem + buf * kTile;
 #pragma unroll
-                for (uint32_t k = 0; k < (PRECISE ? 3u : 1u); ++k) {       // q k, q_lo k, q k_lo
-                    const uint32_t qa = q_at + (k == 1 ? S::Q_TERM : 0u), kb = k_at + buf * S::KV_TERM * S::TERMS + (k == 2 ? S::KV_TERM : 0u);
+                for (uint32_t k = 0; k < (PRECISE ? 3u : 1u); ++k)     // q k, q_lo k, q k_lo
 #pragma unroll
                     for (uint32_t s = 0; s < D / 16; ++s)
-                        mma_ss(tmem + buf * kTile, operand(qa + s * 2u * kRows * 16u, kRows), operand(kb + s * 2u * kTile * 16u, kTile),
+                        mma_ss(to, q_op + ((k == 1 ? S::Q_TERM : 0u) + s * 2u * kRows * 16u >> 4), kb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * kTile * 16u >> 4),
                                instruction(kTile), k + s != 0u);
-                }
                 commit(&c.k_free[buf]);
                 commit(&c.s_full[buf]);
                 bar_arrive(&c.s_full[buf]);
                 return true;
             };
-            auto outputs = [&](uint32_t i) {             // O += P(i) V
+            auto outputs = [&](uint32_t i) {         // O += P(i) V
                 const uint32_t buf = i & 1u;
                 if (!bar_wait(&c.v_full[buf], (i >> 1) & 1u, &c.abort) || !bar_wait(&c.p_full[buf], (i >> 1) & 1u, &c.abort)) return false;
                 fence_after();
+                const uint64_t vb = v_op + buf * (S::KV_TERM * S::TERMS >> 4);
+                const uint32_t pa = tmem + buf * kTile;
 #pragma unroll
-                for (uint32_t k = 0; k < (PRECISE ? 3u : 1u); ++k) {       // p v, p_lo v, p v_lo
-                    const uint32_t pa = tmem + buf * kTile + (k == 1 ? kTile / 2u : 0u);
-                    const uint32_t vb = v_at + buf * S::KV_TERM * S::TERMS + (k == 2 ? S::KV_TERM : 0u);
+                for (uint32_t k = 0; k < (PRECISE ? 3u : 1u); ++k)     // p v, p_lo v, p v_lo
 #pragma unroll
                     for (uint32_t s = 0; s < kTile / 16; ++s)
-                        mma_ts(tmem + S::O_COL, pa + 8u * s, operand(vb + s * 2u * D * 16u, D), instruction(D), i + k + s != 0u);
-                }
+                        mma_ts(tmem + S::O_COL, pa + (k == 1 ? kTile / 2u : 0u) + 8u * s, vb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * D * 16u >> 4),
+                               instruction(D), k + s == 0u ? i : 1u);
                 commit(&c.v_free[buf]);
                 return true;
             };
