@@ -103,12 +103,25 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 // comes from one more mma per block with 8 2^-24 in every row. The blocks' scales stay out of the products: K's
 // multiply the four (two) partial sums of a score in f32; V's multiply the weights: w = p dV, a set for each block.
 //   Precision: q and w are two fp16 terms each, 22 bits (q scaled by a power of two per row); for bf16 outputs one
-// term, 11 bits. Running maximum, sum and outputs are f32.
+// term, 11 bits. Running maximum, sum and outputs are f32. The tensor cores align a subnormal operand's products as
+// if it were 2^-14, so up to seven of the sum's 24 bits are lost that way (measured: 2^-17 of the largest product at
+// worst, 1.4e-5 of an output row): enough for 16-bit outputs; f32 outputs take n - 8 as an ordinary fp16, one fused
+// step more for two codes, and need neither start value nor weights' sum (1e-6).
 template <class T, int D, int MODE, bool MASK>
 __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_dec_kernel(Fa4Args a) {
     using S = DecShape<D>;
     constexpr uint32_t NB = S::NB, R = kRowsOf<MODE>, NT = R / 8;        // NT: columns of eight rows
-    constexpr bool SPLIT = MODE == kRows8Split;
+    constexpr bool SPLIT = MODE == kRows8Split, WHOLE = std::is_same_v<T, float>;     // WHOLE: operands are n - 8
+    // a word's codes as operands: those in the low four bits, those in the next four
+    auto even = [](uint32_t x) {
+        x &= 0x000F000Fu;
+        return WHOLE ? as_u32(__hsub2(as_h2(x | 0x64006400u), __float2half2_rn(1032.0f))) : x;
+    };
+    auto odd = [](uint32_t x) {
+        x &= 0x00F000F0u;
+        return WHOLE ? as_u32(__hfma2(as_h2(x | 0x64006400u), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f))) : x;
+    };
+    constexpr float kOdd = WHOLE ? 1.0f : 0.0625f;               // makes up for the odd codes' place
     extern __shared__ __align__(128) uint8_t sm[];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t = lane & 3u;
     const uint32_t team = warp / S::NG, sub = warp % S::NG;
@@ -216,7 +229,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
         // the row's largest value to [2^12, 2^13); rows of tiny values by 2^100 at most
         const int e = min(12 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
-        const float f = pow2(e), mine = a.scale * kLog2e * (pow2(-e) * 16777216.0f);
+        const float f = pow2(e), mine = a.scale * kLog2e * (pow2(-e) * (WHOLE ? 1.0f : 16777216.0f));
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) rs[n][i] = __shfl_sync(0xFFFFFFFFu, mine, 8u * t + 4u * i);
 #pragma unroll
@@ -235,12 +248,12 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
 #pragma unroll
                 for (uint32_t j = 0; j < 2; ++j) {
                     qb[n][k][b][j][0] = pack2(y[2 * j], y[2 * j + 4]);
-                    qb[n][k][b][j][1] = pack2(y[2 * j + 1] * 0.0625f, y[2 * j + 5] * 0.0625f);
+                    qb[n][k][b][j][1] = pack2(y[2 * j + 1] * kOdd, y[2 * j + 5] * kOdd);
                 }
             }
             sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
             sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-            sum *= -8.0f / 16777216.0f;
+            sum *= WHOLE ? 0.0f : -8.0f / 16777216.0f;
 #pragma unroll
             for (uint32_t i = 0; i < 2; ++i) start[n][b][i] = __shfl_sync(0xFFFFFFFFu, sum, 8u * t + 4u * i);
         }
@@ -316,20 +329,18 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
                 const uint32_t x0 = w[0][b], x1 = w[1][b], y0 = x0 >> 8, y1 = x1 >> 8;
-                const float2 f0 = __half22float2(as_h2(d[0][b / 2])), f1 = __half22float2(as_h2(d[1][b / 2]));
-                const float d0 = b & 1u ? f0.y : f0.x, d1 = b & 1u ? f1.y : f1.x;
+                const uint32_t e0 = even(x0), e1 = even(x1), o0 = odd(x0), o1 = odd(x1);
+                const uint32_t f0 = even(y0), f1 = even(y1), p0 = odd(y0), p1 = odd(y1);
+                const float2 g0 = __half22float2(as_h2(d[0][b / 2])), g1 = __half22float2(as_h2(d[1][b / 2]));
+                const float d0 = b & 1u ? g0.y : g0.x, d1 = b & 1u ? g1.y : g1.x;
 #pragma unroll
                 for (uint32_t n = 0; n < NT; ++n) {
-                    float c[4];
-                    mma16816(c, x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u, qb[n][0][b][0][0], qb[n][0][b][0][1],
-                             start[n][b][0], start[n][b][1], start[n][b][0], start[n][b][1]);
-                    mma16816(c, y0 & 0x000F000Fu, y1 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x00F000F0u, qb[n][0][b][1][0], qb[n][0][b][1][1],
-                             c[0], c[1], c[2], c[3]);
-                    if constexpr (SPLIT) {
-                        mma16816(c, x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u, qb[n][1][b][0][0], qb[n][1][b][0][1],
-                                 c[0], c[1], c[2], c[3]);
-                        mma16816(c, y0 & 0x000F000Fu, y1 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x00F000F0u, qb[n][1][b][1][0], qb[n][1][b][1][1],
-                                 c[0], c[1], c[2], c[3]);
+                    // the small term first: its roundings are then relative to it alone
+                    float c[4] = {start[n][b][0], start[n][b][1], start[n][b][0], start[n][b][1]};
+#pragma unroll
+                    for (uint32_t k = SPLIT ? 2 : 1; k-- > 0;) {
+                        mma16816(c, e0, e1, o0, o1, qb[n][k][b][0][0], qb[n][k][b][0][1], c[0], c[1], c[2], c[3]);
+                        mma16816(c, f0, f1, p0, p1, qb[n][k][b][1][0], qb[n][k][b][1][1], c[0], c[1], c[2], c[3]);
                     }
                     acc[n][0] = fmaf(c[0], d0, acc[n][0]);
                     acc[n][1] = fmaf(c[1], d0, acc[n][1]);
@@ -514,20 +525,22 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
                 const uint32_t sel = b & 1u ? 0x7632 : 0x5410;
                 const uint32_t x0 = __byte_perm(v[0][b / 2], v[1][b / 2], sel), x1 = __byte_perm(v[2][b / 2], v[3][b / 2], sel);
                 const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
+                const uint32_t e0 = even(x0), e1 = even(x1), o0 = odd(x0), o1 = odd(x1);
+                const uint32_t f0 = even(y0), f1 = even(y1), p0 = odd(y0), p1 = odd(y1);
 #pragma unroll
                 for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
                     for (uint32_t k = 0; k < (SPLIT ? 2u : 1u); ++k) {
                         const uint32_t b0 = wb[n][k][2 * ks][b], b1 = wb[n][k][2 * ks + 1][b];
                         float (&p)[4] = o[n][b][0];
-                        mma16816(p, x0 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x000F000Fu, x1 & 0x00F000F0u, b0, b1, p[0], p[1], p[2], p[3]);
+                        mma16816(p, e0, o0, e1, o1, b0, b1, p[0], p[1], p[2], p[3]);
                         float (&q)[4] = o[n][b][1];
-                        mma16816(q, y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u, b0, b1, q[0], q[1], q[2], q[3]);
+                        mma16816(q, f0, p0, f1, p1, b0, b1, q[0], q[1], q[2], q[3]);
                     }
             }
         }
 #pragma unroll
-        for (uint32_t n = 0; n < NT; ++n)
+        for (uint32_t n = 0; n < NT && !WHOLE; ++n)
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
                 constexpr uint32_t k8 = 0x00080008u;
@@ -549,7 +562,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
 
     // the warp's results in its ring: [R][W] outputs without their scales; maxima and sums beside the rings
     float* wo = reinterpret_cast<float*>(ringp);
-    const float unscale = pow2(24 - value_exp(vexp)), pinv = pow2(-weight_exp(vexp));
+    const float unscale = pow2((WHOLE ? 0 : 24) - value_exp(vexp)), pinv = pow2(-weight_exp(vexp));
 #pragma unroll
     for (uint32_t n = 0; n < NT; ++n) {
 #pragma unroll
@@ -560,7 +573,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
                 for (uint32_t i = 0; i < 2; ++i) {
                     float* p = wo + (8u * n + 2u * t + i) * S::W + 32u * b + 4u * g + 2u * k;
                     p[0] = (o[n][b][k][i] - wsum[n][b][i]) * (unscale * pinv);
-                    p[1] = (o[n][b][k][2 + i] * 0.0625f - wsum[n][b][i]) * (unscale * pinv);
+                    p[1] = (o[n][b][k][2 + i] * kOdd - wsum[n][b][i]) * (unscale * pinv);
                 }
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {

@@ -33,17 +33,26 @@ __device__ unsigned int g_fa4_error;                 // kKv4ErrWait once a wait 
 constexpr uint32_t kTile = 64, kRows = 128;
 constexpr long long kWaitCycles = 1ll << 31;         // a wait gives up after ~1 s of SM clock
 
-template <int D, bool PRECISE> struct TcShape {
+template <class T, int D> struct TcShape {
+    static constexpr bool PRECISE = !std::is_same_v<T, __nv_bfloat16>;              // two terms of K, V and the weights
+    static constexpr bool TOTAL = std::is_same_v<T, float>;                         // two of q (fp16 is one), outputs in total
     static constexpr uint32_t NB = D / 32, TERMS = PRECISE ? 2 : 1;
     static constexpr uint32_t Q_TERM = kRows * D * 2, KV_TERM = kTile * D * 2;      // bytes of one term of an operand
-    static constexpr uint32_t K_AT = Q_TERM * TERMS, V_AT = K_AT + 2 * KV_TERM * TERMS;
+    static constexpr uint32_t K_AT = Q_TERM * (TOTAL ? 2 : 1), V_AT = K_AT + 2 * KV_TERM * TERMS;
     static constexpr uint32_t CTL_AT = V_AT + 2 * KV_TERM * TERMS;
     // two CTAs an SM at most: tensor memory holds no more
     static constexpr uint32_t BYTES = CTL_AT + 3072 < 100 * 1024 ? 100 * 1024 : CTL_AT + 3072;
     static constexpr uint32_t MIN_CTAS = 2 * (BYTES + 1024) <= 227 * 1024 ? 2 : 1;
     static constexpr uint32_t DW = MIN_CTAS == 1 ? 8 : 4, THREADS = 160 + 32 * DW;   // dequant warps
     static constexpr uint32_t KU = 8 / DW, BV = 8 / DW;                             // a lane's cells of K, blocks of V
-    static constexpr uint32_t O_COL = 2 * kTile;                                    // tensor-memory columns: S, S, O
+    // tensor-memory columns: score buffers (P over each), O. With four, S(i + 1) need not wait for the products of
+    // P(i - 1), and the tensor cores never stop; two CTAs on an SM have room for two each.
+    static constexpr uint32_t NS = MIN_CTAS == 1 ? 4 : 2, O_COL = NS * kTile, COLUMNS = MIN_CTAS == 1 ? 512 : 256;
+    // The tensor cores cut every sum towards zero, about 2^-25 of it a product, so a row's output would shrink by 1e-5
+    // over 60 tiles of twelve products. For f32 outputs FLUSH tiles are added up there, and then to the total, in tensor
+    // memory too, by an ordinary f32 addition.
+    static constexpr uint32_t FLUSH = 4, SUM_COL = O_COL + D;
+    static_assert(SUM_COL + (TOTAL ? D : 0) <= COLUMNS, "tensor memory");
 };
 
 struct TileInfo {
@@ -55,14 +64,15 @@ struct TileInfo {
 constexpr uint32_t kFarExp = 19;     // exponent field of scales of 16 to 32, the largest that the common powers follow
 
 struct Control {                     // at most 3 KB
-    uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2];
+    uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[4], p_full[4];
     TileInfo info[4];
     // far tiles: what a cell's scores are times, and what the log2 of its weights is raised by. Of four tiles, as info:
     // the dequant warps are up to two tiles ahead of the softmax when they write these.
     float cell_k[4][kTile], cell_v[4][kTile];
     uint32_t most[2][8][2];  // the dequant warps' largest |d| of K and V, by tile parity
     uint32_t tmem, abort;
-    int32_t span[4][4];      // the softmax warps' first and last cell, and the cells that all their rows see
+    int32_t span[4][2];      // the softmax warps' first and last cell
+    float q_unscale[kRows];
 };
 
 static_assert(sizeof(Control) <= 3072, "room behind the operands");
@@ -174,15 +184,92 @@ __device__ __forceinline__ void store4(T* p, const float (&x)[4], bool wide) {
         for (int i = 0; i < 4; ++i) p[i] = from_f32<T>(x[i]);
     }
 }
-// codes 4 j.. of two halves side by side, as n - 8
-__device__ __forceinline__ __half2 codes(uint32_t x, int j) {
-    const uint32_t u = ((x >> (4 * j)) & 0x000F000Fu) | 0x64006400u;
-    return __hsub2(as_h2(u), __float2half2_rn(1032.0f));
+// Codes i = 0..3 of two halves side by side (four bits each) times d, that is d (n - 8), as operand words.
+//   Two terms: n - 8 without rounding from the fp16 whose last bits are n (1024 + n, or 1024 + 16 n with the code in
+// the next four bits), then the rounded product and what it lacks.
+//   One term: a code in the last bits of an fp16 is the subnormal number n 2^-24 (n 2^-20 in the next four), so one
+// fused step with 2^14 d (2^10 d) and -8 2^-10 d gives d (n - 8) 2^-10, rounded once; d is below 2, so 2^14 d fits.
+template <bool PRECISE> struct Scaled;
+template <> struct Scaled<true> {
+    static constexpr int UNDO = 0;               // log2 of what the operand lacks
+    __half2 d;
+    __device__ __forceinline__ explicit Scaled(__half2 s) : d(s) {}
+    __device__ __forceinline__ void words(uint32_t x, uint32_t (&h)[4], uint32_t (&l)[4]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t y = j & 2 ? x >> 8 : x;
+            const __half2 n = j & 1 ? __hfma2(as_h2((y & 0x00F000F0u) | 0x64006400u), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f))
+                                    : __hsub2(as_h2((y & 0x000F000Fu) | 0x64006400u), __float2half2_rn(1032.0f));
+            const __half2 w = __hmul2(n, d);
+            h[j] = as_u32(w);
+            l[j] = as_u32(__hfma2(n, d, __hneg2(w)));
+        }
+    }
+};
+template <> struct Scaled<false> {
+    static constexpr int UNDO = 10;
+    __half2 a, b, c;
+    __device__ __forceinline__ explicit Scaled(__half2 s)
+        : a(__hmul2(s, __float2half2_rn(16384.0f))), b(__hmul2(s, __float2half2_rn(1024.0f))), c(__hmul2(s, __float2half2_rn(-0.0078125f))) {}
+    __device__ __forceinline__ void words(uint32_t x, uint32_t (&h)[4], uint32_t (&)[4]) const {
+        const uint32_t y = x >> 8;
+        h[0] = as_u32(__hfma2(as_h2(x & 0x000F000Fu), a, c));
+        h[1] = as_u32(__hfma2(as_h2(x & 0x00F000F0u), b, c));
+        h[2] = as_u32(__hfma2(as_h2(y & 0x000F000Fu), a, c));
+        h[3] = as_u32(__hfma2(as_h2(y & 0x00F000F0u), b, c));
+    }
+};
+
+// O times f
+template <int D>
+__device__ __forceinline__ void rescale(uint32_t o_at, float f) {
+#pragma unroll 1
+    for (uint32_t k = 0; k < D; k += 16) {
+        uint32_t o[16];
+        tmem_ld8(o_at + k, o);
+        tmem_ld8(o_at + k + 8u, o + 8);
+        tmem_wait_ld8(o);
+        tmem_wait_ld8(o + 8);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+        tmem_st8(o_at + k, o);
+        tmem_st8(o_at + k + 8u, o + 8);
+    }
+}
+// The total (none before the first) and O times f; flush: O goes into the total.
+template <int D>
+__device__ __forceinline__ void settle(uint32_t o_at, uint32_t sum_at, float f, bool none, bool flush) {
+    if (none && !flush) return rescale<D>(o_at, f);
+#pragma unroll 1
+    for (uint32_t k = 0; k < D; k += 16) {
+        uint32_t o[16], t[16];
+        tmem_ld8(o_at + k, o);
+        tmem_ld8(o_at + k + 8u, o + 8);
+        tmem_ld8(sum_at + k, t);
+        tmem_ld8(sum_at + k + 8u, t + 8);
+        tmem_wait_ld8(o);
+        tmem_wait_ld8(o + 8);
+        tmem_wait_ld8(t);
+        tmem_wait_ld8(t + 8);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float x = __uint_as_float(o[j]), y = none ? 0.0f : __uint_as_float(t[j]);
+            t[j] = __float_as_uint((flush ? x + y : y) * f);
+            o[j] = __float_as_uint(x * f);
+        }
+        tmem_st8(sum_at + k, t);
+        tmem_st8(sum_at + k + 8u, t + 8);
+        if (!flush) {
+            tmem_st8(o_at + k, o);
+            tmem_st8(o_at + k + 8u, o + 8);
+        }
+    }
 }
 
-template <class T, int D, bool PRECISE>
-__global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECISE>::MIN_CTAS) fa4_tc_kernel(Fa4Args a) {
-    using S = TcShape<D, PRECISE>;
+template <class T, int D>
+__global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTAS) fa4_tc_kernel(Fa4Args a) {
+    using S = TcShape<T, D>;
+    constexpr bool PRECISE = S::PRECISE, TOTAL = S::TOTAL;
     constexpr uint32_t NB = S::NB;
     extern __shared__ __align__(1024) uint8_t sm[];
     Control& c = *reinterpret_cast<Control*>(sm + S::CTL_AT);
@@ -194,7 +281,7 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
     const uint32_t tok = grp * a.group + row / a.G, head = hk * a.G + row % a.G;
 
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&c.tmem)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)), "n"(S::COLUMNS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         if (lane == 0) {
             c.abort = 0;
@@ -203,6 +290,8 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
                 bar_init(&c.k_free[i], 1);
                 bar_init(&c.v_full[i], S::DW);
                 bar_init(&c.v_free[i], 1);
+            }
+            for (int i = 0; i < 4; ++i) {
                 bar_init(&c.s_full[i], 2);           // the tensor cores, and the issuing thread for what it has seen
                 bar_init(&c.p_full[i], 4);
             }
@@ -210,7 +299,6 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
         }
     }
     int32_t lo = 0, hi = 0;
-    float qs = 0.0f;                                 // this row's scale, for scores in log2
     if (warp < 4) {
         if (row < rows) {
             hi = (int32_t)a.n_kv;
@@ -225,43 +313,46 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
             c.span[warp][0] = first;
             c.span[warp][1] = last;
         }
-        // q: the row's largest value to [2^12, 2^13), chunks of eight in the order 0 4 1 5 2 6 3 7 that K has
-        const T* q = static_cast<const T*>(a.q) + (size_t)tok * a.q_stride + (size_t)head * D;
-        float top = 0.0f;
-        if (row < rows) {
-#pragma unroll 2
-            for (uint32_t e = 0; e < D; e += 8) {
-                float x[8];
-                if (a.q_wide) load8<T, true>(q + e, x);
-                else load8<T, false>(q + e, x);
+    }
+    // q, eight rows at a time by a warp: the row's largest value to [2^12, 2^13), chunks of eight values in the order
+    // 0 4 1 5 2 6 3 7 that K has
+    for (uint32_t r0 = 8u * warp; warp < 4u + S::DW && r0 < kRows; r0 += 8u * (4u + S::DW)) {
+        const uint32_t r = r0 + (lane & 7u), row_r = rt * kRows + r;
+        const uint32_t tok_r = grp * a.group + row_r / a.G, head_r = hk * a.G + row_r % a.G;
+        const T* q = static_cast<const T*>(a.q) + (size_t)tok_r * a.q_stride + (size_t)head_r * D + 8u * (lane >> 3);
+        float x[D / 32][8], top = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+        for (uint32_t j = 0; j < D / 32; ++j) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
+            if (row_r < rows) {
+                if (a.q_wide) load8<T, true>(q + 32u * j, x[j]);
+                else load8<T, false>(q + 32u * j, x[j]);
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));
         }
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
         const int e2 = min(12 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
         const float f = pow2(e2);
-        qs = a.scale * 1.4426950408889634f * pow2(-e2);
-#pragma unroll 2
-        for (uint32_t e = 0; e < D; e += 8) {
-            float x[8] = {};
-            if (row < rows) {
-                if (a.q_wide) load8<T, true>(q + e, x);
-                else load8<T, false>(q + e, x);
-            }
-            uint32_t w[2][4];
+        if (lane < 8) c.q_unscale[r] = a.scale * 1.4426950408889634f * pow2(-e2);
+#pragma unroll
+        for (uint32_t j = 0; j < D / 32; ++j) {
+            uint32_t h[4], l[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float u = x[i] * f, v = x[i + 4] * f;
-                const __half2 h = __floats2half2_rn(u, v);
-                w[0][i] = as_u32(h);
-                if (PRECISE) {
-                    const float2 back = __half22float2(h);
-                    w[1][i] = as_u32(__floats2half2_rn(u - back.x, v - back.y));
+                const float u = x[j][i] * f, v = x[j][i + 4] * f;
+                const __half2 w = __floats2half2_rn(u, v);
+                h[i] = as_u32(w);
+                if (TOTAL) {
+                    const float2 back = __half22float2(w);
+                    l[i] = as_u32(__floats2half2_rn(u - back.x, v - back.y));
                 }
             }
-#pragma unroll
-            for (uint32_t k = 0; k < S::TERMS; ++k)
-                *reinterpret_cast<uint4*>(sm + k * S::Q_TERM + (e / 8u) * (kRows * 16u) + tid * 16u) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+            uint8_t* p = sm + (4u * j + (lane >> 3)) * (kRows * 16u) + r * 16u;
+            *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
+            if (TOTAL) *reinterpret_cast<uint4*>(p + S::Q_TERM) = make_uint4(l[0], l[1], l[2], l[3]);
         }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -282,36 +373,40 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
         if (one) {
             const uint64_t q_op = operand(smem_u32(sm), kRows), k_op = operand(smem_u32(sm) + S::K_AT, kTile), v_op = operand(smem_u32(sm) + S::V_AT, D);
             auto scores = [&](uint32_t i) {          // S(i)
-                const uint32_t buf = i & 1u;
-                // it takes the place of P(i - 2)
-                if (i >= 2 && !bar_wait(&c.v_free[buf], ((i - 2u) >> 1) & 1u, &c.abort)) return false;
+                const uint32_t buf = i & 1u, sb = i % S::NS;
+                // it takes the place of P(i - 2), or of P(i - 4): then the products of P(i - 3), the latest whose phase is
+                // still the barrier's last, are waited for
+                constexpr uint32_t BACK = S::NS == 2 ? 2 : 3;
+                if (i >= BACK && !bar_wait(&c.v_free[(i - BACK) & 1u], ((i - BACK) >> 1) & 1u, &c.abort)) return false;
                 if (!bar_wait(&c.k_full[buf], (i >> 1) & 1u, &c.abort)) return false;
                 fence_after();
                 const uint64_t kb = k_op + buf * (S::KV_TERM * S::TERMS >> 4);
-                const uint32_t to = tmem + buf * kTile;
+                const uint32_t to = tmem + sb * kTile;
 #pragma unroll
-                for (uint32_t k = 0; k < (PRECISE ? 3u : 1u); ++k)     // q k, q_lo k, q k_lo
+                for (uint32_t k = PRECISE ? 3 : 1; k-- > 0;) {         // q k_lo, q_lo k, q k: the small ones first, so that
+                    if (k == 1 && !TOTAL) continue;                    // what is cut from them is small
 #pragma unroll
                     for (uint32_t s = 0; s < D / 16; ++s)
                         mma_ss(to, q_op + ((k == 1 ? S::Q_TERM : 0u) + s * 2u * kRows * 16u >> 4), kb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * kTile * 16u >> 4),
-                               instruction(kTile), k + s != 0u);
+                               instruction(kTile), k != (PRECISE ? 2u : 0u) || s != 0u);
+                }
                 commit(&c.k_free[buf]);
-                commit(&c.s_full[buf]);
-                bar_arrive(&c.s_full[buf]);
+                commit(&c.s_full[sb]);
+                bar_arrive(&c.s_full[sb]);
                 return true;
             };
             auto outputs = [&](uint32_t i) {         // O += P(i) V
-                const uint32_t buf = i & 1u;
-                if (!bar_wait(&c.v_full[buf], (i >> 1) & 1u, &c.abort) || !bar_wait(&c.p_full[buf], (i >> 1) & 1u, &c.abort)) return false;
+                const uint32_t buf = i & 1u, sb = i % S::NS;
+                if (!bar_wait(&c.v_full[buf], (i >> 1) & 1u, &c.abort) || !bar_wait(&c.p_full[sb], (i / S::NS) & 1u, &c.abort)) return false;
                 fence_after();
                 const uint64_t vb = v_op + buf * (S::KV_TERM * S::TERMS >> 4);
-                const uint32_t pa = tmem + buf * kTile;
+                const uint32_t pa = tmem + sb * kTile;
 #pragma unroll
-                for (uint32_t k = 0; k < (PRECISE ? 3u : 1u); ++k)     // p v, p_lo v, p v_lo
+                for (uint32_t k = PRECISE ? 3 : 1; k-- > 0;)           // p v_lo, p_lo v, p v
 #pragma unroll
                     for (uint32_t s = 0; s < kTile / 16; ++s)
                         mma_ts(tmem + S::O_COL, pa + (k == 1 ? kTile / 2u : 0u) + 8u * s, vb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * D * 16u >> 4),
-                               instruction(D), k + s == 0u ? i : 1u);
+                               instruction(D), k == (PRECISE ? 2u : 0u) && s == 0u ? (TOTAL ? i % S::FLUSH : i) : 1u);
                 commit(&c.v_free[buf]);
                 return true;
             };
@@ -418,7 +513,7 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
             const uint32_t k_exp = min(max(xk >> 10, 1u), kFarExp);
             v_exp = min(max(v_exp, xv >> 10), kFarExp);
             const bool far = max(xk, xv) >> 10 > kFarExp;
-            if (tid == 128) c.info[i & 3u] = TileInfo{pow2((int)k_exp - 15), v_exp, bad, far};
+            if (tid == 128) c.info[i & 3u] = TileInfo{pow2((int)k_exp - 15 + Scaled<PRECISE>::UNDO), v_exp, bad, far};
             __half2 k_one[KU], v_one[4];             // powers of two that take the scales to [1, 2) at most
 #pragma unroll
             for (uint32_t u = 0; u < KU; ++u) k_one[u] = to_one(k_exp);
@@ -460,12 +555,7 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
                     const uint32_t s = ks[u][b / 2];
                     const __half2 d = __hmul2(as_h2(__byte_perm(s, s, b & 1u ? 0x3232 : 0x1010)), k_one[u]);
                     uint32_t h[4], l[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const __half2 n = codes(x, j), y = __hmul2(n, d);
-                        h[j] = as_u32(y);
-                        if (PRECISE) l[j] = as_u32(__hfma2(n, d, __hneg2(y)));
-                    }
+                    Scaled<PRECISE>(d).words(x, h, l);
                     uint8_t* p = kb + (4u * b + kt) * (kTile * 16u) + (kc + 8u * u) * 16u;
                     *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
                     if (PRECISE) *reinterpret_cast<uint4*>(p + S::KV_TERM) = make_uint4(l[0], l[1], l[2], l[3]);
@@ -477,41 +567,41 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
             // V
             if (i >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.v_free[buf], (round - 1u) & 1u, &c.abort));
             if (!ok) continue;
+            uint32_t cw[8], cs[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                cw[k] = vw[k];
+                cs[k] = vs[k];
+            }
+            if (i + 1u < tiles) load_v(i + 1u);
             if (v_live) {
                 uint8_t* vo = sm + S::V_AT + buf * S::KV_TERM * S::TERMS + vg * (D * 16u);
 #pragma unroll
                 for (uint32_t b = 0; b < BV; ++b) {
-                    uint32_t x[4];
-                    __half2 d[4];
+                    uint32_t h[4][4], l[4][4];       // [cell pair][value]
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k) {
-                        x[k] = __byte_perm(vw[2 * k], vw[2 * k + 1], b ? 0x7632 : 0x5410);
-                        d[k] = __hmul2(as_h2(__byte_perm(vs[2 * k], vs[2 * k + 1], b ? 0x7632 : 0x5410)), v_one[k]);
+                        const uint32_t x = __byte_perm(cw[2 * k], cw[2 * k + 1], b ? 0x7632 : 0x5410);
+                        const __half2 d = __hmul2(as_h2(__byte_perm(cs[2 * k], cs[2 * k + 1], b ? 0x7632 : 0x5410)), v_one[k]);
+                        Scaled<PRECISE>(d).words(x, h[k], l[k]);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        uint32_t h[4], l[4];
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            const __half2 n = codes(x[k], j), y = __hmul2(n, d[k]);
-                            h[k] = as_u32(y);
-                            if (PRECISE) l[k] = as_u32(__hfma2(n, d[k], __hneg2(y)));
-                        }
                         // row j D / 4 + 8 (block) + g holds value 32 (block) + 4 g + j
                         uint8_t* p = vo + ((uint32_t)j * (D / 4) + 8u * (vb + b) + g) * 16u;
-                        *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
-                        if (PRECISE) *reinterpret_cast<uint4*>(p + S::KV_TERM) = make_uint4(l[0], l[1], l[2], l[3]);
+                        *reinterpret_cast<uint4*>(p) = make_uint4(h[0][j], h[1][j], h[2][j], h[3][j]);
+                        if (PRECISE) *reinterpret_cast<uint4*>(p + S::KV_TERM) = make_uint4(l[0][j], l[1][j], l[2][j], l[3][j]);
                     }
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) bar_arrive(&c.v_full[buf]);
-            if (i + 1u < tiles) load_v(i + 1u);
         }
     } else {
         // ---- softmax: this thread's row
         const uint32_t mine = tmem + ((warp * 32u) << 16);
+        const float qs = c.q_unscale[tid];           // this row's scale, for scores in log2
         float m = -INFINITY, l = 0.0f;               // reference of the weights' exponents; running sum, both in units of 2^6 p
         uint32_t v_exp = 1, lost = 0;                // lost: blocks of V in which the row sees a scale that is no number
         bool ok = true;
@@ -519,9 +609,9 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
         const int32_t all_lo = __reduce_max_sync(0xFFFFFFFFu, row < rows ? lo : 0), all_hi = __reduce_min_sync(0xFFFFFFFFu, row < rows ? hi : 0x7FFFFFFF);
 #pragma unroll 1
         for (uint32_t i = 0; ok && i < tiles; ++i) {
-            const uint32_t buf = i & 1u, at = mine + buf * kTile;
+            const uint32_t buf = i & 1u, sb = i % S::NS, at = mine + sb * kTile;
             const int32_t c0 = (int32_t)((tile0 + i) * kTile);
-            ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.s_full[buf], (i >> 1) & 1u, &c.abort));
+            ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.s_full[sb], (i / S::NS) & 1u, &c.abort));
             if (!ok) break;
             fence_after();
             const TileInfo info = c.info[i & 3u];
@@ -560,30 +650,25 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
 #pragma unroll
             for (int j = 0; j < 64; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(raw[j]));
             const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            if (__any_sync(0xFFFFFFFFu, most > m + 8.0f || info.v_exp != v_exp)) {
-                const float now = fmaxf(m, most), base = now == -INFINITY ? 0.0f : now, down = ex2(m - base);
-                l *= down;
-                m = now;
+            const bool raise = __any_sync(0xFFFFFFFFu, most > m + 8.0f || info.v_exp != v_exp);
+            const bool flush = TOTAL && i > 0 && i % S::FLUSH == 0u;
+            if (raise || flush) {
+                float both = 1.0f;
+                if (raise) {
+                    const float now = fmaxf(m, most), base = now == -INFINITY ? 0.0f : now, down = ex2(m - base);
+                    l *= down;
+                    m = now;
+                    both = down * pow2((int)v_exp - (int)info.v_exp);
+                    v_exp = info.v_exp;
+                }
                 if (i > 0) {
                     // the products so far have to be there
                     ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.v_free[buf ^ 1u], ((i - 1u) >> 1) & 1u, &c.abort));
                     if (!ok) break;
                     fence_after();
-                    const float both = down * pow2((int)v_exp - (int)info.v_exp);
-#pragma unroll 1
-                    for (uint32_t k = 0; k < D; k += 16) {
-                        uint32_t o[16];
-                        tmem_ld8(mine + S::O_COL + k, o);
-                        tmem_ld8(mine + S::O_COL + k + 8u, o + 8);
-                        tmem_wait_ld8(o);
-                        tmem_wait_ld8(o + 8);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * both);
-                        tmem_st8(mine + S::O_COL + k, o);
-                        tmem_st8(mine + S::O_COL + k + 8u, o + 8);
-                    }
+                    if constexpr (TOTAL) settle<D>(mine + S::O_COL, mine + S::SUM_COL, both, i <= S::FLUSH, flush);
+                    else rescale<D>(mine + S::O_COL, both);
                 }
-                v_exp = info.v_exp;
             }
             const float up = m == -INFINITY ? 0.0f : 6.0f - m;
             float sum[4] = {}, far_sum = 0.0f;
@@ -623,7 +708,7 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
             tmem_wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(&c.p_full[buf]);
+            if (lane == 0) bar_arrive(&c.p_full[sb]);
             if (info.bad) {                          // seldom: which of the blocks left out of V this row would have met
 #pragma unroll 1
                 for (uint32_t j = 0; j < kTile; ++j) {
@@ -639,7 +724,7 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (ok) {
             fence_after();
-            const float f = l == 0.0f ? 0.0f : pow2((int)v_exp - 15) / l;
+            const float f = l == 0.0f ? 0.0f : pow2((int)v_exp - 15 + Scaled<PRECISE>::UNDO) / l;
             T* out = static_cast<T*>(a.out) + (size_t)tok * a.out_stride + (size_t)head * D;
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
@@ -648,6 +733,14 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j) tmem_ld8(mine + S::O_COL + j * (D / 4) + 8u * b, o + 8 * j);
                     tmem_wait_ld(o);
+                    if (TOTAL && tiles > S::FLUSH) {
+                        uint32_t t[32];
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j) tmem_ld8(mine + S::SUM_COL + j * (D / 4) + 8u * b, t + 8 * j);
+                        tmem_wait_ld(t);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(t[j]));
+                    }
                 }
                 if (row < rows) {
 #pragma unroll
@@ -669,32 +762,32 @@ __global__ void __launch_bounds__(TcShape<D, PRECISE>::THREADS, TcShape<D, PRECI
     __syncthreads();
     if (warp == 0) {
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::COLUMNS));
     }
 }
 
-template <class T, int D, bool PRECISE>
+template <class T, int D>
 cudaError_t launch(const Fa4Args& a, uint32_t units, cudaStream_t st) {
-    using S = TcShape<D, PRECISE>;
+    using S = TcShape<T, D>;
     static bool done[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !done[dev]) {
-        e = cudaFuncSetAttribute(fa4_tc_kernel<T, D, PRECISE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
+        e = cudaFuncSetAttribute(fa4_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
         if (e != cudaSuccess) return e;
         if (dev < 64) done[dev] = true;
     }
-    fa4_tc_kernel<T, D, PRECISE><<<units, S::THREADS, S::BYTES, st>>>(a);
+    fa4_tc_kernel<T, D><<<units, S::THREADS, S::BYTES, st>>>(a);
     return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_fa4_tc(uint32_t type, uint32_t D, const Fa4Args& a, uint32_t units, cudaStream_t st) {
-    if (type == TSRC_TYPE_F32) return D == 64u ? launch<float, 64, true>(a, units, st) : launch<float, 128, true>(a, units, st);
-    if (type == TSRC_TYPE_F16) return D == 64u ? launch<__half, 64, true>(a, units, st) : launch<__half, 128, true>(a, units, st);
-    return D == 64u ? launch<__nv_bfloat16, 64, false>(a, units, st) : launch<__nv_bfloat16, 128, false>(a, units, st);
+    if (type == TSRC_TYPE_F32) return D == 64u ? launch<float, 64>(a, units, st) : launch<float, 128>(a, units, st);
+    if (type == TSRC_TYPE_F16) return D == 64u ? launch<__half, 64>(a, units, st) : launch<__half, 128>(a, units, st);
+    return D == 64u ? launch<__nv_bfloat16, 64>(a, units, st) : launch<__nv_bfloat16, 128>(a, units, st);
 }
 
 cudaError_t fa4_error(uint32_t* code, bool clear) {
