@@ -1,6 +1,7 @@
 // tsrc_fa4.cu -- attention over the q4_0 KV cache (tsrc_flash_attn_q4). Cache layout: tsrc_kv4.cuh.
 #include <cmath>
 #include <cstdio>
+#include <type_traits>
 
 #include "tsrc_fa4.cuh"
 
@@ -46,11 +47,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return as_u32(__
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float remote_f32(const float* p, uint32_t rank) {
+__device__ __forceinline__ float4 remote_f32x4(const float4* p, uint32_t rank) {
     uint32_t at;
-    float v;
+    float4 v;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
     return v;
 }
 
@@ -64,10 +65,11 @@ enum : int {
 template <int MODE> constexpr uint32_t kRowsOf = MODE == kRows16 ? 16u : 8u;
 
 template <int D> struct DecShape {
+    static constexpr uint32_t WARPS = kDecWarps;
     static constexpr uint32_t NB = D == 64 ? 2 : 4;            // blocks of a warp's group of values
     static constexpr uint32_t W = NB * 32;                      // values of a group: a warp's share of the head
     static constexpr uint32_t NG = D / W;                       // warps of a team: they share a tile's scores
-    static constexpr uint32_t TEAMS = kDecWarps / NG;
+    static constexpr uint32_t TEAMS = WARPS / NG;
     static constexpr uint32_t ROW = W / 2, DS = NB * 2;         // bytes of a cell's codes and scales in a group
     static constexpr uint32_t V_AT = kDecTile * ROW, KD_AT = 2 * kDecTile * ROW, VD_AT = KD_AT + kDecTile * DS;
     static constexpr uint32_t STAGE = VD_AT + kDecTile * DS;
@@ -75,10 +77,10 @@ template <int D> struct DecShape {
 };
 // ring (later the warps' results), the warps' and the CTA's maxima and sums, the score exchange of teams (two turns)
 // or the factors of a cluster's CTAs
-constexpr uint32_t kRedBytes = (kDecWarps + 1u) * 16u * 3u * 4u;
 template <int D, int MODE> __host__ __device__ constexpr uint32_t dec_smem() {
     using S = DecShape<D>;
-    return kDecWarps * S::RING + kRedBytes + (S::NG > 1 ? 2u * kDecWarps * 32u : kMaxCluster + 1u) * kRowsOf<MODE> * 4u;
+    constexpr uint32_t WARPS = kDecWarps;
+    return WARPS * S::RING + (WARPS + 1u) * 16u * 16u + (S::NG > 1 ? 2u * WARPS * 32u : kMaxCluster + 4u) * kRowsOf<MODE> * 4u;
 }
 
 // The weights' scale, by the exponent field v of the largest |dV| met: p is taken times 2^weight_exp(v) and, where
@@ -110,6 +112,7 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 template <class T, int D, int MODE, bool MASK>
 __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_dec_kernel(Fa4Args a) {
     using S = DecShape<D>;
+    constexpr uint32_t WARPS = kDecWarps;
     constexpr uint32_t NB = S::NB, R = kRowsOf<MODE>, NT = R / 8;        // NT: columns of eight rows
     constexpr bool SPLIT = MODE == kRows8Split, WHOLE = std::is_same_v<T, float>;     // WHOLE: operands are n - 8
     // a word's codes as operands: those in the low four bits, those in the next four
@@ -130,8 +133,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
     const uint32_t rows = a.group * a.G;
     uint8_t* ringp = sm + warp * S::RING;
     const uint32_t ring = smem_u32(ringp);
-    float* red = reinterpret_cast<float*>(sm + kDecWarps * S::RING);     // [warps + 1][16][3]
-    float* xch = red + kRedBytes / 4u;
+    float4* red = reinterpret_cast<float4*>(sm + WARPS * S::RING);       // [warps + 1][16]: mask reference, maximum, sum; then factors
+    float* xch = reinterpret_cast<float*>(red + (WARPS + 1u) * 16u);
 
     // the cells of this lane's rows (8 n + 2 t + i), and the hull of all rows
     int32_t lo[NT][2], hi[NT][2], first = 0x7FFFFFFF, last = 0, all_lo = 0, all_hi = 0x7FFFFFFF;
@@ -212,9 +215,10 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
             const T* q = static_cast<const T*>(a.q) + (size_t)(grp * a.group + row / a.G) * a.q_stride +
                          (size_t)(hk * a.G + row % a.G) * D + sub * S::W + 8u * t;
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b)
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) x[b][i] = to_f32(q[32u * b + i]);
+            for (uint32_t b = 0; b < NB; ++b) {
+                if (a.q_wide) load8<T, true>(q + 32u * b, x[b]);
+                else load8<T, false>(q + 32u * b, x[b]);
+            }
         } else {
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b)
@@ -358,11 +362,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
         }
         if constexpr (S::NG > 1) {
             // the team's partial scores, added in the order of the groups
-            float* mine = xch + (turn * kDecWarps + warp) * NT * 8u * 32u + lane;
+            float* mine = xch + (turn * WARPS + warp) * NT * 8u * 32u + lane;
 #pragma unroll
             for (uint32_t k = 0; k < NT * 8u; ++k) mine[k * 32u] = s[k / 8u][k / 4u % 2u][k % 4u];
             asm volatile("bar.sync %0, %1;" ::"r"(1u + team), "n"(32 * S::NG) : "memory");
-            const float* all = xch + (turn * kDecWarps + team * S::NG) * NT * 8u * 32u + lane;
+            const float* all = xch + (turn * WARPS + team * S::NG) * NT * 8u * 32u + lane;
 #pragma unroll
             for (uint32_t k = 0; k < NT * 8u; ++k) {
                 float x = all[k * 32u];
@@ -580,110 +584,114 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
             float x = l[n][i] * pinv;
 #pragma unroll
             for (uint32_t k = 4; k < 32; k <<= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, k);
-            if (g == 0) {
-                float* p = red + (warp * 16u + 8u * n + 2u * t + i) * 3u;
-                p[0] = MASK ? off[n][i] : 0.0f;
-                p[1] = m[n][i];
-                p[2] = x;
-            }
+            if (g == 0) red[warp * 16u + 8u * n + 2u * t + i] = make_float4(MASK ? off[n][i] : 0.0f, m[n][i], x, 0.0f);
         }
     }
     __syncthreads();
-    // the CTA's teams, added in order, into the first team's place
+    // Each team's factor for each row (a thread per row, in order), the CTA's maximum and sum; then the teams' outputs,
+    // four values a thread, into the first team's place.
     auto result = [&](uint32_t j, uint32_t r, uint32_t d) {
-        return reinterpret_cast<float*>(sm + (j * S::NG + d / S::W) * S::RING) + r * S::W + d % S::W;
+        return reinterpret_cast<float4*>(sm + (j * S::NG + d / S::W) * S::RING) + (r * S::W + d % S::W) / 4u;
     };
-    float* fin = red + kDecWarps * 16u * 3u;
-    for (uint32_t e = tid; e < R * D; e += kDecWarps * 32u) {
-        const uint32_t r = e / D, d = e % D;
-        float ot = -INFINITY, mt = -INFINITY, lt = 0.0f, acc = 0.0f, sh[S::TEAMS];
+    float4* fin = red + WARPS * 16u;
+    if (tid < R) {
+        const uint32_t r = tid;
+        float ot = -INFINITY, mt = -INFINITY, lt = 0.0f;
+        if (MASK) {
 #pragma unroll
-        for (uint32_t j = 0; j < S::TEAMS; ++j) ot = fmaxf(ot, red[(j * S::NG * 16u + r) * 3u]);
-#pragma unroll
-        for (uint32_t j = 0; j < S::TEAMS; ++j) {
-            const float* p = red + (j * S::NG * 16u + r) * 3u;
-            sh[j] = !MASK || p[0] == ot || p[1] == -INFINITY ? p[1] : p[1] + (p[0] - ot) * kLog2e;
-            mt = fmaxf(mt, sh[j]);
+            for (uint32_t j = 0; j < S::TEAMS; ++j) ot = fmaxf(ot, red[j * S::NG * 16u + r].x);
         }
+        auto level = [&](const float4& p) { return !MASK || p.x == ot || p.y == -INFINITY ? p.y : p.y + (p.x - ot) * kLog2e; };
+#pragma unroll
+        for (uint32_t j = 0; j < S::TEAMS; ++j) mt = fmaxf(mt, level(red[j * S::NG * 16u + r]));
         const float base = mt == -INFINITY ? 0.0f : mt;
 #pragma unroll
         for (uint32_t j = 0; j < S::TEAMS; ++j) {
-            const float lj = red[(j * S::NG * 16u + r) * 3u + 2u];
-            if (lj == 0.0f) continue;                            // a team that saw nothing of the row
-            const float f = ex2(sh[j] - base);
-            lt += f * lj;
-            acc += f * *result(j, r, d);
+            const float4 p = red[j * S::NG * 16u + r];
+            const float f = p.z == 0.0f ? 0.0f : ex2(level(p) - base);       // a team that saw nothing of the row: 0
+            lt += f * p.z;
+            red[j * S::NG * 16u + r].w = f;
         }
-        *result(0, r, d) = acc;
-        if (d == 0) {
-            fin[r * 3u] = ot;
-            fin[r * 3u + 1u] = mt;
-            fin[r * 3u + 2u] = lt;
-        }
+        fin[r] = make_float4(ot, mt, lt, 0.0f);
     }
     __syncthreads();
+    for (uint32_t e = tid; e < R * D / 4u; e += WARPS * 32u) {
+        const uint32_t r = e / (D / 4u), d = e % (D / 4u) * 4u;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (uint32_t j = 0; j < S::TEAMS; ++j) {
+            const float f = red[j * S::NG * 16u + r].w;
+            if (f == 0.0f) continue;
+            const float4 x = *result(j, r, d);
+            acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+        }
+        *result(0, r, d) = acc;
+    }
+    __syncthreads();
+    const uint32_t used = min(R, rows - rt * R);
     if (a.splits > 1u && a.part_o) {                             // joined by the merge kernel
-        for (uint32_t e = tid; e < R * D; e += kDecWarps * 32u) {
-            const uint32_t r = e / D, d = e % D;
-            if (rt * R + r >= rows) break;
+        for (uint32_t e = tid; e < used * D / 4u; e += WARPS * 32u) {
+            const uint32_t r = e / (D / 4u), d = e % (D / 4u) * 4u;
             const size_t at = ((size_t)unit * a.splits + split) * R + r;
-            a.part_o[at * D + d] = *result(0, r, d);
-            if (d == 0) *reinterpret_cast<float4*>(a.part_ml + at * 4u) = make_float4(fin[r * 3u], fin[r * 3u + 1u], fin[r * 3u + 2u], 0.0f);
+            *reinterpret_cast<float4*>(a.part_o + at * D + d) = *result(0, r, d);
+            if (d == 0) *reinterpret_cast<float4*>(a.part_ml + at * 4u) = fin[r];
         }
         return;
     }
-    // the cluster's CTAs, added in order: each finishes its share of the outputs
-    const uint32_t used = min(R, rows - rt * R);
-    float* share = xch;                                          // [R][splits + 1]: each CTA's factor, then 1 / sum
-    if (a.splits > 1u) {
-        cluster_sync();
-        // a half warp per row, a lane per CTA
-        for (uint32_t e = tid; e < R * kMaxCluster; e += kDecWarps * 32u) {
-            const uint32_t r = e / kMaxCluster, k = e % kMaxCluster;
-            float ot = -INFINITY, mt = -INFINITY, lt = 0.0f;
-            if (k < a.splits) {
-                if (MASK) ot = remote_f32(fin + r * 3u, k);
-                mt = remote_f32(fin + r * 3u + 1u, k);
-                lt = remote_f32(fin + r * 3u + 2u, k);
-            }
-            if (MASK) {
-                float top = ot;
-#pragma unroll
-                for (uint32_t x = 1; x < kMaxCluster; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-                if (ot != top && mt != -INFINITY) mt += (ot - top) * kLog2e;
-            }
-            float top = mt;
+    auto put = [&](uint32_t r, uint32_t d, float4 x, float l) {
+        const uint32_t row = rt * R + r, tok = grp * a.group + row / a.G, h = hk * a.G + row % a.G;
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+        float y[4] = {x.x * f, x.y * f, x.z * f, x.w * f};
+        if (l == 0.0f) y[0] = y[1] = y[2] = y[3] = 0.0f;
+        T* p = static_cast<T*>(a.out) + (size_t)tok * a.out_stride + (size_t)h * D + d;
+        store4<T>(p, y, a.out_wide);
+    };
+    if (a.splits == 1u) {
+        for (uint32_t e = tid; e < used * D / 4u; e += WARPS * 32u) {
+            const uint32_t r = e / (D / 4u), d = e % (D / 4u) * 4u;
+            put(r, d, *result(0, r, d), fin[r].z);
+        }
+        return;
+    }
+    // The cluster's CTAs, in order: each takes its share of the outputs. A thread per row and CTA finds the factors.
+    float* share = xch;                                          // [R][kMaxCluster + 4]: each CTA's factor, then the sum
+    cluster_sync();
+    for (uint32_t e = tid; e < R * kMaxCluster; e += WARPS * 32u) {
+        const uint32_t r = e / kMaxCluster, k = e % kMaxCluster;
+        float4 p = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
+        if (k < a.splits) p = remote_f32x4(fin + r, k);
+        if (MASK) {
+            float top = p.x;
 #pragma unroll
             for (uint32_t x = 1; x < kMaxCluster; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-            const float f = lt == 0.0f ? 0.0f : ex2(mt - (top == -INFINITY ? 0.0f : top));
-            float sum = lt == 0.0f ? 0.0f : f * lt;
-#pragma unroll
-            for (uint32_t x = 1; x < kMaxCluster; x <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
-            share[r * (kMaxCluster + 1u) + k] = f;
-            if (k == 0) share[r * (kMaxCluster + 1u) + kMaxCluster] = sum;
+            if (p.x != top && p.y != -INFINITY) p.y += (p.x - top) * kLog2e;
         }
-        __syncthreads();
-    }
-    for (uint32_t e = split * kDecWarps * 32u + tid; e < used * D; e += a.splits * kDecWarps * 32u) {
-        const uint32_t r = e / D, d = e % D, row = rt * R + r;
-        float lt, acc;
-        if (a.splits == 1u) {
-            lt = fin[r * 3u + 2u];
-            acc = *result(0, r, d);
-        } else {
-            const float* f = share + r * (kMaxCluster + 1u);
-            float x[kMaxCluster];
+        float top = p.y;
 #pragma unroll
-            for (uint32_t k = 0; k < kMaxCluster; ++k) x[k] = k < a.splits ? remote_f32(result(0, r, d), k) : 0.0f;
-            lt = f[kMaxCluster];
-            acc = 0.0f;
+        for (uint32_t x = 1; x < kMaxCluster; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+        const float f = p.z == 0.0f ? 0.0f : ex2(p.y - (top == -INFINITY ? 0.0f : top));
+        float sum = p.z == 0.0f ? 0.0f : f * p.z;
 #pragma unroll
-            for (uint32_t k = 0; k < kMaxCluster; ++k) acc += f[k] == 0.0f ? 0.0f : f[k] * x[k];
-        }
-        const uint32_t tok = grp * a.group + row / a.G, h = hk * a.G + row % a.G;
-        static_cast<T*>(a.out)[(size_t)tok * a.out_stride + (size_t)h * D + d] = from_f32<T>(lt == 0.0f ? 0.0f : acc / lt);
+        for (uint32_t x = 1; x < kMaxCluster; x <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+        share[r * (kMaxCluster + 4u) + k] = f;
+        if (k == 0) share[r * (kMaxCluster + 4u) + kMaxCluster] = sum;
     }
-    if (a.splits > 1u) cluster_sync();                           // nobody's shared memory goes while it is read
+    __syncthreads();
+    for (uint32_t e = split * WARPS * 32u + tid; e < used * D / 4u; e += a.splits * WARPS * 32u) {
+        const uint32_t r = e / (D / 4u), d = e % (D / 4u) * 4u;
+        const float* f = share + r * (kMaxCluster + 4u);
+        float4 x[kMaxCluster], acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxCluster; ++k)
+            if (k < a.splits) x[k] = remote_f32x4(result(0, r, d), k);
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxCluster; ++k)
+            if (k < a.splits && f[k] != 0.0f) {
+                acc.x += f[k] * x[k].x; acc.y += f[k] * x[k].y; acc.z += f[k] * x[k].z; acc.w += f[k] * x[k].w;
+            }
+        put(r, d, acc, f[kMaxCluster]);
+    }
+    cluster_sync();                                              // nobody's shared memory goes while it is read
 }
 
 // Adds up the splits of each row in order. One CTA per row of a unit.
@@ -748,11 +756,16 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
     p.units = (T / p.group) * n_head_kv * p.row_tiles;
     const uint32_t len = max_len && max_len < n_kv ? max_len : n_kv;
     const uint32_t teams = D <= 128u ? kDecWarps : kDecWarps * 128u / D;
-    // Splits until the CTAs fill the GPU twice over, in powers of two up to a cluster's CTAs, each warp keeping a
-    // tile at least; where even clusters of sixteen leave most SMs empty and the cells are many, more splits and
-    // a merge kernel.
-    const uint32_t most = (len / kDecTile + 1u) / teams;
-    while (p.splits < kMaxCluster && p.splits * 2u <= most && p.units * p.splits < 2u * kDecCtas) p.splits *= 2u;
+    // Splits in powers of two up to a cluster's CTAs, each warp keeping a tile at least: until the GPU's places for
+    // CTAs (four an SM) are taken, since a CTA costs about three tiles' time beside its tiles (13 drafted tokens over
+    // 4113 cells, 56 units: 25.5 us with 8 splits, 38 with 16, 33 with 4); and where a warp keeps eight tiles even so,
+    // once more, which evens out what the last CTAs leave idle (64 ragged sequences, 512 units: 80 us with 2, 89
+    // with 1, 85 with 4). Where even clusters of sixteen leave most SMs empty and the cells are many, more splits and a
+    // merge kernel.
+    const uint32_t tiles = len / kDecTile + 1u, most = tiles / teams;
+    while (p.splits < kMaxCluster && p.splits * 2u <= most &&
+           (p.units * p.splits * 2u <= kDecCtas || (p.units * p.splits < kDecCtas && tiles >= 16u * teams * p.splits)))
+        p.splits *= 2u;
     if (p.units * kMaxCluster < kSms && most >= 8u * kMaxCluster) {
         p.splits = 2u * kSms / p.units;
         p.o_bytes = (size_t)p.units * p.splits * R * D * 4u;

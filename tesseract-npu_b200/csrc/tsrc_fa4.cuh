@@ -21,6 +21,25 @@ struct Fa4Args {
     float *part_o, *part_ml;                   // splits joined by the merge kernel: [unit][split][R][D], [unit][split][R][4]
 };
 
+template <class T>
+__device__ __forceinline__ void store4(T* p, const float (&x)[4], bool wide) {
+    if (wide) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        else {
+            T t[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = from_f32<T>(x[i]);
+            uint2 w;
+            w.x = (uint32_t)reinterpret_cast<const unsigned short&>(t[0]) | (uint32_t)reinterpret_cast<const unsigned short&>(t[1]) << 16;
+            w.y = (uint32_t)reinterpret_cast<const unsigned short&>(t[2]) | (uint32_t)reinterpret_cast<const unsigned short&>(t[3]) << 16;
+            *reinterpret_cast<uint2*>(p) = w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = from_f32<T>(x[i]);
+    }
+}
+
 // Many query rows on one stretch of cells: D 64 or 128, no mask, row tiles of 128 (tsrc_fa4_tc.cu).
 constexpr uint32_t kFa4TcRows = 128;
 cudaError_t launch_fa4_tc(uint32_t type, uint32_t D, const Fa4Args& a, uint32_t units, cudaStream_t st);

@@ -166,24 +166,6 @@ __device__ __forceinline__ uint32_t finite_most(uint32_t u) {
 __device__ __forceinline__ uint32_t finite_only(uint32_t u) {
     return ((u & 0x7C00u) == 0x7C00u ? 0u : u & 0xFFFFu) | ((u & 0x7C000000u) == 0x7C000000u ? 0u : u & 0xFFFF0000u);
 }
-template <class T>
-__device__ __forceinline__ void store4(T* p, const float (&x)[4], bool wide) {
-    if (wide) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-        else {
-            T t[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] = from_f32<T>(x[i]);
-            uint2 w;
-            w.x = (uint32_t)reinterpret_cast<const unsigned short&>(t[0]) | (uint32_t)reinterpret_cast<const unsigned short&>(t[1]) << 16;
-            w.y = (uint32_t)reinterpret_cast<const unsigned short&>(t[2]) | (uint32_t)reinterpret_cast<const unsigned short&>(t[3]) << 16;
-            *reinterpret_cast<uint2*>(p) = w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = from_f32<T>(x[i]);
-    }
-}
 // Codes i = 0..3 of two halves side by side (four bits each) times d, that is d (n - 8), as operand words.
 //   Two terms: n - 8 without rounding from the fp16 whose last bits are n (1024 + n, or 1024 + 16 n with the code in
 // the next four bits), then the rounded product and what it lacks.
