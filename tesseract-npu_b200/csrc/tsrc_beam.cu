@@ -5,9 +5,10 @@
 //
 // Inside a beam s grows with x, so a beam's best are those of the raw logits, which compare exactly; only the few
 // kept of each beam meet the other beams' in f64. Two kernels, the logits read once:
-//   part   one CTA per 8192 logits of a row: maximum, sum of exponentials, and the part's n_out best in order;
-//   merge  one CTA per group: a warp per beam merges its parts' ordered lists and adds up the normaliser, then one
-//          warp merges the beams' lists.
+//   part    one CTA per 8192 logits of a row: maximum and sum of exponentials, and the largest of every 32 neighbours;
+//   select  a cluster per group, a CTA per row (or several): the n_out groups of neighbours with the largest maxima
+//           hold the row's n_out best -- each has one that beats whatever the others hold -- and their few logits are
+//           read again; then the cluster's first CTA merges the rows' ordered lists.
 // A candidate is one 64-bit key, the logit's bits made monotone above the complement of its index, so that equal
 // logits go to the lowest index and no two keys are equal. Key 0 stands for none.
 #include <cmath>
@@ -22,12 +23,12 @@ namespace {
 
 constexpr uint32_t kBeamThreads = 256, kBeamEach = 32, kBeamPart = kBeamThreads * kBeamEach;
 constexpr uint32_t kBeamOut = 64, kBeamBeams = 64, kBeamVocab = 1u << 20;
-constexpr uint32_t kBeamCap = kBeamOut * kBeamEach;      // the list's room: what n_out threads can hold
-constexpr size_t kBeamSmem = 220u * 1024u;
+constexpr uint32_t kBeamCap = kBeamOut * kBeamEach;      // a list's room: what n_out threads can hold
+constexpr uint32_t kBeamLists = (kBeamVocab + 7u + kBeamPart - 1u) / kBeamPart / 32u + 1u;    // parts that a lane adds up
+constexpr uint32_t kBeamRows = 8;                        // rows that a cluster takes at once
 
 // parts of a row, with room for the up to seven values before it that its first 16 bytes may hold
 __host__ __device__ inline uint32_t beam_parts(uint32_t n_vocab) { return (n_vocab + 7u + kBeamPart - 1u) / kBeamPart; }
-constexpr uint32_t kBeamLists = (kBeamVocab + 7u + kBeamPart - 1u) / kBeamPart / 32u + 1u;    // parts that a lane merges
 
 struct BeamPart {
     float max, sum;      // sum of exp(x - max) over the part (-inf and 0 where the part is all -inf)
@@ -87,31 +88,27 @@ template <class T> struct BeamVec {
     }
 };
 
-// A part is 8192 logits from a 16-byte boundary on (`lead` of the first part's lie before the row); a thread holds
-// 32 of them in registers, as they came, for two passes: the largest, then the sum of exponentials and the few that
-// can be among the part's best. Those few are what reaches a bound below the n_out-th best, the least of n_out
-// maxima over disjoint sets of threads: about n_out (1 + 1/2 + ... + 1/n_out) of them where the large ones lie
-// scattered. Where they do not (a sorted row) the list overflows, and the exact n_out-th largest of the threads'
-// own best keys, found bit by bit, takes the bound's place: n_out threads hold all that reaches it.
-// 256 rows of 128256 bf16 logits (65.7 MB): 82 us with scalar loads and a count before the list, 37 us as here.
+// A part is 8192 logits from a 16-byte boundary on (`lead` of the first part's lie before the row), a warp's share
+// 1024 neighbours, so 32 neighbours are 4 (f32: 8) lanes of one load. Each thread adds up its 32 exponentials against its
+// own largest, without waiting for anyone.
+// 256 rows of 128256 bf16 logits (65.7 MB): 82 us with scalar loads and the best chosen in every part, 37 us with wide
+// loads, 14.7 us so (4.5 TB/s).
 template <class T>
-__global__ void __launch_bounds__(kBeamThreads, sizeof(T) == 4 ? 4 : 6) beam_part_kernel(const T* __restrict__ logits, size_t stride, uint32_t n_vocab,
-                                                                 uint32_t n_out, BeamPart* parts, unsigned long long* keys) {
+__global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const T* __restrict__ logits, size_t stride, uint32_t n_vocab, BeamPart* parts,
+                                                                 float* maxima) {
     using V = BeamVec<T>;
-    constexpr uint32_t NV = kBeamEach / V::N;
-    __shared__ unsigned long long list[kBeamCap];
+    constexpr uint32_t NV = kBeamEach / V::N, LANES = 32 / V::N;
     __shared__ float redm[8], reds[8];
-    __shared__ uint32_t least, count;
     asm volatile("griddepcontrol.launch_dependents;");
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const size_t row = blockIdx.y, at = row * gridDim.x + blockIdx.x;
     const T* x = logits + row * stride;
     const uint32_t lead = (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15u) / (uint32_t)sizeof(T);
-    const int64_t first = (int64_t)blockIdx.x * kBeamPart - lead + tid * V::N;       // this thread's first logit
+    const int64_t first = (int64_t)blockIdx.x * kBeamPart - lead + (warp * NV * 32u + lane) * V::N;
     V v[NV];
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j) {
-        const int64_t i = first + j * kBeamThreads * V::N;
+        const int64_t i = first + j * 32u * V::N;
         if (i >= 0 && i + V::N <= n_vocab) v[j].raw = __ldcs(reinterpret_cast<const uint4*>(x + i));
         else {                                                   // a row's ends
             T t[V::N];
@@ -120,36 +117,19 @@ __global__ void __launch_bounds__(kBeamThreads, sizeof(T) == 4 ? 4 : 6) beam_par
             __builtin_memcpy(&v[j].raw, t, 16);
         }
     }
-    float m = -INFINITY, tops[NV];
+    float m = -INFINITY;
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j) {
-        tops[j] = v[j].top();
-        m = fmaxf(m, tops[j]);                                   // NaN only where all are
-    }
-    // the least of n_out maxima over sets of `width` threads (all keys of floats above -inf are above 0)
-    const uint32_t mine = m > -INFINITY ? order_of(m) : 0u;
-    uint32_t width = 1;
-    while (width * 2u * n_out <= kBeamThreads && width < 32u) width *= 2u;
-    uint32_t set = mine;
-    for (uint32_t s = 1; s < width; s <<= 1) set = max(set, __shfl_xor_sync(0xFFFFFFFFu, set, s));
-    const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, tid / width < n_out ? set : 0xFFFFFFFFu);
-    const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, mine);
-    if (tid == 0) {
-        least = 0xFFFFFFFFu;
-        count = 0;
-    }
-    if (lane == 0) redm[warp] = top ? value_of(top) : -INFINITY;
-    __syncthreads();
-    if (lane == 0 && low != 0xFFFFFFFFu) atomicMin(&least, low);
-    float most = redm[0];
+        float top = v[j].top();
+        m = fmaxf(m, top);                                       // NaN is passed over
 #pragma unroll
-    for (int w = 1; w < 8; ++w) most = fmaxf(most, redm[w]);
-    __syncthreads();
-    const float bound = least ? value_of(least) : -3.4028234e38f;
-    // exp(y - most) as 2^(y L - c) 2^(c - most L), c the rounded most L, L = log2 e in f32: one fused step a logit; the
-    // second factor is near 1 while most is not far from 0
+        for (uint32_t s = 1; s < LANES; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
+        if (lane % LANES == 0) maxima[at * kBeamThreads + warp * 32u + j * (32u / LANES) + lane / LANES] = top > -INFINITY ? top : -INFINITY;
+    }
+    // exp(y - m) as 2^(y L - c) 2^(c - m L), c the rounded m L, L = log2 e in f32: one fused step a logit; the second
+    // factor is near 1 while m is not far from 0
     constexpr float L = 1.4426950408889634f;
-    const float shift = most > -INFINITY ? most : 0.0f;
+    const float shift = m > -INFINITY ? m : 0.0f;
     float sum = 0.0f;
     if (fabsf(shift) < 4096.0f) {
         const float c = shift * -L;
@@ -164,59 +144,22 @@ __global__ void __launch_bounds__(kBeamThreads, sizeof(T) == 4 ? 4 : 6) beam_par
 #pragma unroll
             for (uint32_t k = 0; k < V::N; ++k) sum += beam_ex2((v[j].at(k) - shift) * L);
     }
+    float top = m;
 #pragma unroll
-    for (uint32_t j = 0; j < NV; ++j) {
-        if (!(tops[j] >= bound)) continue;
-        const uint32_t at0 = (uint32_t)(first + j * kBeamThreads * V::N);
+    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
+    if (sum != 0.0f) sum *= beam_ex2((shift - (top > -INFINITY ? top : 0.0f)) * L);
 #pragma unroll
-        for (uint32_t k = 0; k < V::N; ++k) {
-            const float y = v[j].at(k);
-            if (y >= bound) {                                    // false for -inf and NaN
-                const uint32_t n = atomicAdd(&count, 1u);
-                if (n < kBeamCap) list[n] = key_of(y, at0 + k);
-            }
-        }
-    }
     for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, s);
-    if (lane == 0) reds[warp] = sum;
+    if (lane == 0) {
+        redm[warp] = top;
+        reds[warp] = sum;
+    }
     __syncthreads();
-    if (count > kBeamCap) {
-        unsigned long long best = 0, limit = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < NV; ++j)
-#pragma unroll
-            for (uint32_t k = 0; k < V::N; ++k) {
-                const unsigned long long key = key_of(v[j].at(k), (uint32_t)(first + j * kBeamThreads * V::N + k));
-                best = key > best ? key : best;
-            }
-        for (int bit = 63; bit >= 0; --bit) {
-            const unsigned long long trial = limit | (1ull << bit);
-            if (__syncthreads_count(best >= trial) >= (int)n_out) limit = trial;
-        }
-        if (tid == 0) count = 0;
-        __syncthreads();
-#pragma unroll
-        for (uint32_t j = 0; j < NV; ++j)
-#pragma unroll
-            for (uint32_t k = 0; k < V::N; ++k) {
-                const unsigned long long key = key_of(v[j].at(k), (uint32_t)(first + j * kBeamThreads * V::N + k));
-                if (key != 0 && key >= limit) list[atomicAdd(&count, 1u)] = key;
-            }
-        __syncthreads();
-    }
-    // the list's order by counting what is larger: few are in it as a rule
-    const uint32_t n = count;
-    unsigned long long* out = keys + at * n_out;
-    for (uint32_t i = tid; i < n; i += kBeamThreads) {
-        const unsigned long long k = list[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; ++j) rank += list[j] > k ? 1u : 0u;
-        if (rank < n_out) out[rank] = k;
-    }
-    for (uint32_t i = n + tid; i < n_out; i += kBeamThreads) out[i] = 0ull;
     if (tid == 0) {
-        float total = 0.0f;
-        for (int w = 0; w < 8; ++w) total += reds[w];
+        float most = redm[0], total = 0.0f;
+        for (int w = 1; w < 8; ++w) most = fmaxf(most, redm[w]);
+        for (int w = 0; w < 8; ++w)
+            if (reds[w] != 0.0f) total += reds[w] * beam_ex2((redm[w] - (most > -INFINITY ? most : 0.0f)) * L);
         parts[at] = BeamPart{most, total};
     }
 }
@@ -227,70 +170,185 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
     return ((unsigned long long)hi << 32) | lo;
 }
 
-// One CTA per group; warp w takes beams w, w + warps, ...: it brings the beam's lists into shared memory, takes the
-// best of the lists' heads n_out times, and has the normaliser summed in f64 meanwhile.
-template <uint32_t LISTS>
-__global__ void __launch_bounds__(512) beam_merge_kernel(const BeamPart* parts, const unsigned long long* keys, uint32_t n_parts,
-                                                         const float* scores, uint32_t n_beam, uint32_t n_out, float* out_scores,
-                                                         int32_t* out_beam, int32_t* out_token) {
-    extern __shared__ unsigned long long sm[];
-    unsigned long long* val = sm;                                        // [n_beam][n_out] f64 order of s
-    uint32_t* tok = reinterpret_cast<uint32_t*>(sm + n_beam * n_out);    // [n_beam][n_out]
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    unsigned long long* mine = sm + (n_beam * n_out * 12u + 15u) / 16u * 2u + (size_t)warp * n_parts * n_out;
-    const size_t group = blockIdx.x;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (uint32_t b = warp; b < n_beam; b += warps) {
-        const size_t row = group * n_beam + b;
-        const unsigned long long* kr = keys + row * n_parts * n_out;
-        for (uint32_t i = lane; i < n_parts * n_out; i += 32u) mine[i] = kr[i];
-        const BeamPart* pr = parts + row * n_parts;
-        float top = -INFINITY;
-        for (uint32_t i = lane; i < n_parts; i += 32u) top = fmaxf(top, pr[i].max);
-        for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
-        double sum = 0.0;
-        for (uint32_t i = lane; i < n_parts; i += 32u)
-            if (pr[i].sum != 0.0f) sum += (double)pr[i].sum * exp((double)pr[i].max - (double)top);
-        for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, s);
-        const double norm = log(sum);                        // above top, so that logits far from 0 keep their digits
-        const double score = scores ? (double)scores[row] : 0.0;
-        __syncwarp();
-        uint32_t at[LISTS];
-        unsigned long long head[LISTS];
+struct SelectShared {
+    unsigned long long list[kBeamCap], best[kBeamOut];   // candidates; the chosen, in order
+    uint32_t least, count;
+};
+
+// A bound below the n_out-th largest of the values that the CTA's threads hold, m being this thread's largest: the least
+// of n_out maxima over disjoint sets of threads. About n_out (1 + 1/2 + ... + 1/n_out) values reach it where the large
+// ones lie scattered.
+__device__ __forceinline__ float select_bound(SelectShared& s, float m, uint32_t n_out) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t width = 1;
+    while (width * 2u * n_out <= kBeamThreads && width < 32u) width *= 2u;
+    uint32_t set = m > -INFINITY ? order_of(m) : 0u;
+    for (uint32_t x = 1; x < width; x <<= 1) set = max(set, __shfl_xor_sync(0xFFFFFFFFu, set, x));
+    const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, tid / width < n_out ? set : 0xFFFFFFFFu);
+    if (tid == 0) s.least = 0xFFFFFFFFu;
+    __syncthreads();
+    if ((tid & 31u) == 0 && low != 0xFFFFFFFFu) atomicMin(&s.least, low);
+    __syncthreads();
+    return s.least ? value_of(s.least) : -3.4028234e38f;
+}
+
+// The n_out largest of up to 8192 values, all of which reach `bound`, into s.best in order (0 where there are fewer);
+// value j of this thread is candidate `index(j)`. What reaches the bound is listed, and the order comes from counting
+// what is larger. Where the list overflows (sorted values, ties) the exact n_out-th largest of the threads' own best
+// keys, found bit by bit, takes the bound's place: n_out threads hold all that reaches it.
+template <class I>
+__device__ __forceinline__ void select_best(SelectShared& s, const float (&v)[kBeamEach], uint32_t used, float bound, uint32_t n_out, const I& index) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t mine = 0;
 #pragma unroll
-        for (uint32_t j = 0; j < LISTS; ++j) {
-            at[j] = (lane + 32u * j) * n_out;
-            head[j] = lane + 32u * j < n_parts ? mine[at[j]] : 0ull;
-        }
-        for (uint32_t k = 0; k < n_out; ++k) {
-            unsigned long long best = 0;
+    for (uint32_t j = 0; j < kBeamEach; ++j) mine += j < used && v[j] >= bound ? 1u : 0u;        // false for -inf and NaN
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    if (mine) {
+        uint32_t n = atomicAdd(&s.count, mine);
 #pragma unroll
-            for (uint32_t j = 0; j < LISTS; ++j) best = head[j] > best ? head[j] : best;
-            best = warp_max(best);
-#pragma unroll
-            for (uint32_t j = 0; j < LISTS; ++j)
-                if (best != 0 && head[j] == best) head[j] = ++at[j] < (lane + 32u * j + 1u) * n_out ? mine[at[j]] : 0ull;
-            if (lane == 0) {
-                val[b * n_out + k] = best;
-                tok[b * n_out + k] = ~(uint32_t)best;
+        for (uint32_t j = 0; j < kBeamEach; ++j)
+            if (j < used && v[j] >= bound) {
+                if (n < kBeamCap) s.list[n] = key_of(v[j], index(j));
+                ++n;
             }
-        }
-        __syncwarp();
-        for (uint32_t k = lane; k < n_out; k += 32u) {
-            const unsigned long long best = val[b * n_out + k];
-            const double s = score + (((double)value_of((uint32_t)(best >> 32)) - (double)top) - norm);
-            val[b * n_out + k] = best != 0 && s > -INFINITY ? order_of(s == 0.0 ? 0.0 : s) : 0ull;      // NaN: none
-        }
     }
     __syncthreads();
-    if (warp) return;
+    if (s.count > kBeamCap) {
+        unsigned long long best = 0, limit = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kBeamEach; ++j) {
+            const unsigned long long key = j < used ? key_of(v[j], index(j)) : 0ull;
+            best = key > best ? key : best;
+        }
+#pragma unroll 1
+        for (int bit = 63; bit >= 0; --bit) {
+            const unsigned long long trial = limit | (1ull << bit);
+            if (__syncthreads_count(best >= trial) >= (int)n_out) limit = trial;
+        }
+        if (tid == 0) s.count = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t j = 0; j < kBeamEach; ++j) {
+            const unsigned long long key = j < used ? key_of(v[j], index(j)) : 0ull;
+            if (key != 0 && key >= limit) s.list[atomicAdd(&s.count, 1u)] = key;
+        }
+        __syncthreads();
+    }
+    const uint32_t n = s.count;
+    for (uint32_t i = tid; i < n; i += kBeamThreads) {
+        const unsigned long long k = s.list[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < n; ++j) rank += s.list[j] > k ? 1u : 0u;
+        if (rank < n_out) s.best[rank] = k;
+    }
+    for (uint32_t i = n + tid; i < n_out; i += kBeamThreads) s.best[i] = 0ull;
+    __syncthreads();
+}
+
+template <class T>
+__global__ void __launch_bounds__(kBeamThreads, 3) beam_select_kernel(const T* __restrict__ logits, size_t stride, uint32_t n_vocab, const BeamPart* parts,
+                                                                   const float* maxima, uint32_t n_parts, const float* scores, uint32_t n_beam,
+                                                                   uint32_t n_out, float* out_scores, int32_t* out_beam, int32_t* out_token) {
+    extern __shared__ unsigned long long lists[];        // in the cluster's first CTA: [n_beam][n_out] f64 order of s, then tokens
+    __shared__ SelectShared s;
+    __shared__ double norm;
+    __shared__ float top;
+    uint32_t rank, size;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+    const uint32_t tid = threadIdx.x, lane = tid & 31u;
+    const size_t group = blockIdx.x / size;
+    // every CTA of the cluster has begun before one writes into the first one's shared memory
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (uint32_t b = rank; b < n_beam; b += size) {
+        const size_t row = group * n_beam + b;
+        const T* x = logits + row * stride;
+        const uint32_t lead = (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15u) / (uint32_t)sizeof(T);
+        // groups of 32 neighbours, or of 64 or 128 in the largest vocabularies
+        const float* mx = maxima + row * n_parts * kBeamThreads;
+        uint32_t fold = 0;
+        while (n_parts * kBeamThreads >> fold > kBeamPart) ++fold;
+        const uint32_t n_groups = (n_parts * kBeamThreads + (1u << fold) - 1u) >> fold;
+        float v[kBeamEach];
+#pragma unroll
+        for (uint32_t j = 0; j < kBeamEach; ++j) {       // all loads together
+            const uint32_t i = j * kBeamThreads + tid;
+            v[j] = i < n_groups ? mx[i << fold] : -INFINITY;
+        }
+        for (uint32_t k = 1; k < 1u << fold; ++k)
+#pragma unroll
+            for (uint32_t j = 0; j < kBeamEach; ++j) {
+                const uint32_t i = ((j * kBeamThreads + tid) << fold) + k;
+                if (i < n_parts * kBeamThreads) v[j] = fmaxf(v[j], mx[i]);
+            }
+        if (tid < 32u) {                                 // the row's normaliser
+            const BeamPart* pr = parts + row * n_parts;
+            float mp[kBeamLists], p[kBeamLists], t = -INFINITY;
+#pragma unroll
+            for (uint32_t j = 0; j < kBeamLists; ++j) {
+                const BeamPart q = lane + 32u * j < n_parts ? pr[lane + 32u * j] : BeamPart{-INFINITY, 0.0f};
+                mp[j] = q.max;
+                p[j] = q.sum;
+                t = fmaxf(t, q.max);
+            }
+            for (int k = 16; k; k >>= 1) t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, k));
+            double sum = 0.0;
+#pragma unroll
+            for (uint32_t j = 0; j < kBeamLists; ++j)
+                if (p[j] != 0.0f) sum += (double)p[j] * (double)beam_ex2((mp[j] - t) * 1.4426950408889634f);
+            for (int k = 16; k; k >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, k);
+            if (lane == 0) {
+                norm = log(sum);                         // above top, so that logits far from 0 keep their digits
+                top = t;
+            }
+        }
+        float m = v[0];
+#pragma unroll
+        for (uint32_t j = 1; j < kBeamEach; ++j) m = fmaxf(m, v[j]);
+        select_best(s, v, (n_groups + kBeamThreads - 1u) / kBeamThreads, select_bound(s, m, n_out), n_out, [&](uint32_t j) { return j * kBeamThreads + tid; });
+        // their logits: the last group's largest bounds the row's best
+        const float least = s.best[n_out - 1u] ? value_of((uint32_t)(s.best[n_out - 1u] >> 32)) : -3.4028234e38f;
+        const uint32_t shift = 5u + fold, n = n_out << shift;
+        auto token = [&](uint32_t j) {                   // of this thread's logit j (s.best changes only when all have asked)
+            const uint32_t e = j * kBeamThreads + tid;
+            return (int32_t)(~(uint32_t)s.best[min(e >> shift, n_out - 1u)] << shift) + (int32_t)(e & ((1u << shift) - 1u)) - (int32_t)lead;
+        };
+#pragma unroll
+        for (uint32_t j = 0; j < kBeamEach; ++j) {
+            v[j] = -INFINITY;
+            if (j * kBeamThreads >= n) continue;
+            const uint32_t e = j * kBeamThreads + tid;
+            const int32_t i = token(j);
+            if (e < n && s.best[min(e >> shift, n_out - 1u)] != 0 && i >= 0 && i < (int32_t)n_vocab) v[j] = to_f32(x[i]);
+        }
+        select_best(s, v, (n + kBeamThreads - 1u) / kBeamThreads, least, n_out, [&](uint32_t j) { return (uint32_t)token(j); });
+        for (uint32_t k = tid; k < n_out; k += kBeamThreads) {
+            const unsigned long long key = s.best[k];
+            const double score = scores ? (double)scores[row] : 0.0;
+            const double z = score + (((double)value_of((uint32_t)(key >> 32)) - (double)top) - norm);
+            const unsigned long long order = key != 0 && z > -INFINITY ? order_of(z == 0.0 ? 0.0 : z) : 0ull;      // NaN: none
+            const uint32_t best = ~(uint32_t)key;
+            uint32_t to = (uint32_t)__cvta_generic_to_shared(lists + b * n_out + k), far;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(far) : "r"(to));
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(far), "l"(order) : "memory");
+            to = (uint32_t)__cvta_generic_to_shared(reinterpret_cast<uint32_t*>(lists + n_beam * n_out) + b * n_out + k);
+            asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(far) : "r"(to));
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(far), "r"(best) : "memory");
+        }
+        __syncthreads();
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank || tid >= 32u) return;
+    // the rows' lists: the best of their heads, n_out times; equal scores: the lowest beam
+    const uint32_t* tok = reinterpret_cast<const uint32_t*>(lists + n_beam * n_out);
     uint32_t at[2] = {0, 0};
     unsigned long long h[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) h[j] = lane + 32u * j < n_beam ? val[(lane + 32u * j) * n_out] : 0ull;
+    for (int j = 0; j < 2; ++j) h[j] = lane + 32u * j < n_beam ? lists[(lane + 32u * j) * n_out] : 0ull;
     for (uint32_t k = 0; k < n_out; ++k) {
         const unsigned long long best = warp_max(h[1] > h[0] ? h[1] : h[0]);
-        // equal scores: the lowest beam
         const uint32_t b = __reduce_min_sync(0xFFFFFFFFu, h[0] == best ? lane : h[1] == best ? lane + 32u : 0xFFFFFFFFu);
         const size_t o = group * n_out + k;
         if (best == 0) {
@@ -305,7 +363,7 @@ __global__ void __launch_bounds__(512) beam_merge_kernel(const BeamPart* parts, 
             out_beam[o] = (int32_t)b;
             out_token[o] = (int32_t)tok[b * n_out + at[j]];
             ++at[j];
-            h[j] = at[j] < n_out ? val[b * n_out + at[j]] : 0ull;
+            h[j] = at[j] < n_out ? lists[b * n_out + at[j]] : 0ull;
         }
     }
 }
@@ -313,8 +371,36 @@ __global__ void __launch_bounds__(512) beam_merge_kernel(const BeamPart* parts, 
 size_t beam_parts_bytes(uint32_t rows, uint32_t n_vocab) { return ((size_t)rows * beam_parts(n_vocab) * sizeof(BeamPart) + 255u) & ~(size_t)255u; }
 
 template <class T>
-void launch_part(const void* x, size_t stride, uint32_t rows, uint32_t n_vocab, uint32_t n_out, BeamPart* parts, unsigned long long* keys, cudaStream_t st) {
-    beam_part_kernel<T><<<dim3(beam_parts(n_vocab), rows), kBeamThreads, 0, st>>>(static_cast<const T*>(x), stride, n_vocab, n_out, parts, keys);
+cudaError_t launch_beam(const void* logits, size_t stride, const float* scores, uint32_t n_group, uint32_t n_beam, uint32_t n_vocab, uint32_t n_out,
+                        float* out_scores, int32_t* out_beam, int32_t* out_token, BeamPart* parts, float* maxima, cudaStream_t st) {
+    const uint32_t n_parts = beam_parts(n_vocab), size = n_beam < kBeamRows ? n_beam : kBeamRows;
+    const T* x = static_cast<const T*>(logits);
+    beam_part_kernel<T><<<dim3(n_parts, n_group * n_beam), kBeamThreads, 0, st>>>(x, stride, n_vocab, parts, maxima);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    static bool done[64];
+    int dev = 0;
+    e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev >= 64 || !done[dev])) {
+        e = cudaFuncSetAttribute(beam_select_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kBeamBeams * kBeamOut * 12u));
+        if (e == cudaSuccess && dev < 64) done[dev] = true;
+    }
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n_group * size);
+    cfg.blockDim = dim3(kBeamThreads);
+    cfg.dynamicSmemBytes = (size_t)n_beam * n_out * 12u;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = size;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, beam_select_kernel<T>, x, stride, n_vocab, static_cast<const BeamPart*>(parts), static_cast<const float*>(maxima), n_parts,
+                              scores, n_beam, n_out, out_scores, out_beam, out_token);
 }
 
 template <class... A>
@@ -343,7 +429,7 @@ const char* tsrc_beam_select_unsupported(uint32_t type, uint32_t n_beam, uint32_
 size_t tsrc_beam_select_workspace(uint32_t n_group, uint32_t n_beam, uint32_t n_vocab, uint32_t n_out) {
     if (tsrc_beam_select_unsupported(TSRC_TYPE_F32, n_beam, n_vocab, n_out)) return 0;
     const size_t rows = (size_t)n_group * n_beam;
-    return beam_parts_bytes((uint32_t)rows, n_vocab) + rows * beam_parts(n_vocab) * n_out * 8u;
+    return beam_parts_bytes((uint32_t)rows, n_vocab) + rows * beam_parts(n_vocab) * kBeamThreads * 4u;
 }
 
 int tsrc_beam_select(tsrc_ctx* ctx, uint32_t type, const void* logits, uint32_t stride, const float* scores, uint32_t n_group,
@@ -365,41 +451,12 @@ int tsrc_beam_select(tsrc_ctx* ctx, uint32_t type, const void* logits, uint32_t 
     DeviceScope scope(ctx);
     if (scope.rc) return scope.rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const uint32_t rows = n_group * n_beam, n_parts = beam_parts(n_vocab);
     BeamPart* parts = static_cast<BeamPart*>(ws);
-    unsigned long long* keys = reinterpret_cast<unsigned long long*>(static_cast<uint8_t*>(ws) + beam_parts_bytes(rows, n_vocab));
-    if (type == TSRC_TYPE_F32) launch_part<float>(logits, stride, rows, n_vocab, n_out, parts, keys, st);
-    else if (type == TSRC_TYPE_F16) launch_part<__half>(logits, stride, rows, n_vocab, n_out, parts, keys, st);
-    else launch_part<__nv_bfloat16>(logits, stride, rows, n_vocab, n_out, parts, keys, st);
-    cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess) {
-        // as many warps as beams, up to sixteen and to the shared memory that their lists take
-        const size_t fixed = (size_t)(n_beam * n_out * 12u + 15u) / 16u * 16u, each = (size_t)n_parts * n_out * 8u;
-        uint32_t warps = n_beam < 16u ? n_beam : 16u;
-        while (warps > 1u && fixed + warps * each > kBeamSmem) --warps;
-        const auto kernel = n_parts <= 32u ? beam_merge_kernel<1> : beam_merge_kernel<kBeamLists>;
-        static bool done[64];
-        int dev = 0;
-        e = cudaGetDevice(&dev);
-        if (e == cudaSuccess && (dev >= 64 || !done[dev])) {
-            e = cudaFuncSetAttribute(beam_merge_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBeamSmem);
-            if (e == cudaSuccess) e = cudaFuncSetAttribute(beam_merge_kernel<kBeamLists>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBeamSmem);
-            if (e == cudaSuccess && dev < 64) done[dev] = true;
-        }
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(n_group);
-        cfg.blockDim = dim3(warps * 32u);
-        cfg.dynamicSmemBytes = fixed + warps * each;
-        cfg.stream = st;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        if (e == cudaSuccess)
-            e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const BeamPart*>(parts), static_cast<const unsigned long long*>(keys), n_parts,
-                                   scores, n_beam, n_out, out_scores, out_beam, out_token);
-    }
+    float* maxima = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + beam_parts_bytes(n_group * n_beam, n_vocab));
+    cudaError_t e;
+    if (type == TSRC_TYPE_F32) e = launch_beam<float>(logits, stride, scores, n_group, n_beam, n_vocab, n_out, out_scores, out_beam, out_token, parts, maxima, st);
+    else if (type == TSRC_TYPE_F16) e = launch_beam<__half>(logits, stride, scores, n_group, n_beam, n_vocab, n_out, out_scores, out_beam, out_token, parts, maxima, st);
+    else e = launch_beam<__nv_bfloat16>(logits, stride, scores, n_group, n_beam, n_vocab, n_out, out_scores, out_beam, out_token, parts, maxima, st);
     if (e != cudaSuccess) return refuse(TSRC_E_CUDA, "tsrc_beam_select: %s (%s)", cudaGetErrorString(e), cudaGetErrorName(e));
     return TSRC_OK;
 }
