@@ -744,17 +744,35 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
     p.group = group ? group : T;
     const uint32_t rows = p.group * (n_head / n_head_kv);
     p.splits = 1;
-    if (!mask && D <= 128u && rows >= 96u) {
-        p.mode = kRows128;
-        p.row_tiles = (rows + kFa4TcRows - 1u) / kFa4TcRows;
-        p.units = (T / p.group) * n_head_kv * p.row_tiles;
-        return p;
-    }
+    const uint32_t len = max_len && max_len < n_kv ? max_len : n_kv;
     p.mode = type != TSRC_TYPE_BF16 ? kRows8Split : rows <= 8u ? kRows8 : kRows16;
     const uint32_t R = p.mode == kRows16 ? 16u : 8u;
     p.row_tiles = (rows + R - 1u) / R;
     p.units = (T / p.group) * n_head_kv * p.row_tiles;
-    const uint32_t len = max_len && max_len < n_kv ? max_len : n_kv;
+    if (!mask && D <= 128u) {
+        // The kernel for many rows where it is the faster one, by what both measured (ns): a tile of 64 cells keeps one
+        // of its CTAs 1.1 (bf16) to 1.6 us (f32), and its CTAs are split over the cells while SMs are idle and eight tiles
+        // are left to each; the other kernel's 592 places take 0.93 us for 32 cells of 8 rows (1.35 for 16 rows; D = 64:
+        // two thirds). 32 rows of 8 KV heads over 8192 cells in f32: 38 us there, 221 here unsplit; 2048 rows: 797 and 231.
+        const uint64_t units = (uint64_t)(T / p.group) * n_head_kv * ((rows + kFa4TcRows - 1u) / kFa4TcRows), tiles = len / 64u + 1u;
+        const uint32_t each = type == TSRC_TYPE_BF16 ? 1150u : type == TSRC_TYPE_F16 ? 1450u : 1650u;
+        const uint64_t places = type == TSRC_TYPE_BF16 || D == 64u ? 2u * kSms : kSms;
+        uint64_t splits = places / units < tiles / 8u ? places / units : tiles / 8u;
+        if (splits < 1u) splits = 1;
+        const uint64_t tc = 9000u + (units * splits + places - 1u) / places * ((tiles + splits - 1u) / splits) * each + (splits > 1u ? 6000u : 0u);
+        const uint64_t dec = 11000u + (uint64_t)p.units * (len / kDecTile + 1u) * (R == 16u ? 1350u : 930u) / (D == 64u ? 900u : 592u);
+        if (tc < dec) {
+            p.mode = kRows128;
+            p.row_tiles = (rows + kFa4TcRows - 1u) / kFa4TcRows;
+            p.units = (uint32_t)units;
+            p.splits = (uint32_t)splits;
+            if (p.splits > 1u) {
+                p.o_bytes = (size_t)p.units * p.splits * kFa4TcRows * D * 4u;
+                p.ml_bytes = (size_t)p.units * p.splits * kFa4TcRows * 16u;
+            }
+            return p;
+        }
+    }
     const uint32_t teams = D <= 128u ? kDecWarps : kDecWarps * 128u / D;
     // Splits in powers of two up to a cluster's CTAs, each warp keeping a tile at least: until the GPU's places for
     // CTAs (four an SM) are taken, since a CTA costs about three tiles' time beside its tiles (13 drafted tokens over
@@ -772,6 +790,27 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
         p.ml_bytes = (size_t)p.units * p.splits * R * 16u;
     }
     return p;
+}
+
+// Joins the splits that a kernel left in the workspace.
+template <class T, int D, uint32_t R>
+cudaError_t merge_launch(const Fa4Args& a, uint32_t units, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(units, R);
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fa4_merge_kernel<T, D, R>, a);
+}
+template <class T>
+cudaError_t tc_launch(uint32_t type, uint32_t D, const Fa4Args& a, uint32_t units, cudaStream_t st) {
+    cudaError_t e = launch_fa4_tc(type, D, a, units, st);
+    if (e != cudaSuccess || a.splits == 1u) return e;
+    return D == 64u ? merge_launch<T, 64, kFa4TcRows>(a, units, st) : merge_launch<T, 128, kFa4TcRows>(a, units, st);
 }
 
 template <class T, int D, int MODE, bool MASK>
@@ -801,14 +840,7 @@ cudaError_t dec_launch_m(const Fa4Args& a, uint32_t units, cudaStream_t st) {
         cfg.numAttrs = 1;
     }
     e = cudaLaunchKernelEx(&cfg, fa4_dec_kernel<T, D, MODE, MASK>, a);
-    if (e != cudaSuccess || !a.part_o) return e;
-    cfg.gridDim = dim3(units, kRowsOf<MODE>);
-    cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = 0;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, fa4_merge_kernel<T, D, kRowsOf<MODE>>, a);
+    return e != cudaSuccess || !a.part_o ? e : merge_launch<T, D, kRowsOf<MODE>>(a, units, st);
 }
 template <class T, int D, int MODE>
 cudaError_t dec_launch(const Fa4Args& a, uint32_t units, cudaStream_t st) {
@@ -852,7 +884,8 @@ size_t tsrc_flash_attn_q4_workspace(uint32_t type, uint32_t n_head_kv, uint32_t 
     if (T == 0 || tsrc_flash_attn_q4_unsupported(type, n_head_kv, head_dim, n_head)) return 0;
     // the largest a call of these sizes needs, with a mask or without
     const Fa4Plan p = fa4_plan(type, n_head_kv, head_dim, T, n_head, n_kv, group, max_len, true);
-    return p.o_bytes + p.ml_bytes;
+    const Fa4Plan q = fa4_plan(type, n_head_kv, head_dim, T, n_head, n_kv, group, max_len, false);
+    return p.o_bytes + p.ml_bytes > q.o_bytes + q.ml_bytes ? p.o_bytes + p.ml_bytes : q.o_bytes + q.ml_bytes;
 }
 
 int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const void* q, uint32_t q_stride, uint32_t T, uint32_t n_head,
@@ -914,7 +947,9 @@ int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const v
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (p.mode == kRows128) e = launch_fa4_tc(type, kv->D, a, p.units, st);
+    if (p.mode == kRows128)
+        e = type == TSRC_TYPE_F32 ? tc_launch<float>(type, kv->D, a, p.units, st) : type == TSRC_TYPE_F16 ? tc_launch<__half>(type, kv->D, a, p.units, st)
+                                                                                                      : tc_launch<__nv_bfloat16>(type, kv->D, a, p.units, st);
     else if (type == TSRC_TYPE_F32) e = dec_launch_d<float, kRows8Split>(a, kv->D, p.units, st);
     else if (type == TSRC_TYPE_F16) e = dec_launch_d<__half, kRows8Split>(a, kv->D, p.units, st);
     else e = p.mode == kRows8 ? dec_launch_d<__nv_bfloat16, kRows8>(a, kv->D, p.units, st) : dec_launch_d<__nv_bfloat16, kRows16>(a, kv->D, p.units, st);

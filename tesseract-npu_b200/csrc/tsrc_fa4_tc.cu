@@ -257,7 +257,8 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
     Control& c = *reinterpret_cast<Control*>(sm + S::CTL_AT);
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     // the last rows first: in a causal prompt they see the most cells
-    const uint32_t hk = blockIdx.x % a.n_head_kv, rest = blockIdx.x / a.n_head_kv;
+    const uint32_t split = blockIdx.x % a.splits, place = blockIdx.x / a.splits;
+    const uint32_t hk = place % a.n_head_kv, rest = place / a.n_head_kv;
     const uint32_t rt = a.row_tiles - 1u - rest % a.row_tiles, grp = rest / a.row_tiles;
     const uint32_t rows = a.group * a.G, row = rt * kRows + tid;
     const uint32_t tok = grp * a.group + row / a.G, head = hk * a.G + row % a.G;
@@ -344,8 +345,10 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
     const uint32_t tmem = c.tmem;
     const int32_t first = min(min(c.span[0][0], c.span[1][0]), min(c.span[2][0], c.span[3][0]));
     const int32_t last = max(max(c.span[0][1], c.span[1][1]), max(c.span[2][1], c.span[3][1]));
-    const uint32_t tile0 = last > first ? (uint32_t)first / kTile : 0u;
-    const uint32_t tiles = last > first ? ((uint32_t)last + kTile - 1u) / kTile - tile0 : 0u;
+    const uint32_t from = last > first ? (uint32_t)first / kTile : 0u;
+    const uint32_t span = last > first ? ((uint32_t)last + kTile - 1u) / kTile - from : 0u;
+    const uint32_t tile0 = from + (uint32_t)((uint64_t)span * split / a.splits);             // this split's tiles
+    const uint32_t tiles = from + (uint32_t)((uint64_t)span * (split + 1u) / a.splits) - tile0;
 
     if (warp == 4u + S::DW) {
         // ---- products, issued by one thread. Descriptors are made once and advanced by constants: made anew for every
@@ -706,8 +709,11 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (ok) {
             fence_after();
-            const float f = l == 0.0f ? 0.0f : pow2((int)v_exp - 15 + Scaled<PRECISE>::UNDO) / l;
+            // l and O are in units of 2^6 p: a split's share names 2^-6 of its reference
+            const float unit = pow2((int)v_exp - 15 + Scaled<PRECISE>::UNDO), f = a.splits > 1u ? unit : l == 0.0f ? 0.0f : unit / l;
             T* out = static_cast<T*>(a.out) + (size_t)tok * a.out_stride + (size_t)head * D;
+            const size_t part = ((((size_t)grp * a.row_tiles + rt) * a.n_head_kv + hk) * a.splits + split) * kRows + tid;
+            if (a.splits > 1u && row < rows) *reinterpret_cast<float4*>(a.part_ml + part * 4u) = make_float4(0.0f, m - 6.0f, l, 0.0f);
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
                 uint32_t o[32] = {};
@@ -733,7 +739,8 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
                             x[j] = l == 0.0f ? 0.0f : __uint_as_float(o[8 * j + g]) * f;
                             if (lost >> b & 1u) x[j] = __int_as_float(0x7FC00000);
                         }
-                        store4<T>(out + 32u * b + 4u * g, x, a.out_wide);
+                        if (a.splits > 1u) store4<float>(a.part_o + part * D + 32u * b + 4u * g, x, true);
+                        else store4<T>(out + 32u * b + 4u * g, x, a.out_wide);
                     }
                 }
                 __syncwarp();
@@ -760,7 +767,7 @@ cudaError_t launch(const Fa4Args& a, uint32_t units, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         if (dev < 64) done[dev] = true;
     }
-    fa4_tc_kernel<T, D><<<units, S::THREADS, S::BYTES, st>>>(a);
+    fa4_tc_kernel<T, D><<<units * a.splits, S::THREADS, S::BYTES, st>>>(a);
     return cudaGetLastError();
 }
 
