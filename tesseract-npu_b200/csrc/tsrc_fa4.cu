@@ -739,7 +739,7 @@ struct Fa4Plan {
     size_t o_bytes, ml_bytes;                  // of the workspace, where a merge kernel joins the splits
 };
 
-Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint32_t n_head, uint32_t n_kv, uint32_t group, uint32_t max_len, bool mask) {
+Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint32_t n_head, uint32_t n_kv, uint32_t group, uint32_t max_len) {
     Fa4Plan p{};
     p.group = group ? group : T;
     const uint32_t rows = p.group * (n_head / n_head_kv);
@@ -749,15 +749,15 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
     const uint32_t R = p.mode == kRows16 ? 16u : 8u;
     p.row_tiles = (rows + R - 1u) / R;
     p.units = (T / p.group) * n_head_kv * p.row_tiles;
-    if (!mask && D <= 128u) {
+    if (D <= 128u) {
         // The kernel for many rows where it is the faster one, by what both measured (ns): a tile of 64 cells keeps one
-        // of its CTAs 1.1 (bf16) to 1.6 us (f32), and its CTAs are split over the cells while SMs are idle and eight tiles
-        // are left to each; the other kernel's 592 places take 0.93 us for 32 cells of 8 rows (1.35 for 16 rows; D = 64:
+        // of its CTAs 1.1 (bf16) to 1.6 us (f32), and its CTAs are split over the cells while SMs have none and eight
+        // tiles are left to each; the other kernel's 592 places take 0.93 us for 32 cells of 8 rows (1.35 for 16 rows; D = 64:
         // two thirds). 32 rows of 8 KV heads over 8192 cells in f32: 38 us there, 221 here unsplit; 2048 rows: 797 and 231.
         const uint64_t units = (uint64_t)(T / p.group) * n_head_kv * ((rows + kFa4TcRows - 1u) / kFa4TcRows), tiles = len / 64u + 1u;
         const uint32_t each = type == TSRC_TYPE_BF16 ? 1150u : type == TSRC_TYPE_F16 ? 1450u : 1650u;
         const uint64_t places = type == TSRC_TYPE_BF16 || D == 64u ? 2u * kSms : kSms;
-        uint64_t splits = places / units < tiles / 8u ? places / units : tiles / 8u;
+        uint64_t splits = kSms / units < tiles / 8u ? kSms / units : tiles / 8u;
         if (splits < 1u) splits = 1;
         const uint64_t tc = 9000u + (units * splits + places - 1u) / places * ((tiles + splits - 1u) / splits) * each + (splits > 1u ? 6000u : 0u);
         const uint64_t dec = 11000u + (uint64_t)p.units * (len / kDecTile + 1u) * (R == 16u ? 1350u : 930u) / (D == 64u ? 900u : 592u);
@@ -882,10 +882,8 @@ const char* tsrc_flash_attn_q4_unsupported(uint32_t type, uint32_t n_head_kv, ui
 size_t tsrc_flash_attn_q4_workspace(uint32_t type, uint32_t n_head_kv, uint32_t head_dim, uint32_t T, uint32_t n_head,
                                     uint32_t n_kv, uint32_t group, uint32_t max_len) {
     if (T == 0 || tsrc_flash_attn_q4_unsupported(type, n_head_kv, head_dim, n_head)) return 0;
-    // the largest a call of these sizes needs, with a mask or without
-    const Fa4Plan p = fa4_plan(type, n_head_kv, head_dim, T, n_head, n_kv, group, max_len, true);
-    const Fa4Plan q = fa4_plan(type, n_head_kv, head_dim, T, n_head, n_kv, group, max_len, false);
-    return p.o_bytes + p.ml_bytes > q.o_bytes + q.ml_bytes ? p.o_bytes + p.ml_bytes : q.o_bytes + q.ml_bytes;
+    const Fa4Plan p = fa4_plan(type, n_head_kv, head_dim, T, n_head, n_kv, group, max_len);
+    return p.o_bytes + p.ml_bytes;
 }
 
 int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const void* q, uint32_t q_stride, uint32_t T, uint32_t n_head,
@@ -915,7 +913,7 @@ int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const v
     if (T == 0) return TSRC_OK;
     DeviceScope scope(ctx);
     if (scope.rc) return scope.rc;
-    const Fa4Plan p = fa4_plan(type, kv->n_head_kv, kv->D, T, n_head, n_kv, group, max_len, mask != nullptr);
+    const Fa4Plan p = fa4_plan(type, kv->n_head_kv, kv->D, T, n_head, n_kv, group, max_len);
     Fa4Args a{};
     a.q = q;
     a.out = out;
@@ -937,6 +935,7 @@ int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const v
     a.ranges = ranges;
     a.mask = reinterpret_cast<const __half*>(mask);
     a.mask_stride = mask_stride;
+    a.mask_wide = (reinterpret_cast<uintptr_t>(mask) & 15u) == 0 && mask_stride % 8u == 0;
     a.scale = scale;
     a.group = p.group;
     a.row_tiles = p.row_tiles;

@@ -9,7 +9,7 @@ struct Fa4Args {
     const void* q;
     void* out;
     size_t q_stride, out_stride;
-    bool q_wide, out_wide;                     // rows allow 16-byte (out: four-value) accesses
+    bool q_wide, out_wide, mask_wide;          // rows allow 16-byte (out: four-value) accesses
     const uint8_t *kq, *vq;
     const __half *kd, *vd;
     uint32_t T, n_head, n_head_kv, G, n_kv, n_alloc;
@@ -40,7 +40,7 @@ __device__ __forceinline__ void store4(T* p, const float (&x)[4], bool wide) {
     }
 }
 
-// Many query rows on one stretch of cells: D 64 or 128, no mask, row tiles of 128 (tsrc_fa4_tc.cu).
+// Many query rows on one stretch of cells: D 64 or 128, row tiles of 128 (tsrc_fa4_tc.cu).
 constexpr uint32_t kFa4TcRows = 128;
 cudaError_t launch_fa4_tc(uint32_t type, uint32_t D, const Fa4Args& a, uint32_t units, cudaStream_t st);
 // The error word of its waits (kKv4ErrWait), cleared when read with clear = true.

@@ -202,6 +202,28 @@ template <> struct Scaled<false> {
     }
 };
 
+// Eight cells of a row's mask from `cell` on, -inf where `seen` lacks the cell's bit (the mask there may hold anything,
+// or not be there).
+__device__ __forceinline__ uint4 mask_of(const Fa4Args& a, const __half* row, int32_t cell, uint32_t seen) {
+    uint32_t w[4];
+    if (a.mask_wide && seen && cell + 8 <= (int32_t)a.n_kv) {
+        const uint4 h = *reinterpret_cast<const uint4*>(row + cell);
+        w[0] = h.x; w[1] = h.y; w[2] = h.z; w[3] = h.w;
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            w[j] = seen >> (2 * j) & 1u ? __half_as_ushort(row[cell + 2 * (int32_t)j]) : 0u;
+            if (seen >> (2 * j) & 2u) w[j] |= (uint32_t)__half_as_ushort(row[cell + 2 * (int32_t)j + 1]) << 16;
+        }
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t keep = (seen >> (2 * j) & 1u ? 0x0000FFFFu : 0u) | (seen >> (2 * j) & 2u ? 0xFFFF0000u : 0u);
+        w[j] = (w[j] & keep) | (0xFC00FC00u & ~keep);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // O times f
 template <int D>
 __device__ __forceinline__ void rescale(uint32_t o_at, float f) {
@@ -248,7 +270,7 @@ __device__ __forceinline__ void settle(uint32_t o_at, uint32_t sum_at, float f, 
     }
 }
 
-template <class T, int D>
+template <class T, int D, bool MASK>
 __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTAS) fa4_tc_kernel(Fa4Args a) {
     using S = TcShape<T, D>;
     constexpr bool PRECISE = S::PRECISE, TOTAL = S::TOTAL;
@@ -588,6 +610,8 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
         const uint32_t mine = tmem + ((warp * 32u) << 16);
         const float qs = c.q_unscale[tid];           // this row's scale, for scores in log2
         float m = -INFINITY, l = 0.0f;               // reference of the weights' exponents; running sum, both in units of 2^6 p
+        float off = MASK ? -INFINITY : 0.0f;         // the mask's maximum so far: scores and m are relative to it
+        const __half* mrow = MASK && row < rows ? a.mask + (size_t)tok * a.mask_stride : nullptr;
         uint32_t v_exp = 1, lost = 0;                // lost: blocks of V in which the row sees a scale that is no number
         bool ok = true;
         // the cells that all rows of the warp see; rows behind the group's last lose nothing
@@ -621,14 +645,39 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
             tmem_wait_ld64(raw);
 #pragma unroll
             for (int j = 0; j < 64; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * f);
-            if (!open) {                             // bit j of the words: the row sees cell c0 + j
+            uint32_t w0 = ~0u, w1 = ~0u;             // bit j of the words: the row's range holds cell c0 + j
+            if (!open) {
                 const int32_t from = min(max(lo - c0, 0), 64), to = min(max(hi - c0, from), 64);
                 const unsigned long long bits = (to >= 64 ? ~0ull : (1ull << to) - 1ull) & ~(from >= 64 ? ~0ull : (1ull << from) - 1ull);
-                const uint32_t w0 = (uint32_t)bits, w1 = (uint32_t)(bits >> 32);
+                w0 = (uint32_t)bits;
+                w1 = (uint32_t)(bits >> 32);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
                     raw[j] = w0 >> j & 1u ? raw[j] : 0xFF800000u;
                     raw[32 + j] = w1 >> j & 1u ? raw[32 + j] : 0xFF800000u;
+                }
+            }
+            if constexpr (MASK) {
+                // the mask's running maximum is taken out first: a row of the type's lowest value keeps its scores' digits
+                __half2 most2 = __half2half2(__ushort_as_half((unsigned short)0xFC00u));
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) {
+                    const uint4 h = mask_of(a, mrow, c0 + 8 * (int32_t)k, (k < 4 ? w0 >> 8u * k : w1 >> (8u * k - 32u)) & 0xFFu);
+                    most2 = __hmax2(most2, __hmax2(__hmax2(as_h2(h.x), as_h2(h.y)), __hmax2(as_h2(h.z), as_h2(h.w))));
+                }
+                const float now = fmaxf(off, fmaxf(__low2float(most2), __high2float(most2))), base = now == -INFINITY ? 0.0f : now;
+                if (off != -INFINITY && off != now) m += (off - base) * 1.4426950408889634f;
+                off = now;
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) {
+                    const uint4 h = mask_of(a, mrow, c0 + 8 * (int32_t)k, (k < 4 ? w0 >> 8u * k : w1 >> (8u * k - 32u)) & 0xFFu);
+                    const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; ++j) {
+                        const float x = __half2float(__ushort_as_half((unsigned short)(w[j / 2] >> (j & 1u ? 16 : 0))));
+                        const float z = fmaf(x - base, 1.4426950408889634f, __uint_as_float(raw[8 * k + j]));
+                        raw[8 * k + j] = __float_as_uint(x == -INFINITY ? -INFINITY : z);
+                    }
                 }
             }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -657,7 +706,10 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
             }
             const float up = m == -INFINITY ? 0.0f : 6.0f - m;
             float sum[4] = {}, far_sum = 0.0f;
-            if (info.far) {                          // the sum takes the weights without V's powers of two
+            if (MASK && info.far) {                  // the sum takes the weights without V's powers of two
+#pragma unroll
+                for (int j = 0; j < 64; ++j) far_sum += ex2(__uint_as_float(raw[j]) - c.cell_v[i & 3u][j] + up);
+            } else if (info.far) {
 #pragma unroll 1
                 for (uint32_t k = 0; k < kTile; k += 8) {
                     uint32_t x[8];
@@ -697,7 +749,7 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
             if (info.bad) {                          // seldom: which of the blocks left out of V this row would have met
 #pragma unroll 1
                 for (uint32_t j = 0; j < kTile; ++j) {
-                    if (c0 + (int32_t)j < lo || c0 + (int32_t)j >= hi) continue;
+                    if (c0 + (int32_t)j < lo || c0 + (int32_t)j >= hi || (MASK && __half2float(mrow[c0 + (int32_t)j]) == -INFINITY)) continue;
                     const __half* d = a.vd + ((size_t)hk * a.n_alloc + (uint32_t)c0 + j) * NB;
                     for (uint32_t b = 0; b < NB; ++b)
                         if ((__half_as_ushort(d[b]) & 0x7C00u) == 0x7C00u) lost |= 1u << b;
@@ -713,7 +765,7 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
             const float unit = pow2((int)v_exp - 15 + Scaled<PRECISE>::UNDO), f = a.splits > 1u ? unit : l == 0.0f ? 0.0f : unit / l;
             T* out = static_cast<T*>(a.out) + (size_t)tok * a.out_stride + (size_t)head * D;
             const size_t part = ((((size_t)grp * a.row_tiles + rt) * a.n_head_kv + hk) * a.splits + split) * kRows + tid;
-            if (a.splits > 1u && row < rows) *reinterpret_cast<float4*>(a.part_ml + part * 4u) = make_float4(0.0f, m - 6.0f, l, 0.0f);
+            if (a.splits > 1u && row < rows) *reinterpret_cast<float4*>(a.part_ml + part * 4u) = make_float4(off, m - 6.0f, l, 0.0f);
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
                 uint32_t o[32] = {};
@@ -755,20 +807,25 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
     }
 }
 
-template <class T, int D>
-cudaError_t launch(const Fa4Args& a, uint32_t units, cudaStream_t st) {
+template <class T, int D, bool MASK>
+cudaError_t launch_m(const Fa4Args& a, uint32_t units, cudaStream_t st) {
     using S = TcShape<T, D>;
     static bool done[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !done[dev]) {
-        e = cudaFuncSetAttribute(fa4_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
+        e = cudaFuncSetAttribute(fa4_tc_kernel<T, D, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
         if (e != cudaSuccess) return e;
         if (dev < 64) done[dev] = true;
     }
-    fa4_tc_kernel<T, D><<<units * a.splits, S::THREADS, S::BYTES, st>>>(a);
+    fa4_tc_kernel<T, D, MASK><<<units * a.splits, S::THREADS, S::BYTES, st>>>(a);
     return cudaGetLastError();
+}
+
+template <class T, int D>
+cudaError_t launch(const Fa4Args& a, uint32_t units, cudaStream_t st) {
+    return a.mask ? launch_m<T, D, true>(a, units, st) : launch_m<T, D, false>(a, units, st);
 }
 
 }  // namespace

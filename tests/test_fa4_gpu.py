@@ -145,7 +145,7 @@ def test_many_sequences(dev, dtype, H, Hk, D, group):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
-@pytest.mark.parametrize("T,n,D", [(1, 70, 128), (5, 200, 128), (13, 515, 64), (90, 260, 128), (66, 100, 256)])
+@pytest.mark.parametrize("T,n,D", [(1, 70, 128), (5, 200, 128), (13, 515, 64), (90, 260, 128), (66, 100, 256), (200, 264, 64), (130, 700, 128)])
 def test_masks(dev, dtype, T, n, D):
     """Hidden cells at random, a slope, a row that sees nothing, one that sees one cell, rows of the type's lowest value."""
     rng, q, kb, vb = _inputs(T + n, T, 8, 2, D, n, dtype)
