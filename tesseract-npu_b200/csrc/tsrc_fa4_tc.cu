@@ -645,7 +645,8 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
             tmem_wait_ld64(raw);
 #pragma unroll
             for (int j = 0; j < 64; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * f);
-            uint32_t w0 = ~0u, w1 = ~0u;             // bit j of the words: the row's range holds cell c0 + j
+            // bit j of the words: the row's range holds cell c0 + j; a thread without a row sees none (and has no mask)
+            uint32_t w0 = row < rows ? ~0u : 0u, w1 = w0;
             if (!open) {
                 const int32_t from = min(max(lo - c0, 0), 64), to = min(max(hi - c0, from), 64);
                 const unsigned long long bits = (to >= 64 ? ~0ull : (1ull << to) - 1ull) & ~(from >= 64 ? ~0ull : (1ull << from) - 1ull);

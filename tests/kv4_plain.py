@@ -80,3 +80,32 @@ def beam(logits, scores, n_out):
         first = first[flat[first] > -np.inf]
         res[0][g, :len(first)], res[1][g, :len(first)], res[2][g, :len(first)] = flat[first], first // V, first % V
     return res
+
+
+def attend_many(q, kb, vb, n_head_kv, scale, ranges, mask=None):
+    """attend() by matrices, for many tokens, and the sums that a tolerance needs: (out, sum p |v|, sum p |d|, the largest
+    scale * sum |q||k|, per token and head). Cells with a scale that is no number must be hidden from every token."""
+    T, H, D = q.shape
+    n = len(kb)
+    seen = (np.arange(n) >= np.maximum(np.asarray(ranges)[:, :1], 0)) & (np.arange(n) < np.asarray(ranges)[:, 1:])
+    if mask is not None:
+        seen &= ~np.isneginf(mask[:, :n].astype(np.float64))
+    any_seen = seen.any(0)
+    k, v = (np.where(any_seen[:, None], unpack(b), 0.0).reshape(n, n_head_kv, D) for b in (kb, vb))
+    d = np.abs(np.ascontiguousarray(vb.reshape(n, -1, 18)[..., :2]).view(np.float16).astype(np.float64)).reshape(n, n_head_kv, D // 32)
+    d = np.repeat(np.where(any_seen[:, None, None], d, 0.0), 32, -1)
+    out, pv, pd = (np.zeros((T, H, D)) for _ in range(3))
+    A = np.zeros((T, H, 1))
+    for h in range(H):
+        g = h // (H // n_head_kv)
+        s = q[:, h] @ k[:, g].T * scale
+        if mask is not None:
+            s = s + np.where(seen, mask[:, :n].astype(np.float64), 0.0)
+        s = np.where(seen, s, -np.inf)
+        top = s.max(1, keepdims=True)
+        p = np.exp(s - np.where(np.isneginf(top), 0.0, top))
+        total = p.sum(1, keepdims=True)
+        p = np.divide(p, total, out=np.zeros_like(p), where=total > 0)
+        out[:, h], pv[:, h], pd[:, h] = p @ v[:, g], p @ np.abs(v[:, g]), p @ d[:, g]
+        A[:, h, 0] = np.where(seen, abs(scale) * (np.abs(q[:, h]) @ np.abs(k[:, g]).T), 0.0).max(1)
+    return out, pv, pd, A

@@ -163,6 +163,98 @@ def test_masks(dev, dtype, T, n, D):
     _check(dev, q, kb, vb, 2, dtype, ranges, mask=mask)
 
 
+def _compare_many(got, want, pv, pd, A, D, n, dtype, spread):
+    e = 2.0 ** -24
+    ds = ((3 * D / 16 + 16) + 2) * e * A + 4 * e * spread
+    tol = (2 * ds + 2.0 ** -20 + 64 * e) * pv + (34 * (n / 64 + 2) + 4) * e * 16 * pd
+    tol += np.maximum(HALF[dtype] * np.abs(want), 2.0 ** -25 if dtype == "float16" else 0.0) + 1e-30
+    if dtype == "bfloat16":
+        tol += 2.0 ** -10 * (A + 1) * pv
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (int(bad.sum()), bad.size, float(np.nanmax(np.abs(got - want) / tol)), np.argwhere(bad)[:3].tolist())
+
+
+def _check_many(dev, q, kb, vb, Hk, dtype, ranges, scale=None):
+    """_check by matrices."""
+    T, H, D = q.shape
+    scale = float(np.float32(1 / np.sqrt(D))) if scale is None else scale
+    want, pv, pd, A = P.attend_many(q.double().cpu().numpy(), kb, vb, Hk, scale, ranges)
+    got = _run(dev, q, kb, vb, Hk, scale, ranges)
+    _compare_many(got, want, pv, pd, A, D, len(kb), dtype, 0.0)
+
+
+# (T, n, H, Hk, D): a last row tile of a few rows, all cells in a split; splits over the cells; one tile of rows; a short prompt
+MANY = [(70, 1500, 32, 8, 128), (70, 4200, 32, 8, 64), (64, 6000, 8, 1, 128), (301, 301, 32, 8, 128), (513, 513, 14, 2, 64), (40, 9000, 32, 8, 128)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("T,n,H,Hk,D", MANY)
+def test_many_rows_causal(dev, dtype, T, n, H, Hk, D):
+    _, q, kb, vb = _inputs(T + n, T, H, Hk, D, n, dtype)
+    _check_many(dev, q, kb, vb, Hk, dtype, [[0, n - T + t + 1] for t in range(T)])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("T,n,H,Hk,D", MANY)
+def test_many_rows_masks_windows_and_hidden_cells(dev, dtype, T, n, H, Hk, D):
+    """A mask with hidden cells, empty rows and rows of the type's lowest value; windows; what hides, and the mask beside
+    the ranges, holds NaN, infinities and huge scales. Also a mask whose rows start off every wide boundary."""
+    import torch
+    rng, q, kb, vb = _inputs(T * 3 + n, T, H, Hk, D, n, dtype)
+    mask = np.where(rng.random((T, n)) < 0.3, -np.inf, -0.001 * np.arange(n)[::-1]).astype(np.float16)
+    mask[1] = -np.inf
+    mask[2] = np.finfo(np.float16).min
+    mask[3, : n // 2] = np.finfo(np.float16).min
+    ranges = np.array([[max(0, n - T + t + 1 - (700 if t % 3 else n)), n - T + t + 1] for t in range(T)])
+    ranges[5] = [9, 9]
+    ranges[6] = [n + 5, n + 9]
+    ranges[7] = [-5, n + 100]
+    hidden = np.arange(20, n, 97)
+    mask[:, hidden] = -np.inf
+    for rows in (kb, vb):
+        b = rows.reshape(n, -1, 18)
+        for i, c in enumerate(hidden):
+            bits = (0x7E00, 0x7C00, 0xFC00, 0x7BFF)[i % 4]
+            b[c, :, :2] = np.array([bits & 255, bits >> 8], np.uint8)
+    beside = (np.arange(n) < ranges[:, :1]) | (np.arange(n) >= ranges[:, 1:])
+    mask[beside] = np.where(rng.random(int(beside.sum())) < 0.5, np.nan, np.inf).astype(np.float16)
+    clean = np.where(beside, np.float16(-np.inf), mask)
+    q64 = q.double().cpu().numpy()
+    want, pv, pd, A = P.attend_many(q64, kb, vb, Hk, float(np.float32(1 / np.sqrt(D))), ranges, clean)
+    got = _run(dev, q, kb, vb, Hk, float(np.float32(1 / np.sqrt(D))), ranges, mask)
+    _compare_many(got, want, pv, pd, A, D, n, dtype, 0.001 * n)
+    wide = np.full((T, n + 3), 7.0, np.float16)
+    wide[:, :n] = clean
+    kv = dev.kv4_create(Hk, D, n)
+    try:
+        kv.set_bytes(tsrc.KV_K, kb)
+        kv.set_bytes(tsrc.KV_V, vb)
+        out = torch.full_like(q, float("nan"))
+        dev.flash_attn_q4(kv, q, out, T=T, n_head=H, n_kv=n, scale=float(np.float32(1 / np.sqrt(D))), mask=torch.from_numpy(wide).cuda(),
+                          ranges=torch.from_numpy(ranges.astype(np.int32)).cuda())
+        dev.sync()
+        _compare_many(out.double().cpu().numpy(), want, pv, pd, A, D, n, dtype, 0.001 * n)
+    finally:
+        kv.free()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_rows_magnitudes(dev, dtype, D):
+    """Scales from tiny to far above the common ones, differing from cell to cell, in tiles of the kernel for many rows."""
+    import torch
+    T, n, H, Hk = 300, 300, 32, 8
+    for qs, ks, vs, scale in ((1e3, 1e-3, 1e-4, 0.09), (1e-3, 3e2, 2e3, 0.05), (3e2, 1.0, 1.0, 0.0003), (1.0, 1.0, 6e-6, 0.0), (1.0, 20.0, 60.0, -0.004)):
+        rng, q, kb, vb = _inputs(int(10 * ks) + D, T, H, Hk, D, n, "float32")
+        q = (q * qs).to(getattr(torch, dtype))
+        for rows, f in ((kb, ks), (vb, vs)):
+            b = rows.reshape(n, -1, 18)
+            d = np.ascontiguousarray(b[..., :2]).view(np.float16).astype(np.float32) * f
+            d *= np.where(rng.random(d.shape) < 0.1, 8.0, 1.0)
+            b[..., :2] = d.astype(np.float16).view(np.uint8).reshape(b[..., :2].shape)
+        _check_many(dev, q, kb, vb, Hk, dtype, [[t % 3, n] for t in range(T)], scale=scale)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("T", [1, 80])
 def test_what_is_hidden_has_no_effect(dev, dtype, T):
