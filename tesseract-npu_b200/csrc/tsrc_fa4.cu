@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(128) fa4_merge_kernel(Fa4Args a) {
 // The shape of a call: which rows a CTA takes and how the cells are split.
 struct Fa4Plan {
     int mode;
-    uint32_t group, row_tiles, units, splits;
+    uint32_t group, row_tiles, units, splits, tile_rows;
     size_t o_bytes, ml_bytes;                  // of the workspace, where a merge kernel joins the splits
 };
 
@@ -762,9 +762,13 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
         const uint64_t tc = 9000u + (units * splits + places - 1u) / places * ((tiles + splits - 1u) / splits) * each + (splits > 1u ? 6000u : 0u);
         const uint64_t dec = 11000u + (uint64_t)p.units * (len / kDecTile + 1u) * (R == 16u ? 1350u : 930u) / (D == 64u ? 900u : 592u);
         if (tc < dec) {
+            // bf16: 256 rows a CTA from one and a half such CTAs an SM on (2048 rows of 8 KV heads x 4, causal: 74 us, 81 with
+            // 128 rows; 8192 cells behind 4096 rows: 589 and 614; 160 CTAs, a second turn of the SMs for a few: 223 and 214)
+            const uint64_t wide = (uint64_t)(T / p.group) * n_head_kv * ((rows + 2u * kFa4TcRows - 1u) / (2u * kFa4TcRows));
             p.mode = kRows128;
-            p.row_tiles = (rows + kFa4TcRows - 1u) / kFa4TcRows;
-            p.units = (uint32_t)units;
+            p.tile_rows = type == TSRC_TYPE_BF16 && 2u * wide >= 3u * kSms ? 2u * kFa4TcRows : kFa4TcRows;
+            p.row_tiles = (rows + p.tile_rows - 1u) / p.tile_rows;
+            p.units = (uint32_t)(p.tile_rows > kFa4TcRows ? wide : units);
             p.splits = (uint32_t)splits;
             if (p.splits > 1u) {
                 p.o_bytes = (size_t)p.units * p.splits * kFa4TcRows * D * 4u;
@@ -939,6 +943,7 @@ int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const v
     a.scale = scale;
     a.group = p.group;
     a.row_tiles = p.row_tiles;
+    a.tile_rows = p.tile_rows;
     a.splits = p.splits;
     if (p.o_bytes) {
         a.part_o = static_cast<float*>(ws);

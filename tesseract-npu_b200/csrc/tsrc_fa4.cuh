@@ -17,6 +17,7 @@ struct Fa4Args {
     const __half* mask;
     size_t mask_stride;
     float scale;
+    uint32_t tile_rows;                        // rows of a row tile, in the kernel for many rows
     uint32_t group, row_tiles, splits;         // tokens a group, row tiles a group and KV head, splits of the cells
     float *part_o, *part_ml;                   // splits joined by the merge kernel: [unit][split][R][D], [unit][split][R][4]
 };
@@ -40,7 +41,8 @@ __device__ __forceinline__ void store4(T* p, const float (&x)[4], bool wide) {
     }
 }
 
-// Many query rows on one stretch of cells: D 64 or 128, row tiles of 128 (tsrc_fa4_tc.cu).
+// Many query rows on one stretch of cells: D 64 or 128, row tiles of 128, or of 256 for bf16 (one split)
+// (tsrc_fa4_tc.cu).
 constexpr uint32_t kFa4TcRows = 128;
 cudaError_t launch_fa4_tc(uint32_t type, uint32_t D, const Fa4Args& a, uint32_t units, cudaStream_t st);
 // The error word of its waits (kKv4ErrWait), cleared when read with clear = true.

@@ -2,15 +2,16 @@
 // fifth-generation tensor cores. Layout of the cache: tsrc_kv4.cuh; the entry point and the rule that chooses
 // between this kernel and the one for few rows: tsrc_fa4.cu.
 //
-// A CTA takes 128 query rows -- the (token, head) pairs of a group that share a KV head -- and passes over the cells
-// they span in tiles of 64, its warps in three roles that hand over by mbarriers:
+// A CTA takes 128 query rows -- the (token, head) pairs of a group that share a KV head -- or two lots of 128 that share
+// the dequantized tiles (bf16 outputs, where that fills the SMs), and passes over the cells they span in tiles of 64, its
+// warps in three roles that hand over by mbarriers:
 //   dequant (4 or 8 warps)  codes and scales from global memory (a tile ahead, in registers) to fp16 operands in
 //                      shared memory: K as [8 values][cell][16 B], V transposed as [8 cells][value][16 B], the
 //                      tensor cores' unswizzled layout, every 16-byte store of a quarter warp side by side. Two buffers
 //                      each.
 //   products (1 thread)  S(i + 1) = Q K^T while the softmax of tile i runs, then O += P(i) V; S twice and O in tensor
 //                      memory, P written over its S.
-//   softmax (4 warps)  a thread per row: scores from tensor memory, running sum, weights back as fp16.
+//   softmax (4 warps for 128 rows)  a thread per row: scores from tensor memory, running sum, weights back as fp16.
 // The reference that the weights' exponents are taken from follows the running maximum only when that has risen by
 // 8 (in log2): outputs in tensor memory are then rescaled, seldom after the first tiles; up to there weights reach
 // 2^8, which fp16 holds, and results do not depend on the reference.
@@ -33,26 +34,29 @@ __device__ unsigned int g_fa4_error;                 // kKv4ErrWait once a wait 
 constexpr uint32_t kTile = 64, kRows = 128;
 constexpr long long kWaitCycles = 1ll << 31;         // a wait gives up after ~1 s of SM clock
 
-template <class T, int D> struct TcShape {
+template <class T, int D, uint32_t RG> struct TcShape {                             // RG: lots of 128 rows
     static constexpr bool PRECISE = !std::is_same_v<T, __nv_bfloat16>;              // two terms of K, V and the weights
     static constexpr bool TOTAL = std::is_same_v<T, float>;                         // two of q (fp16 is one), outputs in total
     static constexpr uint32_t NB = D / 32, TERMS = PRECISE ? 2 : 1;
     static constexpr uint32_t Q_TERM = kRows * D * 2, KV_TERM = kTile * D * 2;      // bytes of one term of an operand
-    static constexpr uint32_t K_AT = Q_TERM * (TOTAL ? 2 : 1), V_AT = K_AT + 2 * KV_TERM * TERMS;
+    static constexpr uint32_t Q_ROWS = Q_TERM * (TOTAL ? 2 : 1), K_AT = Q_ROWS * RG, V_AT = K_AT + 2 * KV_TERM * TERMS;
     static constexpr uint32_t CTL_AT = V_AT + 2 * KV_TERM * TERMS;
-    // two CTAs an SM at most: tensor memory holds no more
-    static constexpr uint32_t BYTES = CTL_AT + 3072 < 100 * 1024 ? 100 * 1024 : CTL_AT + 3072;
-    static constexpr uint32_t MIN_CTAS = 2 * (BYTES + 1024) <= 227 * 1024 ? 2 : 1;
-    static constexpr uint32_t DW = MIN_CTAS == 1 ? 8 : 4, THREADS = 160 + 32 * DW;   // dequant warps
+    // two CTAs an SM at most, or one that takes all of tensor memory
+    static constexpr uint32_t WANT = CTL_AT + 4096;
+    static constexpr uint32_t MIN_CTAS = RG == 1 && 2 * (WANT + 1024) <= 227 * 1024 ? 2 : 1;
+    static constexpr uint32_t LEAST = MIN_CTAS == 2 ? 100 * 1024 : 116 * 1024, BYTES = WANT < LEAST ? LEAST : WANT;
+    static constexpr uint32_t DW = MIN_CTAS == 1 ? 8 : 4, SW = 4 * RG;              // dequant, softmax warps
+    static constexpr uint32_t WARPS = SW + DW + 1, THREADS = 32 * WARPS;
     static constexpr uint32_t KU = 8 / DW, BV = 8 / DW;                             // a lane's cells of K, blocks of V
-    // tensor-memory columns: score buffers (P over each), O. With four, S(i + 1) need not wait for the products of
-    // P(i - 1), and the tensor cores never stop; two CTAs on an SM have room for two each.
-    static constexpr uint32_t NS = MIN_CTAS == 1 ? 4 : 2, O_COL = NS * kTile, COLUMNS = MIN_CTAS == 1 ? 512 : 256;
+    // tensor-memory columns: score buffers (P over each) of each lot of rows, then the outputs. With four buffers S(i + 1)
+    // need not wait for the products of P(i - 1), and the tensor cores never stop; two CTAs or two lots of rows have room
+    // for two each.
+    static constexpr uint32_t NS = MIN_CTAS == 1 && RG == 1 ? 4 : 2, O_COL = RG * NS * kTile, COLUMNS = MIN_CTAS == 1 ? 512 : 256;
     // The tensor cores cut every sum towards zero, about 2^-25 of it a product, so a row's output would shrink by 1e-5
     // over 60 tiles of twelve products. For f32 outputs FLUSH tiles are added up there, and then to the total, in tensor
     // memory too, by an ordinary f32 addition.
     static constexpr uint32_t FLUSH = 4, SUM_COL = O_COL + D;
-    static_assert(SUM_COL + (TOTAL ? D : 0) <= COLUMNS, "tensor memory");
+    static_assert(O_COL + RG * D <= COLUMNS && SUM_COL + (TOTAL ? D : 0) <= COLUMNS && (RG == 1 || !TOTAL), "tensor memory");
 };
 
 struct TileInfo {
@@ -63,19 +67,20 @@ struct TileInfo {
 };
 constexpr uint32_t kFarExp = 19;     // exponent field of scales of 16 to 32, the largest that the common powers follow
 
-struct Control {                     // at most 3 KB
-    uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[4], p_full[4];
+struct Control {                     // at most 4 KB
+    uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
+    uint64_t s_full[2][4], p_full[2][4], o_done[2][2];    // of a lot of rows
     TileInfo info[4];
     // far tiles: what a cell's scores are times, and what the log2 of its weights is raised by. Of four tiles, as info:
     // the dequant warps are up to two tiles ahead of the softmax when they write these.
     float cell_k[4][kTile], cell_v[4][kTile];
     uint32_t most[2][8][2];  // the dequant warps' largest |d| of K and V, by tile parity
     uint32_t tmem, abort;
-    int32_t span[4][2];      // the softmax warps' first and last cell
-    float q_unscale[kRows];
+    int32_t span[8][2];      // the softmax warps' first and last cell
+    float q_unscale[2 * kRows];
 };
 
-static_assert(sizeof(Control) <= 3072, "room behind the operands");
+static_assert(sizeof(Control) <= 4096, "room behind the operands");
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n) : "memory"); }
@@ -270,9 +275,9 @@ __device__ __forceinline__ void settle(uint32_t o_at, uint32_t sum_at, float f, 
     }
 }
 
-template <class T, int D, bool MASK>
-__global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTAS) fa4_tc_kernel(Fa4Args a) {
-    using S = TcShape<T, D>;
+template <class T, int D, bool MASK, uint32_t RG>
+__global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>::MIN_CTAS) fa4_tc_kernel(Fa4Args a) {
+    using S = TcShape<T, D, RG>;
     constexpr bool PRECISE = S::PRECISE, TOTAL = S::TOTAL;
     constexpr uint32_t NB = S::NB;
     extern __shared__ __align__(1024) uint8_t sm[];
@@ -282,7 +287,7 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
     const uint32_t split = blockIdx.x % a.splits, place = blockIdx.x / a.splits;
     const uint32_t hk = place % a.n_head_kv, rest = place / a.n_head_kv;
     const uint32_t rt = a.row_tiles - 1u - rest % a.row_tiles, grp = rest / a.row_tiles;
-    const uint32_t rows = a.group * a.G, row = rt * kRows + tid;
+    const uint32_t rows = a.group * a.G, row = rt * kRows * RG + tid;
     const uint32_t tok = grp * a.group + row / a.G, head = hk * a.G + row % a.G;
 
     if (warp == 0) {
@@ -296,15 +301,16 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
                 bar_init(&c.v_full[i], S::DW);
                 bar_init(&c.v_free[i], 1);
             }
-            for (int i = 0; i < 4; ++i) {
-                bar_init(&c.s_full[i], 2);           // the tensor cores, and the issuing thread for what it has seen
-                bar_init(&c.p_full[i], 4);
+            for (uint32_t i = 0; i < 4 * RG; ++i) {
+                bar_init(&c.s_full[i / 4][i % 4], 2);      // the tensor cores, and the issuing thread for what it has seen
+                bar_init(&c.p_full[i / 4][i % 4], 4);
             }
+            for (uint32_t i = 0; i < 2 * RG; ++i) bar_init(&c.o_done[i / 2][i % 2], 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
     }
     int32_t lo = 0, hi = 0;
-    if (warp < 4) {
+    if (warp < S::SW) {
         if (row < rows) {
             hi = (int32_t)a.n_kv;
             if (a.ranges) {
@@ -321,8 +327,8 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
     }
     // q, eight rows at a time by a warp: the row's largest value to [2^12, 2^13), chunks of eight values in the order
     // 0 4 1 5 2 6 3 7 that K has
-    for (uint32_t r0 = 8u * warp; warp < 4u + S::DW && r0 < kRows; r0 += 8u * (4u + S::DW)) {
-        const uint32_t r = r0 + (lane & 7u), row_r = rt * kRows + r;
+    for (uint32_t r0 = 8u * warp; warp < S::SW + S::DW && r0 < kRows * RG; r0 += 8u * (S::SW + S::DW)) {
+        const uint32_t r = r0 + (lane & 7u), row_r = rt * kRows * RG + r;
         const uint32_t tok_r = grp * a.group + row_r / a.G, head_r = hk * a.G + row_r % a.G;
         const T* q = static_cast<const T*>(a.q) + (size_t)tok_r * a.q_stride + (size_t)head_r * D + 8u * (lane >> 3);
         float x[D / 32][8], top = 0.0f;
@@ -355,7 +361,7 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
                     l[i] = as_u32(__floats2half2_rn(u - back.x, v - back.y));
                 }
             }
-            uint8_t* p = sm + (4u * j + (lane >> 3)) * (kRows * 16u) + r * 16u;
+            uint8_t* p = sm + r / kRows * S::Q_ROWS + (4u * j + (lane >> 3)) * (kRows * 16u) + r % kRows * 16u;
             *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
             if (TOTAL) *reinterpret_cast<uint4*>(p + S::Q_TERM) = make_uint4(l[0], l[1], l[2], l[3]);
         }
@@ -365,66 +371,73 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
     __syncthreads();
     fence_after();
     const uint32_t tmem = c.tmem;
-    const int32_t first = min(min(c.span[0][0], c.span[1][0]), min(c.span[2][0], c.span[3][0]));
-    const int32_t last = max(max(c.span[0][1], c.span[1][1]), max(c.span[2][1], c.span[3][1]));
+    int32_t first = c.span[0][0], last = c.span[0][1];
+#pragma unroll
+    for (uint32_t w = 1; w < S::SW; ++w) {
+        first = min(first, c.span[w][0]);
+        last = max(last, c.span[w][1]);
+    }
     const uint32_t from = last > first ? (uint32_t)first / kTile : 0u;
     const uint32_t span = last > first ? ((uint32_t)last + kTile - 1u) / kTile - from : 0u;
     const uint32_t tile0 = from + (uint32_t)((uint64_t)span * split / a.splits);             // this split's tiles
     const uint32_t tiles = from + (uint32_t)((uint64_t)span * (split + 1u) / a.splits) - tile0;
 
-    if (warp == 4u + S::DW) {
+    if (warp == S::SW + S::DW) {
         // ---- products, issued by one thread. Descriptors are made once and advanced by constants: made anew for every
         // product they cost the issuing thread 90 cycles each, more than a 128 x 64 x 16 product takes (48).
         uint32_t one;
         asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
         if (one) {
             const uint64_t q_op = operand(smem_u32(sm), kRows), k_op = operand(smem_u32(sm) + S::K_AT, kTile), v_op = operand(smem_u32(sm) + S::V_AT, D);
-            auto scores = [&](uint32_t i) {          // S(i)
+            auto scores = [&](uint32_t i, uint32_t rg) {   // S(i) of a lot of rows
                 const uint32_t buf = i & 1u, sb = i % S::NS;
                 // it takes the place of P(i - 2), or of P(i - 4): then the products of P(i - 3), the latest whose phase is
                 // still the barrier's last, are waited for
                 constexpr uint32_t BACK = S::NS == 2 ? 2 : 3;
-                if (i >= BACK && !bar_wait(&c.v_free[(i - BACK) & 1u], ((i - BACK) >> 1) & 1u, &c.abort)) return false;
+                if (i >= BACK && !bar_wait(&c.o_done[rg][(i - BACK) & 1u], ((i - BACK) >> 1) & 1u, &c.abort)) return false;
                 if (!bar_wait(&c.k_full[buf], (i >> 1) & 1u, &c.abort)) return false;
                 fence_after();
-                const uint64_t kb = k_op + buf * (S::KV_TERM * S::TERMS >> 4);
-                const uint32_t to = tmem + sb * kTile;
+                const uint64_t kb = k_op + buf * (S::KV_TERM * S::TERMS >> 4), qa = q_op + rg * (S::Q_ROWS >> 4);
+                const uint32_t to = tmem + (rg * S::NS + sb) * kTile;
 #pragma unroll
                 for (uint32_t k = PRECISE ? 3 : 1; k-- > 0;) {         // q k_lo, q_lo k, q k: the small ones first, so that
                     if (k == 1 && !TOTAL) continue;                    // what is cut from them is small
 #pragma unroll
                     for (uint32_t s = 0; s < D / 16; ++s)
-                        mma_ss(to, q_op + ((k == 1 ? S::Q_TERM : 0u) + s * 2u * kRows * 16u >> 4), kb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * kTile * 16u >> 4),
+                        mma_ss(to, qa + ((k == 1 ? S::Q_TERM : 0u) + s * 2u * kRows * 16u >> 4), kb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * kTile * 16u >> 4),
                                instruction(kTile), k != (PRECISE ? 2u : 0u) || s != 0u);
                 }
-                commit(&c.k_free[buf]);
-                commit(&c.s_full[sb]);
-                bar_arrive(&c.s_full[sb]);
+                if (rg + 1u == RG) commit(&c.k_free[buf]);
+                commit(&c.s_full[rg][sb]);
+                bar_arrive(&c.s_full[rg][sb]);
                 return true;
             };
-            auto outputs = [&](uint32_t i) {         // O += P(i) V
+            auto outputs = [&](uint32_t i, uint32_t rg) {  // O += P(i) V
                 const uint32_t buf = i & 1u, sb = i % S::NS;
-                if (!bar_wait(&c.v_full[buf], (i >> 1) & 1u, &c.abort) || !bar_wait(&c.p_full[sb], (i / S::NS) & 1u, &c.abort)) return false;
+                if (!bar_wait(&c.v_full[buf], (i >> 1) & 1u, &c.abort) || !bar_wait(&c.p_full[rg][sb], (i / S::NS) & 1u, &c.abort)) return false;
                 fence_after();
                 const uint64_t vb = v_op + buf * (S::KV_TERM * S::TERMS >> 4);
-                const uint32_t pa = tmem + sb * kTile;
+                const uint32_t pa = tmem + (rg * S::NS + sb) * kTile;
 #pragma unroll
                 for (uint32_t k = PRECISE ? 3 : 1; k-- > 0;)           // p v_lo, p_lo v, p v
 #pragma unroll
                     for (uint32_t s = 0; s < kTile / 16; ++s)
-                        mma_ts(tmem + S::O_COL, pa + (k == 1 ? kTile / 2u : 0u) + 8u * s, vb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * D * 16u >> 4),
+                        mma_ts(tmem + S::O_COL + rg * D, pa + (k == 1 ? kTile / 2u : 0u) + 8u * s, vb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * D * 16u >> 4),
                                instruction(D), k == (PRECISE ? 2u : 0u) && s == 0u ? (TOTAL ? i % S::FLUSH : i) : 1u);
-                commit(&c.v_free[buf]);
+                commit(&c.o_done[rg][buf]);
+                if (rg + 1u == RG) commit(&c.v_free[buf]);
                 return true;
             };
-            bool ok = tiles == 0 || scores(0);
-            for (uint32_t i = 0; ok && i < tiles; ++i) ok = (i + 1u == tiles || scores(i + 1u)) && outputs(i);
+            bool ok = true;
+            for (uint32_t rg = 0; ok && tiles && rg < RG; ++rg) ok = scores(0, rg);
+            for (uint32_t i = 0; ok && i < tiles; ++i)
+                for (uint32_t rg = 0; ok && rg < RG; ++rg) ok = (i + 1u == tiles || scores(i + 1u, rg)) && outputs(i, rg);
         }
         __syncwarp();
-    } else if (warp >= 4) {
+    } else if (warp >= S::SW) {
         // ---- dequant
         constexpr uint32_t KU = S::KU, BV = S::BV;
-        const uint32_t dw = warp - 4u;
+        const uint32_t dw = warp - S::SW;
         // K: unit u is cell kc + 8 u, values 8t .. 8t + 7 of every block, t = lane / 8
         const uint32_t kt = lane >> 3, kc = 8u * KU * dw + (lane & 7u);
         const size_t plane = (size_t)hk * a.n_alloc + (size_t)tile0 * kTile;
@@ -520,7 +533,7 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
             const uint32_t k_exp = min(max(xk >> 10, 1u), kFarExp);
             v_exp = min(max(v_exp, xv >> 10), kFarExp);
             const bool far = max(xk, xv) >> 10 > kFarExp;
-            if (tid == 128) c.info[i & 3u] = TileInfo{pow2((int)k_exp - 15 + Scaled<PRECISE>::UNDO), v_exp, bad, far};
+            if (dw == 0 && lane == 0) c.info[i & 3u] = TileInfo{pow2((int)k_exp - 15 + Scaled<PRECISE>::UNDO), v_exp, bad, far};
             __half2 k_one[KU], v_one[4];             // powers of two that take the scales to [1, 2) at most
 #pragma unroll
             for (uint32_t u = 0; u < KU; ++u) k_one[u] = to_one(k_exp);
@@ -607,7 +620,7 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
         }
     } else {
         // ---- softmax: this thread's row
-        const uint32_t mine = tmem + ((warp * 32u) << 16);
+        const uint32_t rg = warp / 4u, mine = tmem + ((warp % 4u * 32u) << 16), o_at = mine + S::O_COL + rg * D;
         const float qs = c.q_unscale[tid];           // this row's scale, for scores in log2
         float m = -INFINITY, l = 0.0f;               // reference of the weights' exponents; running sum, both in units of 2^6 p
         float off = MASK ? -INFINITY : 0.0f;         // the mask's maximum so far: scores and m are relative to it
@@ -618,9 +631,9 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
         const int32_t all_lo = __reduce_max_sync(0xFFFFFFFFu, row < rows ? lo : 0), all_hi = __reduce_min_sync(0xFFFFFFFFu, row < rows ? hi : 0x7FFFFFFF);
 #pragma unroll 1
         for (uint32_t i = 0; ok && i < tiles; ++i) {
-            const uint32_t buf = i & 1u, sb = i % S::NS, at = mine + sb * kTile;
+            const uint32_t buf = i & 1u, sb = i % S::NS, at = mine + (rg * S::NS + sb) * kTile;
             const int32_t c0 = (int32_t)((tile0 + i) * kTile);
-            ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.s_full[sb], (i / S::NS) & 1u, &c.abort));
+            ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.s_full[rg][sb], (i / S::NS) & 1u, &c.abort));
             if (!ok) break;
             fence_after();
             const TileInfo info = c.info[i & 3u];
@@ -698,11 +711,11 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
                 }
                 if (i > 0) {
                     // the products so far have to be there
-                    ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.v_free[buf ^ 1u], ((i - 1u) >> 1) & 1u, &c.abort));
+                    ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.o_done[rg][buf ^ 1u], ((i - 1u) >> 1) & 1u, &c.abort));
                     if (!ok) break;
                     fence_after();
-                    if constexpr (TOTAL) settle<D>(mine + S::O_COL, mine + S::SUM_COL, both, i <= S::FLUSH, flush);
-                    else rescale<D>(mine + S::O_COL, both);
+                    if constexpr (TOTAL) settle<D>(o_at, mine + S::SUM_COL, both, i <= S::FLUSH, flush);
+                    else rescale<D>(o_at, both);
                 }
             }
             const float up = m == -INFINITY ? 0.0f : 6.0f - m;
@@ -746,7 +759,7 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
             tmem_wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(&c.p_full[sb]);
+            if (lane == 0) bar_arrive(&c.p_full[rg][sb]);
             if (info.bad) {                          // seldom: which of the blocks left out of V this row would have met
 #pragma unroll 1
                 for (uint32_t j = 0; j < kTile; ++j) {
@@ -758,21 +771,21 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
             }
         }
         // every product has ended: the outputs are there, and the tensor memory may go
-        if (ok && tiles) ok = bar_wait(&c.v_free[(tiles - 1u) & 1u], ((tiles - 1u) >> 1) & 1u, &c.abort);
+        if (ok && tiles) ok = bar_wait(&c.o_done[rg][(tiles - 1u) & 1u], ((tiles - 1u) >> 1) & 1u, &c.abort);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (ok) {
             fence_after();
             // l and O are in units of 2^6 p: a split's share names 2^-6 of its reference
             const float unit = pow2((int)v_exp - 15 + Scaled<PRECISE>::UNDO), f = a.splits > 1u ? unit : l == 0.0f ? 0.0f : unit / l;
             T* out = static_cast<T*>(a.out) + (size_t)tok * a.out_stride + (size_t)head * D;
-            const size_t part = ((((size_t)grp * a.row_tiles + rt) * a.n_head_kv + hk) * a.splits + split) * kRows + tid;
+            const size_t part = ((((size_t)grp * a.row_tiles + rt) * a.n_head_kv + hk) * a.splits + split) * (kRows * RG) + tid;
             if (a.splits > 1u && row < rows) *reinterpret_cast<float4*>(a.part_ml + part * 4u) = make_float4(off, m - 6.0f, l, 0.0f);
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
                 uint32_t o[32] = {};
                 if (tiles) {
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) tmem_ld8(mine + S::O_COL + j * (D / 4) + 8u * b, o + 8 * j);
+                    for (uint32_t j = 0; j < 4; ++j) tmem_ld8(o_at + j * (D / 4) + 8u * b, o + 8 * j);
                     tmem_wait_ld(o);
                     if (TOTAL && tiles > S::FLUSH) {
                         uint32_t t[32];
@@ -808,25 +821,31 @@ __global__ void __launch_bounds__(TcShape<T, D>::THREADS, TcShape<T, D>::MIN_CTA
     }
 }
 
-template <class T, int D, bool MASK>
+template <class T, int D, bool MASK, uint32_t RG>
 cudaError_t launch_m(const Fa4Args& a, uint32_t units, cudaStream_t st) {
-    using S = TcShape<T, D>;
+    using S = TcShape<T, D, RG>;
     static bool done[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !done[dev]) {
-        e = cudaFuncSetAttribute(fa4_tc_kernel<T, D, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
+        e = cudaFuncSetAttribute(fa4_tc_kernel<T, D, MASK, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
         if (e != cudaSuccess) return e;
         if (dev < 64) done[dev] = true;
     }
-    fa4_tc_kernel<T, D, MASK><<<units * a.splits, S::THREADS, S::BYTES, st>>>(a);
+    fa4_tc_kernel<T, D, MASK, RG><<<units * a.splits, S::THREADS, S::BYTES, st>>>(a);
     return cudaGetLastError();
 }
 
+template <class T, int D, uint32_t RG>
+cudaError_t launch_g(const Fa4Args& a, uint32_t units, cudaStream_t st) {
+    return a.mask ? launch_m<T, D, true, RG>(a, units, st) : launch_m<T, D, false, RG>(a, units, st);
+}
 template <class T, int D>
 cudaError_t launch(const Fa4Args& a, uint32_t units, cudaStream_t st) {
-    return a.mask ? launch_m<T, D, true>(a, units, st) : launch_m<T, D, false>(a, units, st);
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
+        if (a.tile_rows == 2u * kFa4TcRows) return launch_g<T, D, 2>(a, units, st);
+    return launch_g<T, D, 1>(a, units, st);
 }
 
 }  // namespace

@@ -183,8 +183,10 @@ def _check_many(dev, q, kb, vb, Hk, dtype, ranges, scale=None):
     _compare_many(got, want, pv, pd, A, D, len(kb), dtype, 0.0)
 
 
-# (T, n, H, Hk, D): a last row tile of a few rows, all cells in a split; splits over the cells; one tile of rows; a short prompt
-MANY = [(70, 1500, 32, 8, 128), (70, 4200, 32, 8, 64), (64, 6000, 8, 1, 128), (301, 301, 32, 8, 128), (513, 513, 14, 2, 64), (40, 9000, 32, 8, 128)]
+# (T, n, H, Hk, D): a last row tile of a few rows, all cells in a split; splits over the cells; one tile of rows; a short prompt;
+# enough rows for CTAs of 256, their second half filled, with a few rows, empty
+MANY = [(70, 1500, 32, 8, 128), (70, 4200, 32, 8, 64), (64, 6000, 8, 1, 128), (301, 301, 32, 8, 128), (513, 513, 14, 2, 64), (40, 9000, 32, 8, 128),
+        (1300, 1400, 44, 11, 64), (300, 333, 120, 120, 128), (333, 500, 150, 75, 128)]
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
