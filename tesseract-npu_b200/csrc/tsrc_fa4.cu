@@ -739,6 +739,7 @@ struct Fa4Plan {
     size_t o_bytes, ml_bytes;                  // of the workspace, where a merge kernel joins the splits
 };
 
+constexpr uint32_t kMaxT = 1u << 20;
 Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint32_t n_head, uint32_t n_kv, uint32_t group, uint32_t max_len) {
     Fa4Plan p{};
     p.group = group ? group : T;
@@ -885,7 +886,7 @@ const char* tsrc_flash_attn_q4_unsupported(uint32_t type, uint32_t n_head_kv, ui
 
 size_t tsrc_flash_attn_q4_workspace(uint32_t type, uint32_t n_head_kv, uint32_t head_dim, uint32_t T, uint32_t n_head,
                                     uint32_t n_kv, uint32_t group, uint32_t max_len) {
-    if (T == 0 || tsrc_flash_attn_q4_unsupported(type, n_head_kv, head_dim, n_head)) return 0;
+    if (T == 0 || T > kMaxT || (group && T % group) || tsrc_flash_attn_q4_unsupported(type, n_head_kv, head_dim, n_head)) return 0;
     const Fa4Plan p = fa4_plan(type, n_head_kv, head_dim, T, n_head, n_kv, group, max_len);
     return p.o_bytes + p.ml_bytes;
 }
@@ -906,7 +907,7 @@ int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const v
     if (!std::isfinite(scale)) return set_error(TSRC_E_ARG, "tsrc_flash_attn_q4: scale is not finite");
     if (group == 0) group = T;
     if (T && T % group) return refuse(TSRC_E_ARG, "tsrc_flash_attn_q4: T %u is not a multiple of group %u", T, group);
-    if (T > (1u << 20)) return set_error(TSRC_E_SHAPE, "tsrc_flash_attn_q4: T above 2^20");
+    if (T > kMaxT) return set_error(TSRC_E_SHAPE, "tsrc_flash_attn_q4: T above 2^20");
     const uintptr_t m = kv4_type_size(type) - 1u;
     if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & m) || (reinterpret_cast<uintptr_t>(ranges) & 3u) ||
         (reinterpret_cast<uintptr_t>(mask) & 1u))

@@ -54,6 +54,21 @@ def test_workspace_sizes():
     assert L.tsrc_flash_attn_q4_workspace(F32, 8, 96, 1, 32, 100, 1, 0) == 0
 
 
+@pytest.mark.parametrize("T,group", [(4, 5), (4, 3), (1, 1 << 31), ((1 << 20) + 1, 1), (0xFFFFFFFF, 0), (0, 7)])
+@pytest.mark.parametrize("dim", [128, 256])
+def test_refused_groups_and_token_counts_need_no_workspace(T, group, dim):
+    assert tsrc.lib().tsrc_flash_attn_q4_workspace(F32, 1, dim, T, 64, 1 << 16, group, 0) == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("n_kv", [0, 1, 0xFFFFFFFF])
+@pytest.mark.parametrize("group", [0, 1])
+def test_workspace_at_the_largest_sizes(dim, n_kv, group):
+    """The largest token count and heads, no cell and the largest cell number: a size, and no division by nothing."""
+    for T, heads in ((1, 1), (1, 64), (1 << 20, 64)):
+        assert tsrc.lib().tsrc_flash_attn_q4_workspace(F32, 1, dim, T, heads, n_kv, group, 0) < 1 << 40
+
+
 def test_wrapper_checks_types():
     torch = pytest.importorskip("torch")
     a, b = torch.zeros(2, 64), torch.zeros(2, 64, dtype=torch.float16)
