@@ -763,11 +763,13 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
         const uint64_t tc = 9000u + (units * splits + places - 1u) / places * ((tiles + splits - 1u) / splits) * each + (splits > 1u ? 6000u : 0u);
         const uint64_t dec = 11000u + (uint64_t)p.units * (len / kDecTile + 1u) * (R == 16u ? 1350u : 930u) / (D == 64u ? 900u : 592u);
         if (tc < dec) {
-            // bf16: 256 rows a CTA from one and a half such CTAs an SM on (2048 rows of 8 KV heads x 4, causal: 74 us, 81 with
-            // 128 rows; 8192 cells behind 4096 rows: 589 and 614; 160 CTAs, a second turn of the SMs for a few: 223 and 214)
             const uint64_t wide = (uint64_t)(T / p.group) * n_head_kv * ((rows + 2u * kFa4TcRows - 1u) / (2u * kFa4TcRows));
+            // bf16: 256 rows a CTA where 128 give at least four CTAs to three SMs, and 256, of which an SM holds one, take no
+            // more turns (32 / 8 heads, us with 256 and 128: 2048 tokens, causal 70 and 82; 4096 cells before 640 tokens 109 and
+            // 125; before 1184, in two turns, 193 and 140; 400 tokens 23 and 19). For f16 they win 8 % at most and are not there.
+            const bool two = type == TSRC_TYPE_BF16 && 3u * units >= 4u * kSms && (wide + kSms - 1u) / kSms <= (units + places - 1u) / places;
             p.mode = kRows128;
-            p.tile_rows = type == TSRC_TYPE_BF16 && 2u * wide >= 3u * kSms ? 2u * kFa4TcRows : kFa4TcRows;
+            p.tile_rows = two ? 2u * kFa4TcRows : kFa4TcRows;
             p.row_tiles = (rows + p.tile_rows - 1u) / p.tile_rows;
             p.units = (uint32_t)(p.tile_rows > kFa4TcRows ? wide : units);
             p.splits = (uint32_t)splits;

@@ -15,8 +15,9 @@
 // The reference that the weights' exponents are taken from follows the running maximum only when that has risen by
 // 8 (in log2): outputs in tensor memory are then rescaled, seldom after the first tiles; up to there weights reach
 // 2^8, which fp16 holds, and results do not depend on the reference.
-//   Range: q is scaled by a power of two per row, K's and V's scales by one per tile (V's follows the largest seen,
-// with O rescaled), so that all operands stay inside fp16. Scales of 32 and above, which no row of ordinary size
+//   Range: q is scaled by a power of two per row, K's and V's scales by one per dequant warp's cells, so that all
+// operands stay inside fp16 and the dequant warps need not agree on one. K's is made good in the scores, V's in the
+// weights, relative to the largest seen (with O rescaled when that rises). Scales of 32 and above, which no row of ordinary size
 // has, do not move these: such a cell gets a power of two of its own, which its scores and weights make good, so that
 // rows that do not see it keep their digits. Precision: bf16 outputs take one fp16 term (11 bits) of
 // q (exact), K, V and the weights. f32 and f16 outputs take two terms of each, 22 bits (d (n - 8) has 15, so K and V
@@ -41,11 +42,12 @@ template <class T, int D, uint32_t RG> struct TcShape {                         
     static constexpr uint32_t Q_TERM = kRows * D * 2, KV_TERM = kTile * D * 2;      // bytes of one term of an operand
     static constexpr uint32_t Q_ROWS = Q_TERM * (TOTAL ? 2 : 1), K_AT = Q_ROWS * RG, V_AT = K_AT + 2 * KV_TERM * TERMS;
     static constexpr uint32_t CTL_AT = V_AT + 2 * KV_TERM * TERMS;
-    // two CTAs an SM at most, or one that takes all of tensor memory
+    // two CTAs an SM at most, or one that takes all of tensor memory. Two lots of rows take four dequant warps: with eight
+    // the registers a thread may have, 96, do not hold a row's scores (2048 tokens: 71.3 us, 68.6 with four).
     static constexpr uint32_t WANT = CTL_AT + 4096;
     static constexpr uint32_t MIN_CTAS = RG == 1 && 2 * (WANT + 1024) <= 227 * 1024 ? 2 : 1;
     static constexpr uint32_t LEAST = MIN_CTAS == 2 ? 100 * 1024 : 116 * 1024, BYTES = WANT < LEAST ? LEAST : WANT;
-    static constexpr uint32_t DW = MIN_CTAS == 1 ? 8 : 4, SW = 4 * RG;              // dequant, softmax warps
+    static constexpr uint32_t DW = MIN_CTAS == 1 && RG == 1 ? 8 : 4, SW = 4 * RG;              // dequant, softmax warps
     static constexpr uint32_t WARPS = SW + DW + 1, THREADS = 32 * WARPS;
     static constexpr uint32_t KU = 8 / DW, BV = 8 / DW;                             // a lane's cells of K, blocks of V
     // tensor-memory columns: score buffers (P over each) of each lot of rows, then the outputs. With four buffers S(i + 1)
@@ -59,12 +61,14 @@ template <class T, int D, uint32_t RG> struct TcShape {                         
     static_assert(O_COL + RG * D <= COLUMNS && SUM_COL + (TOTAL ? D : 0) <= COLUMNS && (RG == 1 || !TOTAL), "tensor memory");
 };
 
-struct TileInfo {
-    float k_unscale;         // the tile's K operand times this is K
-    uint32_t v_exp;          // exponent field that V's scale follows from this tile on
-    uint32_t bad;            // a scale of V that is no number or infinite is in the tile (its block is 0 in the operand)
-    uint32_t far;            // a scale above the common one is in it: the cells' own powers of two count
+// What the dequant warps tell of a tile: each of its own cells, 64 / DW in a row.
+struct __align__(16) TileInfo {
+    float k_unscale[8];      // the K operand times this is K
+    float v_log[8], v_inv[8];    // log2 of what the V operand lacks, and 2 to minus that
+    uint8_t flags[8];        // kBad, kFar
 };
+constexpr uint32_t kBad = 1;         // a scale of V that is no number or infinite is there (its block is 0 in the operand)
+constexpr uint32_t kFar = 2;         // a scale above the common ones is there: the cells' own powers of two count
 constexpr uint32_t kFarExp = 19;     // exponent field of scales of 16 to 32, the largest that the common powers follow
 
 struct Control {                     // at most 4 KB
@@ -74,7 +78,6 @@ struct Control {                     // at most 4 KB
     // far tiles: what a cell's scores are times, and what the log2 of its weights is raised by. Of four tiles, as info:
     // the dequant warps are up to two tiles ahead of the softmax when they write these.
     float cell_k[4][kTile], cell_v[4][kTile];
-    uint32_t most[2][8][2];  // the dequant warps' largest |d| of K and V, by tile parity
     uint32_t tmem, abort;
     int32_t span[8][2];      // the softmax warps' first and last cell
     float q_unscale[2 * kRows];
@@ -161,6 +164,24 @@ __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast
 // 2^(15 - e) in fp16: a scale with exponent field e goes to [1, 2)
 __device__ __forceinline__ __half2 to_one(uint32_t e) {
     return __half2half2(__ushort_as_half(e < 30u ? (unsigned short)((30u - e) << 10) : (unsigned short)0x0200u));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// Two f32 side by side: a b + c, a + b
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 y;
+    asm("{\n\t.reg .b64 a, b, c, y;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 y, a, b, c;\n\tmov.b64 {%0, %1}, y;\n\t}"
+        : "=f"(y.x), "=f"(y.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return y;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 y;
+    asm("{\n\t.reg .b64 a, b, y;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 y, a, b;\n\tmov.b64 {%0, %1}, y;\n\t}"
+        : "=f"(y.x), "=f"(y.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return y;
 }
 // the largest finite magnitude among the four halves of two words
 __device__ __forceinline__ uint32_t finite_most(uint32_t u) {
@@ -346,8 +367,8 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
         const int e2 = min(12 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
-        const float f = pow2(e2);
-        if (lane < 8) c.q_unscale[r] = a.scale * 1.4426950408889634f * pow2(-e2);
+        const float f = copysignf(pow2(e2), a.scale);        // the factor that scores get is positive
+        if (lane < 8) c.q_unscale[r] = fabsf(a.scale) * 1.4426950408889634f * pow2(-e2);
 #pragma unroll
         for (uint32_t j = 0; j < D / 32; ++j) {
             uint32_t h[4], l[4];
@@ -482,8 +503,7 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
                 }
             }
         };
-        uint32_t v_exp = 1;
-        bool ok = true;                              // after a wait that ran out the warps still meet at their barrier
+        bool ok = true;
         if (tiles) {
             load_k(0);
             load_v(0);
@@ -491,7 +511,7 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
 #pragma unroll 1
         for (uint32_t i = 0; i < tiles; ++i) {
             const uint32_t buf = i & 1u, round = i >> 1;
-            // the tile's largest scales, from what the warps hold
+            // the largest scales among the warp's cells
             __half2 mk = __float2half2_rn(0.0f), mv = mk;
 #pragma unroll
             for (uint32_t u = 0; u < KU; ++u)
@@ -502,6 +522,7 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
             uint32_t xk = max(as_u32(mk) & 0xFFFFu, as_u32(mk) >> 16), xv = max(as_u32(mv) & 0xFFFFu, as_u32(mv) >> 16);
             xk = __reduce_max_sync(0xFFFFFFFFu, xk);
             xv = __reduce_max_sync(0xFFFFFFFFu, xv);
+            bool bad = false;
             if (xk >= 0x7C00u) {
                 uint32_t x = 0;
 #pragma unroll
@@ -514,26 +535,18 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
                 uint32_t x = 0;
 #pragma unroll
                 for (uint32_t k = 0; k < 8; ++k) x = max(x, finite_most(vs[k]));
-                xv = __reduce_max_sync(0xFFFFFFFFu, x) | 0x8000u;
+                xv = __reduce_max_sync(0xFFFFFFFFu, x);
+                bad = true;
             }
-            if (lane == 0) {
-                c.most[buf][dw][0] = xk;
-                c.most[buf][dw][1] = xv;
-            }
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * S::DW) : "memory");
-            uint32_t bad = 0;
-            xk = xv = 0;
-#pragma unroll
-            for (uint32_t w = 0; w < S::DW; ++w) {
-                const uint2 v = *reinterpret_cast<const uint2*>(c.most[buf][w]);
-                xk = max(xk, v.x);
-                xv = max(xv, v.y & 0x7FFFu);
-                bad |= v.y >> 15;
-            }
-            const uint32_t k_exp = min(max(xk >> 10, 1u), kFarExp);
-            v_exp = min(max(v_exp, xv >> 10), kFarExp);
+            const uint32_t k_exp = min(max(xk >> 10, 1u), kFarExp), v_exp = min(max(xv >> 10, 1u), kFarExp);
             const bool far = max(xk, xv) >> 10 > kFarExp;
-            if (dw == 0 && lane == 0) c.info[i & 3u] = TileInfo{pow2((int)k_exp - 15 + Scaled<PRECISE>::UNDO), v_exp, bad, far};
+            if (lane == 0) {
+                TileInfo& info = c.info[i & 3u];
+                info.k_unscale[dw] = pow2((int)k_exp - 15 + Scaled<PRECISE>::UNDO);
+                info.v_log[dw] = (float)((int)v_exp - 15 + Scaled<PRECISE>::UNDO);
+                info.v_inv[dw] = pow2(15 - Scaled<PRECISE>::UNDO - (int)v_exp);
+                info.flags[dw] = (uint8_t)((bad ? kBad : 0u) | (far ? kFar : 0u));
+            }
             __half2 k_one[KU], v_one[4];             // powers of two that take the scales to [1, 2) at most
 #pragma unroll
             for (uint32_t u = 0; u < KU; ++u) k_one[u] = to_one(k_exp);
@@ -564,8 +577,8 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
                 for (uint32_t k = 0; k < 8; ++k) vs[k] = finite_only(vs[k]);
             }
             // K
-            if (i >= 2) ok = __all_sync(0xFFFFFFFFu, ok && bar_wait(&c.k_free[buf], (round - 1u) & 1u, &c.abort));
-            if (!ok) continue;
+            if (i >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.k_free[buf], (round - 1u) & 1u, &c.abort));
+            if (!ok) break;
             uint8_t* kb = sm + S::K_AT + buf * S::KV_TERM * S::TERMS;
 #pragma unroll
             for (uint32_t u = 0; u < KU; ++u)
@@ -586,7 +599,7 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
             if (i + 1u < tiles) load_k(i + 1u);
             // V
             if (i >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.v_free[buf], (round - 1u) & 1u, &c.abort));
-            if (!ok) continue;
+            if (!ok) break;
             uint32_t cw[8], cs[8];
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k) {
@@ -625,7 +638,8 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
         float m = -INFINITY, l = 0.0f;               // reference of the weights' exponents; running sum, both in units of 2^6 p
         float off = MASK ? -INFINITY : 0.0f;         // the mask's maximum so far: scores and m are relative to it
         const __half* mrow = MASK && row < rows ? a.mask + (size_t)tok * a.mask_stride : nullptr;
-        uint32_t v_exp = 1, lost = 0;                // lost: blocks of V in which the row sees a scale that is no number
+        float v_ref = -14.0f + Scaled<PRECISE>::UNDO;    // log2 of what outputs lack: the largest v_log so far
+        uint32_t lost = 0;                           // blocks of V in which the row sees a scale that is no number
         bool ok = true;
         // the cells that all rows of the warp see; rows behind the group's last lose nothing
         const int32_t all_lo = __reduce_max_sync(0xFFFFFFFFu, row < rows ? lo : 0), all_hi = __reduce_min_sync(0xFFFFFFFFu, row < rows ? hi : 0x7FFFFFFF);
@@ -636,30 +650,49 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
             ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.s_full[rg][sb], (i / S::NS) & 1u, &c.abort));
             if (!ok) break;
             fence_after();
-            const TileInfo info = c.info[i & 3u];
-            const bool open = c0 >= all_lo && c0 + (int32_t)kTile <= all_hi;
-            float f = qs * info.k_unscale;
-            if (info.far) {                          // seldom: scores with the cells' own powers of two, put back for what follows
+            constexpr uint32_t GC = kTile / S::DW;   // cells of a dequant warp
+            const TileInfo& info = c.info[i & 3u];
+            float f[S::DW], v_log[S::DW];            // factors of scores
+            uint32_t flags = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < S::DW; w += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(info.k_unscale + w), y = *reinterpret_cast<const float4*>(info.v_log + w);
+                f[w] = qs * x.x; f[w + 1] = qs * x.y; f[w + 2] = qs * x.z; f[w + 3] = qs * x.w;
+                v_log[w] = y.x; v_log[w + 1] = y.y; v_log[w + 2] = y.z; v_log[w + 3] = y.w;
+                flags |= *reinterpret_cast<const uint32_t*>(info.flags + w);
+            }
+            const bool open = c0 >= all_lo && c0 + (int32_t)kTile <= all_hi, far = flags & kFar * 0x01010101u, bad = flags & kBad * 0x01010101u;
+            if (far) {                               // seldom: scores with the cells' own powers of two, put back for what follows
 #pragma unroll 1
                 for (uint32_t k = 0; k < kTile; k += 8) {
+                    const float fk = qs * info.k_unscale[k / GC];
+                    const bool own = info.flags[k / GC] & kFar;
                     uint32_t x[8];
                     tmem_ld8(at + k, x);
                     tmem_wait_ld8(x);
 #pragma unroll
-                    for (uint32_t j = 0; j < 8; ++j) x[j] = __float_as_uint(fmaf(__uint_as_float(x[j]) * f, c.cell_k[i & 3u][k + j], c.cell_v[i & 3u][k + j]));
+                    for (uint32_t j = 0; j < 8; ++j) {
+                        const float z = __uint_as_float(x[j]) * fk;
+                        x[j] = __float_as_uint(own ? fmaf(z, c.cell_k[i & 3u][k + j], c.cell_v[i & 3u][k + j]) : z);
+                    }
                     tmem_st8(at + k, x);
                 }
                 tmem_wait_st();
-                f = 1.0f;
             }
             uint32_t raw[64];
             tmem_ld32(at, raw);
             tmem_ld32(at + 32u, raw + 32);
             tmem_wait_ld64(raw);
-#pragma unroll
-            for (int j = 0; j < 64; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * f);
             // bit j of the words: the row's range holds cell c0 + j; a thread without a row sees none (and has no mask)
             uint32_t w0 = row < rows ? ~0u : 0u, w1 = w0;
+            if (MASK || !open || far) {              // then these are the scores, elsewhere their factors wait for the exponent
+                if (!far) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * f[j / GC]);
+                }
+#pragma unroll
+                for (uint32_t w = 0; w < S::DW; ++w) f[w] = 1.0f;
+            }
             if (!open) {
                 const int32_t from = min(max(lo - c0, 0), 64), to = min(max(hi - c0, from), 64);
                 const unsigned long long bits = (to >= 64 ? ~0ull : (1ull << to) - 1ull) & ~(from >= 64 ? ~0ull : (1ull << from) - 1ull);
@@ -694,11 +727,16 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
                     }
                 }
             }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float most = -INFINITY, v_now = v_ref;
 #pragma unroll
-            for (int j = 0; j < 64; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(raw[j]));
-            const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            const bool raise = __any_sync(0xFFFFFFFFu, most > m + 8.0f || info.v_exp != v_exp);
+            for (uint32_t w = 0; w < S::DW; ++w) {
+                float top = max3(__uint_as_float(raw[GC * w]), __uint_as_float(raw[GC * w + 1]), __uint_as_float(raw[GC * w + 2]));
+#pragma unroll
+                for (uint32_t j = 3; j + 1 < GC; j += 2) top = max3(top, __uint_as_float(raw[GC * w + j]), __uint_as_float(raw[GC * w + j + 1]));
+                most = fmaxf(most, fmaxf(top, __uint_as_float(raw[GC * w + GC - 1])) * f[w]);
+                v_now = fmaxf(v_now, v_log[w]);
+            }
+            const bool raise = __any_sync(0xFFFFFFFFu, most > m + 8.0f || v_now != v_ref);
             const bool flush = TOTAL && i > 0 && i % S::FLUSH == 0u;
             if (raise || flush) {
                 float both = 1.0f;
@@ -706,8 +744,8 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
                     const float now = fmaxf(m, most), base = now == -INFINITY ? 0.0f : now, down = ex2(m - base);
                     l *= down;
                     m = now;
-                    both = down * pow2((int)v_exp - (int)info.v_exp);
-                    v_exp = info.v_exp;
+                    both = down * pow2((int)(v_ref - v_now));
+                    v_ref = v_now;
                 }
                 if (i > 0) {
                     // the products so far have to be there
@@ -719,48 +757,61 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
                 }
             }
             const float up = m == -INFINITY ? 0.0f : 6.0f - m;
-            float sum[4] = {}, far_sum = 0.0f;
-            if (MASK && info.far) {                  // the sum takes the weights without V's powers of two
+            float far_sum = 0.0f;
+            if (MASK && far) {                       // the sum takes the weights without V's powers of two
 #pragma unroll
-                for (int j = 0; j < 64; ++j) far_sum += ex2(__uint_as_float(raw[j]) - c.cell_v[i & 3u][j] + up);
-            } else if (info.far) {
+                for (int j = 0; j < 64; ++j)
+                    far_sum += ex2(__uint_as_float(raw[j]) - (info.flags[j / GC] & kFar ? c.cell_v[i & 3u][j] : 0.0f) + up);
+            } else if (far) {
 #pragma unroll 1
                 for (uint32_t k = 0; k < kTile; k += 8) {
+                    const bool own = info.flags[k / GC] & kFar;
                     uint32_t x[8];
                     tmem_ld8(at + k, x);
                     tmem_wait_ld8(x);
 #pragma unroll
                     for (uint32_t j = 0; j < 8; ++j) {
                         const int32_t cell = c0 + (int32_t)(k + j);
-                        if (cell >= lo && cell < hi) far_sum += ex2(__uint_as_float(x[j]) - c.cell_v[i & 3u][k + j] + up);
+                        if (cell >= lo && cell < hi) far_sum += ex2(__uint_as_float(x[j]) - (own ? c.cell_v[i & 3u][k + j] : 0.0f) + up);
                     }
                     __syncwarp();
                 }
             }
+            // The weights times what their cells' V lacks beside v_ref. Sums are of these, each dequant warp's cells for
+            // themselves, and then made good.
+            float near_sum = 0.0f;
+            float2 sum[2];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {            // sixteen cells at a time: eight words of each term
                 uint32_t hw[8], lw[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float p0 = ex2(__uint_as_float(raw[16 * k + 2 * j]) + up), p1 = ex2(__uint_as_float(raw[16 * k + 2 * j + 1]) + up);
-                    sum[j & 1] += p0;
-                    sum[2 + (j & 1)] += p1;
-                    const __half2 h = __floats2half2_rn(p0, p1);
+                    const uint32_t e = 16 * k + 2 * j, w = e / GC;
+                    const float uw = up + (v_log[w] - v_ref);
+                    const float2 z = fma2(make_float2(__uint_as_float(raw[e]), __uint_as_float(raw[e + 1])), make_float2(f[w], f[w]), make_float2(uw, uw));
+                    const float2 p = make_float2(ex2(z.x), ex2(z.y));
+                    if (e % GC < 4) sum[e / 2 & 1u] = p;
+                    else sum[e / 2 & 1u] = add2(sum[e / 2 & 1u], p);
+                    if (e % GC == GC - 2u) {
+                        const float2 both = add2(sum[0], sum[1]);
+                        near_sum = fmaf(both.x + both.y, info.v_inv[w], near_sum);
+                    }
+                    const __half2 h = __floats2half2_rn(p.x, p.y);
                     hw[j] = as_u32(h);
                     if (PRECISE) {
                         const float2 back = __half22float2(h);
-                        lw[j] = as_u32(__floats2half2_rn(p0 - back.x, p1 - back.y));
+                        lw[j] = as_u32(__floats2half2_rn(p.x - back.x, p.y - back.y));
                     }
                 }
                 tmem_st8(at + 8u * k, hw);
                 if (PRECISE) tmem_st8(at + kTile / 2u + 8u * k, lw);
             }
-            l += info.far ? far_sum : (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l += far ? far_sum : near_sum * pow2((int)v_ref);
             tmem_wait_st();
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(&c.p_full[rg][sb]);
-            if (info.bad) {                          // seldom: which of the blocks left out of V this row would have met
+            if (bad) {                          // seldom: which of the blocks left out of V this row would have met
 #pragma unroll 1
                 for (uint32_t j = 0; j < kTile; ++j) {
                     if (c0 + (int32_t)j < lo || c0 + (int32_t)j >= hi || (MASK && __half2float(mrow[c0 + (int32_t)j]) == -INFINITY)) continue;
@@ -776,7 +827,7 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
         if (ok) {
             fence_after();
             // l and O are in units of 2^6 p: a split's share names 2^-6 of its reference
-            const float unit = pow2((int)v_exp - 15 + Scaled<PRECISE>::UNDO), f = a.splits > 1u ? unit : l == 0.0f ? 0.0f : unit / l;
+            const float unit = pow2((int)v_ref), f = a.splits > 1u ? unit : l == 0.0f ? 0.0f : unit / l;
             T* out = static_cast<T*>(a.out) + (size_t)tok * a.out_stride + (size_t)head * D;
             const size_t part = ((((size_t)grp * a.row_tiles + rt) * a.n_head_kv + hk) * a.splits + split) * (kRows * RG) + tid;
             if (a.splits > 1u && row < rows) *reinterpret_cast<float4*>(a.part_ml + part * 4u) = make_float4(off, m - 6.0f, l, 0.0f);
