@@ -1,5 +1,6 @@
 // tsrc_fa4.cu -- attention over the q4_0 KV cache (tsrc_flash_attn_q4). Cache layout: tsrc_kv4.cuh.
 #include <cmath>
+#include <algorithm>
 #include <cstdio>
 #include <type_traits>
 
@@ -10,7 +11,7 @@ namespace tsrc {
 namespace {
 
 constexpr uint32_t kDecWarps = 4, kDecTile = 32, kDecStages = 3;
-constexpr uint32_t kSms = 148, kDecCtas = 4 * kSms;      // the CTAs that a B200 holds at once, four to an SM
+constexpr uint32_t kSms = 148;
 constexpr uint32_t kMaxCluster = 16;
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -740,28 +741,48 @@ struct Fa4Plan {
 };
 
 constexpr uint32_t kMaxT = 1u << 20;
-Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint32_t n_head, uint32_t n_kv, uint32_t group, uint32_t max_len) {
+Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint32_t n_head, uint32_t n_kv, uint32_t group, uint32_t max_len, bool mask) {
     Fa4Plan p{};
     p.group = group ? group : T;
     const uint32_t rows = p.group * (n_head / n_head_kv);
     p.splits = 1;
     const uint32_t len = max_len && max_len < n_kv ? max_len : n_kv;
+
+    // The kernel for few rows. Splits in powers of two up to a cluster's CTAs, each warp keeping a tile at least: until the
+    // GPU's places for CTAs (four an SM; three with 16 rows, whose registers are more) are taken, since a CTA costs about
+    // three tiles' time beside its tiles; and where a warp keeps eight tiles even so, once more, which evens out what the
+    // last CTAs leave idle (64 ragged sequences, 512 units: 80 us with 2, 89 with 1, 85 with 4). Clusters of sixteen only
+    // where two CTAs an SM are all there are: more of them do not fit side by side (8 tokens, 32 / 8 heads, 4113 cells in
+    // f16: 28 us with 16, 18.5 with 8). Where even these leave most SMs empty and the cells are many, more splits and a
+    // merge kernel.
     p.mode = type != TSRC_TYPE_BF16 ? kRows8Split : rows <= 8u ? kRows8 : kRows16;
-    const uint32_t R = p.mode == kRows16 ? 16u : 8u;
+    const uint32_t R = p.mode == kRows16 ? 16u : 8u, all = (R == 16u ? 3u : 4u) * kSms;
     p.row_tiles = (rows + R - 1u) / R;
     p.units = (T / p.group) * n_head_kv * p.row_tiles;
+    const uint32_t teams = D <= 128u ? kDecWarps : kDecWarps * 128u / D;
+    const uint32_t tiles = len / kDecTile + 1u, most = tiles / teams;
+    while (p.splits < (p.units * kMaxCluster <= 2u * kSms ? kMaxCluster : 8u) && p.splits * 2u <= most &&
+           (p.units * p.splits * 2u <= all || (p.units * p.splits < all && tiles >= 16u * teams * p.splits)))
+        p.splits *= 2u;
+    const bool merge = p.units * kMaxCluster < kSms && most >= 8u * kMaxCluster;
+    const uint32_t parts = merge ? std::min(2u * kSms / p.units, most / 2u) : p.splits;      // a warp keeps two tiles
     if (D <= 128u) {
-        // The kernel for many rows where it is the faster one, by what both measured (ns): a tile of 64 cells keeps one
-        // of its CTAs 1.1 (bf16) to 1.6 us (f32), and its CTAs are split over the cells while SMs have none and eight
-        // tiles are left to each; the other kernel's 592 places take 0.93 us for 32 cells of 8 rows (1.35 for 16 rows; D = 64:
-        // two thirds). 32 rows of 8 KV heads over 8192 cells in f32: 38 us there, 221 here unsplit; 2048 rows: 797 and 231.
-        const uint64_t units = (uint64_t)(T / p.group) * n_head_kv * ((rows + kFa4TcRows - 1u) / kFa4TcRows), tiles = len / 64u + 1u;
-        const uint32_t each = type == TSRC_TYPE_BF16 ? 1150u : type == TSRC_TYPE_F16 ? 1450u : 1650u;
-        const uint64_t places = type == TSRC_TYPE_BF16 || D == 64u ? 2u * kSms : kSms;
-        uint64_t splits = kSms / units < tiles / 8u ? kSms / units : tiles / 8u;
-        if (splits < 1u) splits = 1;
-        const uint64_t tc = 9000u + (units * splits + places - 1u) / places * ((tiles + splits - 1u) / splits) * each + (splits > 1u ? 6000u : 0u);
-        const uint64_t dec = 11000u + (uint64_t)p.units * (len / kDecTile + 1u) * (R == 16u ? 1350u : 930u) / (D == 64u ? 900u : 592u);
+        // The kernel for many rows where it is the faster one, by what both measured (ns). Its CTAs take 1.25 (bf16) to 1.75
+        // us (f32) for a tile of 64 cells, 1.4 to 1.8 more under a mask, and are split over the cells as far as there are
+        // SMs; a split costs the merge about a sixth of a tile, so that the tiles left to each and the splits are balanced.
+        // The other kernel's warps take 2 us for 32 cells of 8 rows (3 for 16) up to two CTAs an SM, then in proportion
+        // to those. f16, 32 / 8 heads, 4113 cells: 8 tokens 19.6 us here and 18.5 there, 13 tokens 19.8 and 23.2, 64 tokens
+        // 28.6 and 72; 16384 cells: 13 tokens 35 and 65.
+        const uint64_t units = (uint64_t)(T / p.group) * n_head_kv * ((rows + kFa4TcRows - 1u) / kFa4TcRows), blocks = len / 64u + 1u;
+        const uint64_t each = (type == TSRC_TYPE_BF16 ? 1250u : type == TSRC_TYPE_F16 ? 1450u : 1750u) + (!mask ? 0u : type == TSRC_TYPE_BF16 ? 1400u : 1800u);
+        const uint64_t places = !mask && (type == TSRC_TYPE_BF16 || D == 64u) ? 2u * kSms : kSms;
+        uint64_t splits = 1;
+        while ((splits + 1u) * units <= kSms && (splits + 1u) * (splits + 1u) <= 6u * blocks && 2u * (splits + 1u) <= blocks) ++splits;
+        const uint64_t tc = (units * splits + places - 1u) / places * ((blocks + splits - 1u) / splits) * each +
+                            (splits > 1u ? 13000u + (uint64_t)T * n_head * splits * D / 750u : 8200u);
+        const uint64_t ctas = (uint64_t)p.units * parts, share = (uint64_t)teams * ctas / p.units;
+        const uint64_t busy = ctas * (R == 16u ? 1700u : 1050u) / kSms, alone = R == 16u ? 3000u : 2000u;
+        const uint64_t dec = 8000u + (tiles + share - 1u) / share * (busy > alone ? busy : alone) / (D == 64u ? 2u : 1u) + (merge ? 3000u : 0u);
         if (tc < dec) {
             const uint64_t wide = (uint64_t)(T / p.group) * n_head_kv * ((rows + 2u * kFa4TcRows - 1u) / (2u * kFa4TcRows));
             // bf16: 256 rows a CTA where 128 give at least four CTAs to three SMs, and 256, of which an SM holds one, take no
@@ -771,7 +792,7 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
             p.mode = kRows128;
             p.tile_rows = two ? 2u * kFa4TcRows : kFa4TcRows;
             p.row_tiles = (rows + p.tile_rows - 1u) / p.tile_rows;
-            p.units = (uint32_t)(p.tile_rows > kFa4TcRows ? wide : units);
+            p.units = (uint32_t)(two ? wide : units);
             p.splits = (uint32_t)splits;
             if (p.splits > 1u) {
                 p.o_bytes = (size_t)p.units * p.splits * kFa4TcRows * D * 4u;
@@ -780,19 +801,8 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
             return p;
         }
     }
-    const uint32_t teams = D <= 128u ? kDecWarps : kDecWarps * 128u / D;
-    // Splits in powers of two up to a cluster's CTAs, each warp keeping a tile at least: until the GPU's places for
-    // CTAs (four an SM) are taken, since a CTA costs about three tiles' time beside its tiles (13 drafted tokens over
-    // 4113 cells, 56 units: 25.5 us with 8 splits, 38 with 16, 33 with 4); and where a warp keeps eight tiles even so,
-    // once more, which evens out what the last CTAs leave idle (64 ragged sequences, 512 units: 80 us with 2, 89
-    // with 1, 85 with 4). Where even clusters of sixteen leave most SMs empty and the cells are many, more splits and a
-    // merge kernel.
-    const uint32_t tiles = len / kDecTile + 1u, most = tiles / teams;
-    while (p.splits < kMaxCluster && p.splits * 2u <= most &&
-           (p.units * p.splits * 2u <= kDecCtas || (p.units * p.splits < kDecCtas && tiles >= 16u * teams * p.splits)))
-        p.splits *= 2u;
-    if (p.units * kMaxCluster < kSms && most >= 8u * kMaxCluster) {
-        p.splits = 2u * kSms / p.units;
+    if (merge) {
+        p.splits = parts;
         p.o_bytes = (size_t)p.units * p.splits * R * D * 4u;
         p.ml_bytes = (size_t)p.units * p.splits * R * 16u;
     }
@@ -889,8 +899,9 @@ const char* tsrc_flash_attn_q4_unsupported(uint32_t type, uint32_t n_head_kv, ui
 size_t tsrc_flash_attn_q4_workspace(uint32_t type, uint32_t n_head_kv, uint32_t head_dim, uint32_t T, uint32_t n_head,
                                     uint32_t n_kv, uint32_t group, uint32_t max_len) {
     if (T == 0 || T > kMaxT || (group && T % group) || tsrc_flash_attn_q4_unsupported(type, n_head_kv, head_dim, n_head)) return 0;
-    const Fa4Plan p = fa4_plan(type, n_head_kv, head_dim, T, n_head, n_kv, group, max_len);
-    return p.o_bytes + p.ml_bytes;
+    const Fa4Plan p = fa4_plan(type, n_head_kv, head_dim, T, n_head, n_kv, group, max_len, false);
+    const Fa4Plan m = fa4_plan(type, n_head_kv, head_dim, T, n_head, n_kv, group, max_len, true);
+    return std::max(p.o_bytes + p.ml_bytes, m.o_bytes + m.ml_bytes);        // a call may have a mask
 }
 
 int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const void* q, uint32_t q_stride, uint32_t T, uint32_t n_head,
@@ -920,7 +931,7 @@ int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const v
     if (T == 0) return TSRC_OK;
     DeviceScope scope(ctx);
     if (scope.rc) return scope.rc;
-    const Fa4Plan p = fa4_plan(type, kv->n_head_kv, kv->D, T, n_head, n_kv, group, max_len);
+    const Fa4Plan p = fa4_plan(type, kv->n_head_kv, kv->D, T, n_head, n_kv, group, max_len, mask != nullptr);
     Fa4Args a{};
     a.q = q;
     a.out = out;

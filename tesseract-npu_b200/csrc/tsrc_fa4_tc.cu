@@ -35,7 +35,7 @@ __device__ unsigned int g_fa4_error;                 // kKv4ErrWait once a wait 
 constexpr uint32_t kTile = 64, kRows = 128;
 constexpr long long kWaitCycles = 1ll << 31;         // a wait gives up after ~1 s of SM clock
 
-template <class T, int D, uint32_t RG> struct TcShape {                             // RG: lots of 128 rows
+template <class T, int D, bool MASK, uint32_t RG> struct TcShape {                        // RG: lots of 128 rows
     static constexpr bool PRECISE = !std::is_same_v<T, __nv_bfloat16>;              // two terms of K, V and the weights
     static constexpr bool TOTAL = std::is_same_v<T, float>;                         // two of q (fp16 is one), outputs in total
     static constexpr uint32_t NB = D / 32, TERMS = PRECISE ? 2 : 1;
@@ -45,7 +45,7 @@ template <class T, int D, uint32_t RG> struct TcShape {                         
     // two CTAs an SM at most, or one that takes all of tensor memory. Two lots of rows take four dequant warps: with eight
     // the registers a thread may have, 96, do not hold a row's scores (2048 tokens: 71.3 us, 68.6 with four).
     static constexpr uint32_t WANT = CTL_AT + 4096;
-    static constexpr uint32_t MIN_CTAS = RG == 1 && 2 * (WANT + 1024) <= 227 * 1024 ? 2 : 1;
+    static constexpr uint32_t MIN_CTAS = RG == 1 && !MASK && 2 * (WANT + 1024) <= 227 * 1024 ? 2 : 1;
     static constexpr uint32_t LEAST = MIN_CTAS == 2 ? 100 * 1024 : 116 * 1024, BYTES = WANT < LEAST ? LEAST : WANT;
     static constexpr uint32_t DW = MIN_CTAS == 1 && RG == 1 ? 8 : 4, SW = 4 * RG;              // dequant, softmax warps
     static constexpr uint32_t WARPS = SW + DW + 1, THREADS = 32 * WARPS;
@@ -228,11 +228,12 @@ template <> struct Scaled<false> {
     }
 };
 
-// Eight cells of a row's mask from `cell` on, -inf where `seen` lacks the cell's bit (the mask there may hold anything,
-// or not be there).
-__device__ __forceinline__ uint4 mask_of(const Fa4Args& a, const __half* row, int32_t cell, uint32_t seen) {
+// Eight cells of a row's mask from `cell` on, -inf where `seen` lacks the cell's bit (the mask there may hold anything).
+// wide: the row holds all of the tile in aligned memory, and the load stands outside any branch, so that a tile's eight are
+// under way together; every: no bit lacks.
+__device__ __forceinline__ uint4 mask_of(const __half* row, int32_t cell, uint32_t seen, bool wide, bool every) {
     uint32_t w[4];
-    if (a.mask_wide && seen && cell + 8 <= (int32_t)a.n_kv) {
+    if (wide) {
         const uint4 h = *reinterpret_cast<const uint4*>(row + cell);
         w[0] = h.x; w[1] = h.y; w[2] = h.z; w[3] = h.w;
     } else {
@@ -242,10 +243,12 @@ __device__ __forceinline__ uint4 mask_of(const Fa4Args& a, const __half* row, in
             if (seen >> (2 * j) & 2u) w[j] |= (uint32_t)__half_as_ushort(row[cell + 2 * (int32_t)j + 1]) << 16;
         }
     }
+    if (!every) {
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-        const uint32_t keep = (seen >> (2 * j) & 1u ? 0x0000FFFFu : 0u) | (seen >> (2 * j) & 2u ? 0xFFFF0000u : 0u);
-        w[j] = (w[j] & keep) | (0xFC00FC00u & ~keep);
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t keep = (seen >> (2 * j) & 1u ? 0x0000FFFFu : 0u) | (seen >> (2 * j) & 2u ? 0xFFFF0000u : 0u);
+            w[j] = (w[j] & keep) | (0xFC00FC00u & ~keep);
+        }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -297,8 +300,8 @@ __device__ __forceinline__ void settle(uint32_t o_at, uint32_t sum_at, float f, 
 }
 
 template <class T, int D, bool MASK, uint32_t RG>
-__global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>::MIN_CTAS) fa4_tc_kernel(Fa4Args a) {
-    using S = TcShape<T, D, RG>;
+__global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D, MASK, RG>::MIN_CTAS) fa4_tc_kernel(Fa4Args a) {
+    using S = TcShape<T, D, MASK, RG>;
     constexpr bool PRECISE = S::PRECISE, TOTAL = S::TOTAL;
     constexpr uint32_t NB = S::NB;
     extern __shared__ __align__(1024) uint8_t sm[];
@@ -637,7 +640,8 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
         const float qs = c.q_unscale[tid];           // this row's scale, for scores in log2
         float m = -INFINITY, l = 0.0f;               // reference of the weights' exponents; running sum, both in units of 2^6 p
         float off = MASK ? -INFINITY : 0.0f;         // the mask's maximum so far: scores and m are relative to it
-        const __half* mrow = MASK && row < rows ? a.mask + (size_t)tok * a.mask_stride : nullptr;
+        // a thread without a row may load the last token's, and sees nothing of it
+        const __half* mrow = MASK ? a.mask + (size_t)min(tok, a.T - 1u) * a.mask_stride : nullptr;
         float v_ref = -14.0f + Scaled<PRECISE>::UNDO;    // log2 of what outputs lack: the largest v_log so far
         uint32_t lost = 0;                           // blocks of V in which the row sees a scale that is no number
         bool ok = true;
@@ -647,6 +651,8 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
         for (uint32_t i = 0; ok && i < tiles; ++i) {
             const uint32_t buf = i & 1u, sb = i % S::NS, at = mine + (rg * S::NS + sb) * kTile;
             const int32_t c0 = (int32_t)((tile0 + i) * kTile);
+            if (MASK && c0 + 2 * (int32_t)kTile <= (int32_t)a.n_kv)      // the next tile's mask, a line or two of this row
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(mrow + c0 + (int32_t)kTile));
             ok = __all_sync(0xFFFFFFFFu, bar_wait(&c.s_full[rg][sb], (i / S::NS) & 1u, &c.abort));
             if (!ok) break;
             fence_after();
@@ -706,26 +712,32 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
             }
             if constexpr (MASK) {
                 // the mask's running maximum is taken out first: a row of the type's lowest value keeps its scores' digits
-                __half2 most2 = __half2half2(__ushort_as_half((unsigned short)0xFC00u));
+                const bool every = __all_sync(0xFFFFFFFFu, (w0 & w1) == ~0u);
+                auto pass = [&](auto whole) {        // two forms, so that no branch stands before the loads
+                    constexpr bool WIDE = decltype(whole)::value;
+                    __half2 most2 = __half2half2(__ushort_as_half((unsigned short)0xFC00u));
 #pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                    const uint4 h = mask_of(a, mrow, c0 + 8 * (int32_t)k, (k < 4 ? w0 >> 8u * k : w1 >> (8u * k - 32u)) & 0xFFu);
-                    most2 = __hmax2(most2, __hmax2(__hmax2(as_h2(h.x), as_h2(h.y)), __hmax2(as_h2(h.z), as_h2(h.w))));
-                }
-                const float now = fmaxf(off, fmaxf(__low2float(most2), __high2float(most2))), base = now == -INFINITY ? 0.0f : now;
-                if (off != -INFINITY && off != now) m += (off - base) * 1.4426950408889634f;
-                off = now;
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                    const uint4 h = mask_of(a, mrow, c0 + 8 * (int32_t)k, (k < 4 ? w0 >> 8u * k : w1 >> (8u * k - 32u)) & 0xFFu);
-                    const uint32_t w[4] = {h.x, h.y, h.z, h.w};
-#pragma unroll
-                    for (uint32_t j = 0; j < 8; ++j) {
-                        const float x = __half2float(__ushort_as_half((unsigned short)(w[j / 2] >> (j & 1u ? 16 : 0))));
-                        const float z = fmaf(x - base, 1.4426950408889634f, __uint_as_float(raw[8 * k + j]));
-                        raw[8 * k + j] = __float_as_uint(x == -INFINITY ? -INFINITY : z);
+                    for (uint32_t k = 0; k < 8; ++k) {
+                        const uint4 h = mask_of(mrow, c0 + 8 * (int32_t)k, (k < 4 ? w0 >> 8u * k : w1 >> (8u * k - 32u)) & 0xFFu, WIDE, WIDE && every);
+                        most2 = __hmax2(most2, __hmax2(__hmax2(as_h2(h.x), as_h2(h.y)), __hmax2(as_h2(h.z), as_h2(h.w))));
                     }
-                }
+                    const float now = fmaxf(off, fmaxf(__low2float(most2), __high2float(most2))), base = now == -INFINITY ? 0.0f : now;
+                    if (off != -INFINITY && off != now) m += (off - base) * 1.4426950408889634f;
+                    off = now;
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; ++k) {
+                        const uint4 h = mask_of(mrow, c0 + 8 * (int32_t)k, (k < 4 ? w0 >> 8u * k : w1 >> (8u * k - 32u)) & 0xFFu, WIDE, WIDE && every);
+                        const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+                        for (uint32_t j = 0; j < 8; ++j) {
+                            const float x = __half2float(__ushort_as_half((unsigned short)(w[j / 2] >> (j & 1u ? 16 : 0))));
+                            const float z = fmaf(x - base, 1.4426950408889634f, __uint_as_float(raw[8 * k + j]));
+                            raw[8 * k + j] = __float_as_uint(x == -INFINITY ? -INFINITY : z);
+                        }
+                    }
+                };
+                if (a.mask_wide && c0 + (int32_t)kTile <= (int32_t)a.n_kv) pass(std::true_type{});
+                else pass(std::false_type{});
             }
             float most = -INFINITY, v_now = v_ref;
 #pragma unroll
@@ -874,7 +886,7 @@ __global__ void __launch_bounds__(TcShape<T, D, RG>::THREADS, TcShape<T, D, RG>:
 
 template <class T, int D, bool MASK, uint32_t RG>
 cudaError_t launch_m(const Fa4Args& a, uint32_t units, cudaStream_t st) {
-    using S = TcShape<T, D, RG>;
+    using S = TcShape<T, D, MASK, RG>;
     static bool done[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
