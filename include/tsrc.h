@@ -317,8 +317,9 @@ TSRC_API int tsrc_kv4_reorder(tsrc_ctx * ctx, tsrc_kv4 * kv, const int32_t * par
 //   out[t][h][:] = sum_c p_c V[c] / sum_c p_c,   p_c = exp(s_c - max_c s_c),   s_c = scale * q[t][h] . K[c] + mask[t][c]
 // with K and V the values the codes stand for, products and sums in f32 or better, and one rounding to `type` (of
 // q and out) at the end. Token t sees cells [ranges[2t], ranges[2t + 1]) (device int32, cut to [0, n_kv); NULL: all
-// n_kv) whose mask (device f16 [T][mask_stride], cells from 0; NULL: none) is not -inf; what other cells hold, NaN
-// or infinities included, has no effect. A token that sees no cell gets zeros. A NaN score makes its row NaN.
+// n_kv) whose mask (device f16 [T][mask_stride], mask_stride >= n_kv or 0 = n_kv, cells from 0; NULL: none) is not
+// -inf; what other cells hold, NaN or infinities included, has no effect. A token that sees no cell gets zeros. A NaN score makes its row NaN; a
+// scale of V that is infinite or no number leaves no finite value in its 32 outputs for the tokens that see its cell.
 // So a decode step of many sequences, a causal or windowed prompt and a drafted tree are one call each; the ranges
 // may be rewritten on the device between replays of a captured call.
 // group (0 = T): consecutive tokens that read about the same cells (a sequence's); T must be a multiple of it.
@@ -330,7 +331,8 @@ TSRC_API int tsrc_flash_attn_q4(tsrc_ctx * ctx, const tsrc_kv4 * kv, uint32_t ty
                                 uint32_t T, uint32_t n_head, uint32_t n_kv, const int32_t * ranges, uint32_t group,
                                 uint32_t max_len, const uint16_t * mask, uint32_t mask_stride, float scale, void * out,
                                 uint32_t out_stride, void * ws, size_t ws_bytes, void * stream);
-// Workspace bytes of such a call (host only, no device needed; the arguments of the call).
+// Workspace bytes of such a call, with or without a mask (host only, no device needed; the arguments of the call). 0 for
+// a call that is refused.
 TSRC_API size_t tsrc_flash_attn_q4_workspace(uint32_t type, uint32_t n_head_kv, uint32_t head_dim, uint32_t T, uint32_t n_head,
                                              uint32_t n_kv, uint32_t group, uint32_t max_len);
 // Why such a call could not run (NULL if it can); host only.

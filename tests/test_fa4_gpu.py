@@ -241,11 +241,11 @@ def test_many_rows_masks_windows_and_hidden_cells(dev, dtype, T, n, H, Hk, D):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
-@pytest.mark.parametrize("D", [64, 128])
-def test_many_rows_magnitudes(dev, dtype, D):
+@pytest.mark.parametrize("T,D", [(300, 64), (300, 128), (1300, 64), (1300, 128)])
+def test_many_rows_magnitudes(dev, dtype, T, D):
     """Scales from tiny to far above the common ones, differing from cell to cell, in tiles of the kernel for many rows."""
     import torch
-    T, n, H, Hk = 300, 300, 32, 8
+    n, H, Hk = 300, 32, 8
     for qs, ks, vs, scale in ((1e3, 1e-3, 1e-4, 0.09), (1e-3, 3e2, 2e3, 0.05), (3e2, 1.0, 1.0, 0.0003), (1.0, 1.0, 6e-6, 0.0), (1.0, 20.0, 60.0, -0.004)):
         rng, q, kb, vb = _inputs(int(10 * ks) + D, T, H, Hk, D, n, "float32")
         q = (q * qs).to(getattr(torch, dtype))
@@ -275,6 +275,26 @@ def test_what_is_hidden_has_no_effect(dev, dtype, T):
     mask[:, 160:] = np.inf
     _check(dev, q, kb, vb, 2, dtype, ranges, mask=mask)
     _check(dev, q, kb, vb, 2, dtype, [[10, 40]] * T)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("T,D", [(3, 128), (3, 256), (300, 64), (1300, 128)])
+def test_visible_scale_of_v_that_is_not_finite(dev, dtype, T, D):
+    """Its block is not finite for the tokens that see the cell, whatever weight they give it; nothing else changes."""
+    n, H, Hk = 200, 32, 8
+    _, q, kb, vb = _inputs(T + D, T, H, Hk, D, n, dtype)
+    ranges = [[0, 200] if t % 2 else [0, 100] if t % 4 else [131, 200] for t in range(T)]
+    clean = _run(dev, q, kb, vb, Hk, 0.1, ranges)
+    b = vb.reshape(n, Hk, D // 32, 18)
+    b[130, 3, 1, :2] = np.array([0x00, 0x7C], np.uint8)
+    b[120, 5, 0, :2] = np.array([0x01, 0x7E], np.uint8)
+    got = _run(dev, q, kb, vb, Hk, 0.1, ranges)
+    lost = np.zeros(got.shape, bool)
+    lost[1::2, 12:16, 32:64] = lost[1::2, 20:24, :32] = True
+    assert not np.isfinite(got[lost]).any()
+    assert np.isfinite(got[~lost]).all()
+    others = [h for h in range(H) if h // 4 not in (3, 5)]
+    assert (got[:, others] == clean[:, others]).all()
 
 
 def test_visible_nan_makes_its_row_nan(dev):
