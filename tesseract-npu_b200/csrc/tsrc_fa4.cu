@@ -1,6 +1,6 @@
 // tsrc_fa4.cu -- attention over the q4_0 KV cache (tsrc_flash_attn_q4). Cache layout: tsrc_kv4.cuh.
-#include <cmath>
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <type_traits>
 
@@ -761,10 +761,10 @@ Fa4Plan fa4_plan(uint32_t type, uint32_t n_head_kv, uint32_t D, uint32_t T, uint
     p.units = (T / p.group) * n_head_kv * p.row_tiles;
     const uint32_t teams = D <= 128u ? kDecWarps : kDecWarps * 128u / D;
     const uint32_t tiles = len / kDecTile + 1u, most = tiles / teams;
-    while (p.splits < (p.units * kMaxCluster <= 2u * kSms ? kMaxCluster : 8u) && p.splits * 2u <= most &&
+    while (p.splits < (p.units <= 2u * kSms / kMaxCluster ? kMaxCluster : 8u) && p.splits * 2u <= most && p.units < all &&
            (p.units * p.splits * 2u <= all || (p.units * p.splits < all && tiles >= 16u * teams * p.splits)))
         p.splits *= 2u;
-    const bool merge = p.units * kMaxCluster < kSms && most >= 8u * kMaxCluster;
+    const bool merge = p.units <= (kSms - 1u) / kMaxCluster && most >= 8u * kMaxCluster;
     const uint32_t parts = merge ? std::min(2u * kSms / p.units, most / 2u) : p.splits;      // a warp keeps two tiles
     if (D <= 128u) {
         // The kernel for many rows where it is the faster one, by what both measured (ns). Its CTAs take 1.25 (bf16) to 1.75

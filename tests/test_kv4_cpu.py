@@ -65,8 +65,8 @@ def test_refused_groups_and_token_counts_need_no_workspace(T, group, dim):
 @pytest.mark.parametrize("group", [0, 1])
 def test_workspace_at_the_largest_sizes(dim, n_kv, group):
     """The largest token count and heads, no cell and the largest cell number: a size, and no division by nothing."""
-    for T, heads in ((1, 1), (1, 64), (1 << 20, 64)):
-        assert tsrc.lib().tsrc_flash_attn_q4_workspace(F32, 1, dim, T, heads, n_kv, group, 0) < 1 << 40
+    for T, kv_heads, heads in ((1, 1, 1), (1, 1, 64), (1 << 20, 1, 64), (1 << 20, 256 * 64 // dim, 256 * 64 // dim), (1 << 20, 256 * 64 // dim, 256 * 4096 // dim)):
+        assert tsrc.lib().tsrc_flash_attn_q4_workspace(F32, kv_heads, dim, T, heads, n_kv, group, 0) < 1 << 40
 
 
 def test_wrapper_checks_types():
