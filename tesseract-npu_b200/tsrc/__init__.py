@@ -230,15 +230,18 @@ def _stream_on(index: int, stream):
 
 def _workspace(like, nbytes: int, given, stream):
     """(tensor kept alive for the call, address, bytes) of a call's workspace: the caller's, or one from torch's
-    allocator, which orders its reuse by stream."""
+    allocator, taken on the call's own stream: a block is free for the stream that it was taken on, while work queued
+    there may still use it."""
     if given is not None:
         return given, _addr(given), nbytes if isinstance(given, int) else given.numel() * given.element_size()
     if nbytes == 0:
         return None, None, 0
     torch = _torch or _load_torch()
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    if stream is not None:
-        ws.record_stream(torch.cuda.ExternalStream(stream, device=like.device) if isinstance(stream, int) else stream)
+    if stream is None:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    else:
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=like.device) if isinstance(stream, int) else stream):
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
     return ws, ws.data_ptr(), nbytes
 
 
