@@ -88,11 +88,30 @@ template <class T> struct BeamVec {
     }
 };
 
-// A part is 8192 logits from a 16-byte boundary on (`lead` of the first part's lie before the row), a warp's share
-// 1024 neighbours, so 32 neighbours are 4 (f32: 8) lanes of one load. Each thread adds up its 32 exponentials against its
-// own largest, without waiting for anyone.
+// The 16 bytes that begin `bytes` (2 .. 14, the same for the whole CTA) into 32.
+__device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, uint32_t bytes) {
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (bytes & 8u) {
+#pragma unroll
+        for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+    }
+    if (bytes & 4u) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+    }
+    const uint32_t bits = 8u * (bytes & 3u);
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                      __funnelshift_r(w[3], w[4], bits));
+}
+
+// A part is 8192 logits counted from the row's own start, a warp's share 1024 neighbours, so 32 neighbours are 4 (f32: 8)
+// lanes of one load. Where the row starts off a 16-byte boundary (`lead` values behind one) a thread's 16 bytes are cut from
+// two aligned loads: which values are added up together, and in which order, does not depend on the row's address, so that
+// alike rows get the same normaliser to the last bit and their candidates tie.
+// Each thread adds up its 32 exponentials against its own largest, without waiting for anyone.
 // 256 rows of 128256 bf16 logits (65.7 MB): 82 us with scalar loads and the best chosen in every part, 37 us with wide
-// loads, 14.7 us so (4.5 TB/s).
+// loads, 14.7 us so (4.5 TB/s). Rows off a boundary: 256 of 50257 fp16 logits, both kernels, 38 us (36 with parts
+// cut by address).
 template <class T>
 __global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const T* __restrict__ logits, size_t stride, uint32_t n_vocab, BeamPart* parts,
                                                                  float* maxima) {
@@ -104,17 +123,41 @@ __global__ void __launch_bounds__(kBeamThreads) beam_part_kernel(const T* __rest
     const size_t row = blockIdx.y, at = row * gridDim.x + blockIdx.x;
     const T* x = logits + row * stride;
     const uint32_t lead = (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15u) / (uint32_t)sizeof(T);
-    const int64_t first = (int64_t)blockIdx.x * kBeamPart - lead + (warp * NV * 32u + lane) * V::N;
+    const uint32_t first = blockIdx.x * kBeamPart + (warp * NV * 32u + lane) * V::N;
     V v[NV];
+    auto ends = [&](uint32_t i) {                                // a row's ends
+        T t[V::N];
 #pragma unroll
-    for (uint32_t j = 0; j < NV; ++j) {
-        const int64_t i = first + j * 32u * V::N;
-        if (i >= 0 && i + V::N <= n_vocab) v[j].raw = __ldcs(reinterpret_cast<const uint4*>(x + i));
-        else {                                                   // a row's ends
-            T t[V::N];
+        for (uint32_t k = 0; k < V::N; ++k) t[k] = i + k < n_vocab ? x[i + k] : from_f32<T>(-INFINITY);
+        uint4 r;
+        __builtin_memcpy(&r, t, 16);
+        return r;
+    };
+    if (lead == 0) {
 #pragma unroll
-            for (uint32_t k = 0; k < V::N; ++k) t[k] = i + k >= 0 && i + k < n_vocab ? x[i + k] : from_f32<T>(-INFINITY);
-            __builtin_memcpy(&v[j].raw, t, 16);
+        for (uint32_t j = 0; j < NV; ++j) {
+            const uint32_t i = first + j * 32u * V::N;
+            v[j].raw = i + V::N <= n_vocab ? __ldcs(reinterpret_cast<const uint4*>(x + i)) : ends(i);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t j0 = 0; j0 < NV; j0 += 4) {                // four loads under way together, in the row whatever the place
+            uint4 lo[4], hi[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t i = first + (j0 + j) * 32u * V::N;
+                lo[j] = hi[j] = make_uint4(0, 0, 0, 0);
+                if (i >= lead && i - lead + 2u * V::N <= n_vocab) {
+                    const uint4* p = reinterpret_cast<const uint4*>(x + i - lead);
+                    lo[j] = p[0];
+                    hi[j] = p[1];
+                }
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t i = first + (j0 + j) * 32u * V::N;
+                v[j0 + j].raw = i >= lead && i - lead + 2u * V::N <= n_vocab ? shifted(lo[j], hi[j], lead * (uint32_t)sizeof(T)) : ends(i);
+            }
         }
     }
     float m = -INFINITY;
@@ -265,7 +308,6 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_select_kernel(const T* _
     for (uint32_t b = rank; b < n_beam; b += size) {
         const size_t row = group * n_beam + b;
         const T* x = logits + row * stride;
-        const uint32_t lead = (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15u) / (uint32_t)sizeof(T);
         // groups of 32 neighbours, or of 64 or 128 in the largest vocabularies
         const float* mx = maxima + row * n_parts * kBeamThreads;
         uint32_t fold = 0;
@@ -313,7 +355,7 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_select_kernel(const T* _
         const uint32_t shift = 5u + fold, n = n_out << shift;
         auto token = [&](uint32_t j) {                   // of this thread's logit j (s.best changes only when all have asked)
             const uint32_t e = j * kBeamThreads + tid;
-            return (int32_t)(~(uint32_t)s.best[min(e >> shift, n_out - 1u)] << shift) + (int32_t)(e & ((1u << shift) - 1u)) - (int32_t)lead;
+            return (int32_t)(~(uint32_t)s.best[min(e >> shift, n_out - 1u)] << shift) + (int32_t)(e & ((1u << shift) - 1u));
         };
 #pragma unroll
         for (uint32_t j = 0; j < kBeamEach; ++j) {
@@ -321,7 +363,7 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_select_kernel(const T* _
             if (j * kBeamThreads >= n) continue;
             const uint32_t e = j * kBeamThreads + tid;
             const int32_t i = token(j);
-            if (e < n && s.best[min(e >> shift, n_out - 1u)] != 0 && i >= 0 && i < (int32_t)n_vocab) v[j] = to_f32(x[i]);
+            if (e < n && s.best[min(e >> shift, n_out - 1u)] != 0 && i < (int32_t)n_vocab) v[j] = to_f32(x[i]);
         }
         select_best(s, v, (n + kBeamThreads - 1u) / kBeamThreads, least, n_out, [&](uint32_t j) { return (uint32_t)token(j); });
         for (uint32_t k = tid; k < n_out; k += kBeamThreads) {

@@ -1,0 +1,118 @@
+"""Attention over the q4_0 cache on the GPU: any content that the cache's format can hold, against 64 bits.
+
+Tolerance of an output value (e = 2^-24), for few visible cells or long rows alike:
+  scores   q is within 2^-22 of its value in two fp16 terms (bf16 and f16: exact in one); d (n - 8) is exact in two terms,
+           and the product of the two small terms, 2^-22, is left out; a sum over D values takes D / 16 tensor-core
+           steps for each of three products at most, each within 2 e of the running sum of magnitudes, and a few f32 steps for
+           the blocks' scales: |ds| <= (2^-21 + (6 D / 16 + 16) e) A, A = scale * max_c sum |q||k|;
+  weights  dp / p <= 2 |ds| + 2^-20 (the exponentials of a weight and of the sum) + 2^-21 (two fp16 terms and the product left out);
+  output   a chain of tensor-core sums, each cut by 2 e of its size at most: f32 prompts 4 tiles x 12 products, then one f32
+           step for 4 tiles; decode warps two products for 16 cells of a quarter of the cells, and a few f32 steps for the joins:
+           (96 + n / 256 + 64) e or (4 (n / 64 + 2) + 64) e; together and rounded up, C e with C = 160 + n / 16;
+           and half a step of `type` for the last rounding.
+All this is relative to sum p |v| of the output's own channel, so nothing that a row does not see, and no other block's scale,
+widens it. 16-bit outputs of the kernel for few rows take codes as subnormal numbers, which costs up to 2^-16 of
+15 sum p |d| besides; bf16 outputs round weights, and in the kernel for many rows K and V, to one fp16: 2^-10 (A + 1) sum p |v|.
+Where a weight is far below the row's largest it is held to 2^-30 of that, which matters only beside scales of
+V that differ by as much: 2^-28 max |d| over the visible cells.
+"""
+import numpy as np
+import pytest
+
+import kv4_plain as P
+import tsrc
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+HALF = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
+
+
+def _attend(q, kb, vb, Hk, scale, ranges, mask, dtype):
+    """(values, tolerances) in f64."""
+    T, H, D = q.shape
+    n = len(kb)
+    want, pv, pd, A = P.attend_many(q, kb, vb, Hk, scale, ranges, mask)
+    seen = (np.arange(n) >= np.maximum(np.asarray(ranges)[:, :1], 0)) & (np.arange(n) < np.asarray(ranges)[:, 1:])
+    if mask is not None:
+        seen &= ~np.isneginf(mask.astype(np.float64))
+    d = np.abs(np.ascontiguousarray(vb.reshape(n, -1, 18)[..., :2]).view(np.float16).astype(np.float64)).reshape(n, Hk, D // 32)
+    most = np.zeros((T, H, D))
+    for t in range(T):
+        if seen[t].any():
+            most[t] = np.repeat(np.repeat(np.nan_to_num(d[seen[t]].max(0), posinf=0.0), 32, -1), H // Hk, 0)
+    ds = (2.0 ** -21 + (6 * D / 16 + 16) * E) * A
+    tol = (2 * ds + 2.0 ** -20 + 2.0 ** -21 + (160 + n / 16) * E) * pv + 2.0 ** -28 * most
+    if mask is not None:
+        spread = np.zeros((T, 1, 1))
+        for t in range(T):
+            m = mask[t][seen[t]].astype(np.float64)
+            spread[t] = min(float(m.max() - m.min()), 200.0) if len(m) else 0.0
+        tol += 8 * E * spread * pv
+    if dtype == "float16":
+        tol += 2.0 ** -16 * 15 * pd
+    if dtype == "bfloat16":
+        tol += 2.0 ** -10 * (A + 1) * pv + 2.0 ** -16 * 15 * pd
+    return want, tol + np.maximum(HALF[dtype] * np.abs(want), 2.0 ** -25 if dtype == "float16" else 0.0) + 1e-30
+
+
+def _run(dev, q, kb, vb, Hk, scale, ranges=None, mask=None, group=0, max_len=0):
+    import torch
+    T, H, D = q.shape
+    kv = dev.kv4_create(Hk, D, len(kb))
+    try:
+        kv.set_bytes(tsrc.KV_K, kb)
+        kv.set_bytes(tsrc.KV_V, vb)
+        out = torch.full_like(q, float("nan"))
+        dev.flash_attn_q4(kv, q, out, T=T, n_head=H, n_kv=len(kb), scale=scale, group=group, max_len=max_len,
+                          ranges=None if ranges is None else torch.from_numpy(np.asarray(ranges, np.int32)).cuda(),
+                          mask=None if mask is None else torch.from_numpy(np.ascontiguousarray(mask)).cuda())
+        dev.sync()
+        return out.double().cpu().numpy()
+    finally:
+        kv.free()
+
+
+def _inputs(seed, T, H, Hk, D, n, dtype, q_size=1.0):
+    import torch
+    rng = np.random.default_rng(seed)
+    q = torch.from_numpy((q_size * rng.standard_normal((T, H, D))).astype(np.float32)).to(getattr(torch, dtype)).cuda()
+    return rng, q, P.random_rows(rng, n, Hk * D), P.random_rows(rng, n, Hk * D)
+
+
+def _scales(rows, Hk, D):
+    """The rows' scales as f16 [n, Hk, D / 32], to be written back by _set."""
+    return np.ascontiguousarray(rows.reshape(len(rows), Hk, D // 32, 18)[..., :2]).view(np.float16)[..., 0].copy()
+
+
+def _set(rows, Hk, D, d):
+    rows.reshape(len(rows), Hk, D // 32, 18)[..., :2] = np.ascontiguousarray(d.astype(np.float16))[..., None].view(np.uint8)
+
+
+def _check(dev, q, kb, vb, Hk, dtype, ranges, mask=None, scale=0.05, **kw):
+    scale = float(np.float32(scale))
+    want, tol = _attend(q.double().cpu().numpy(), kb, vb, Hk, scale, ranges, mask, dtype)
+    got = _run(dev, q, kb, vb, Hk, scale, ranges, mask, **kw)
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (int(bad.sum()), bad.size, float(np.nanmax(np.abs(got - want) / tol)), np.argwhere(bad)[:3].tolist())
+
+
+# tokens and heads that reach the kernel for few rows, and those for 128 and (bf16) 256 rows
+SHAPES = [(1, 8, 2), (5, 32, 8), (300, 32, 8), (1300, 32, 8)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("T,H,Hk", SHAPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_blocks_of_very_different_scales(dev, dtype, T, H, Hk, D):
+    """V's and K's scales fall by 2^0, 2^10, 2^16, 2^13 from block to block of every cell, and by a random power besides; rows
+    that see one cell, a few or all."""
+    if D == 256 and T == 1300:
+        T = 100
+    n = 200
+    rng, q, kb, vb = _inputs(T + D, T, H, Hk, D, n, dtype, 0.2)
+    fall = np.array([0, 10, 16, 13, 5, 11, 15, 3], np.float64)[:D // 32]
+    for rows, by in ((kb, fall[::-1]), (vb, fall)):
+        _set(rows, Hk, D, 4 * _scales(rows, Hk, D).astype(np.float64) * 2.0 ** -by)
+    ranges = [[t % n, t % n + 1] if t % 3 == 0 else [t % (n - 5), t % (n - 5) + 3] if t % 3 == 1 else [0, n] for t in range(T)]
+    _check(dev, q, kb, vb, Hk, dtype, ranges)
