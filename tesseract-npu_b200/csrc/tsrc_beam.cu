@@ -24,11 +24,20 @@ namespace {
 constexpr uint32_t kBeamThreads = 256, kBeamEach = 32, kBeamPart = kBeamThreads * kBeamEach;
 constexpr uint32_t kBeamOut = 64, kBeamBeams = 64, kBeamVocab = 1u << 20;
 constexpr uint32_t kBeamCap = kBeamOut * kBeamEach;      // a list's room: what n_out threads can hold
-constexpr uint32_t kBeamLists = (kBeamVocab + 7u + kBeamPart - 1u) / kBeamPart / 32u + 1u;    // parts that a lane adds up
+constexpr uint32_t kBeamLists = kBeamVocab / kBeamPart / 32u;    // parts that a lane adds up
 constexpr uint32_t kBeamRows = 8;                        // rows that a cluster takes at once
 
-// parts of a row, with room for the up to seven values before it that its first 16 bytes may hold
-__host__ __device__ inline uint32_t beam_parts(uint32_t n_vocab) { return (n_vocab + 7u + kBeamPart - 1u) / kBeamPart; }
+__host__ __device__ inline uint32_t beam_parts(uint32_t n_vocab) { return (n_vocab + kBeamPart - 1u) / kBeamPart; }
+
+// Neighbours that a maximum stands for in the first selection, as a power of two: 32, and 64 or 128 in the largest
+// vocabularies, whose maxima would be more than a CTA holds.
+__host__ __device__ constexpr uint32_t beam_fold(uint32_t n_parts) {
+    uint32_t fold = 0;
+    while (n_parts * kBeamThreads >> fold > kBeamPart) ++fold;
+    return fold;
+}
+// the second selection holds the neighbours of n_out of them
+static_assert(kBeamOut << (5u + beam_fold(kBeamVocab / kBeamPart)) <= kBeamPart, "room for the largest vocabulary");
 
 struct BeamPart {
     float max, sum;      // sum of exp(x - max) over the part (-inf and 0 where the part is all -inf)
@@ -308,10 +317,8 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_select_kernel(const T* _
     for (uint32_t b = rank; b < n_beam; b += size) {
         const size_t row = group * n_beam + b;
         const T* x = logits + row * stride;
-        // groups of 32 neighbours, or of 64 or 128 in the largest vocabularies
         const float* mx = maxima + row * n_parts * kBeamThreads;
-        uint32_t fold = 0;
-        while (n_parts * kBeamThreads >> fold > kBeamPart) ++fold;
+        const uint32_t fold = beam_fold(n_parts);
         const uint32_t n_groups = (n_parts * kBeamThreads + (1u << fold) - 1u) >> fold;
         float v[kBeamEach];
 #pragma unroll

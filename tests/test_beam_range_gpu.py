@@ -44,3 +44,32 @@ def test_alike_rows_tie_wherever_they_lie(dev, dtype, V):
         alone = alone or one
         for a, b in zip(one, alone):
             np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("V", [262137, 262138, 262145, 524282, 524288, 1048569, 1048570, 1 << 20])
+@pytest.mark.parametrize("kind", ["scattered", "ascending", "tied"])
+def test_largest_vocabularies(dev, V, kind):
+    """Where groups of 32 neighbours become groups of 64 and 128; rows on and off a wide boundary."""
+    import torch
+    if kind == "scattered":
+        row = 3 * torch.randn(V, generator=torch.Generator().manual_seed(V))
+    elif kind == "ascending":
+        row = torch.linspace(-8, 8, V)
+    else:
+        row = torch.zeros(V)
+    buf = torch.zeros(V + 16, device="cuda")
+    value, at = row.double().sort(descending=True, stable=True)
+    norm = row.double().logsumexp(0)
+    want = (value[:64] - norm).numpy()
+    for off in (0, 3):
+        buf[off:off + V] = row.cuda()
+        for n_out in (1, 32, 33, 64):
+            s, b, t = _select(dev, buf[off:], None, 1, 1, V, n_out)
+            np.testing.assert_array_equal(t[0], at[:n_out].numpy())
+            assert (b == 0).all()
+            assert (np.abs(s[0] - want[:n_out]) <= 2.0 ** -18 + np.abs(want[:n_out]) * 2.0 ** -24).all()
+    for dtype in (torch.float16, torch.bfloat16):
+        x = row.to(dtype)
+        value, at = x.double().sort(descending=True, stable=True)
+        _, _, t = _select(dev, x.cuda(), None, 1, 1, V, 64)
+        np.testing.assert_array_equal(t[0], at[:64].numpy())
