@@ -15,13 +15,13 @@
 // The reference that the weights' exponents are taken from follows the running maximum only when that has risen by
 // 8 (in log2): outputs in tensor memory are then rescaled, seldom after the first tiles; up to there weights reach
 // 2^8, which fp16 holds, and results do not depend on the reference.
-//   Range: q is scaled by a power of two per row, K's and V's scales by one per dequant warp's cells, so that all
-// operands stay inside fp16 and the dequant warps need not agree on one. K's is made good in the scores, V's in the
-// weights, relative to the largest seen (with O rescaled when that rises). Scales of 32 and above, which no row of ordinary size
-// has, do not move these: such a cell gets a power of two of its own, which its scores and weights make good, so that
-// rows that do not see it keep their digits. Precision: bf16 outputs take one fp16 term (11 bits) of
-// q (exact), K, V and the weights. f32 and f16 outputs take two terms of each, 22 bits (d (n - 8) has 15, so K and V
-// are exact), and three products, the one of the two small terms left out: 2^-22 of the result.
+//   Range: q is scaled by a power of two per row; K and V go in as 2^7 d (n - 8), which fills fp16 from scales of 32
+// down (2^7 32 8 = 2^15) to the smallest that the cache can hold (2^-24: an operand of 2^-17, a normal number from 2^-21 on),
+// so that no block's scale costs another block's digits, in its cell or elsewhere. A cell with a scale of 32 and above, which
+// no row of ordinary size has, gets a power of two of its own, which its scores and weights make good: rows that do not
+// see it keep their digits (beside one of 2^15, a block of the same cell keeps all of its own down to 2^-10). Precision:
+// bf16 outputs take one fp16 term (11 bits) of q (exact), K, V and the weights. f32 and f16 outputs take two terms of each, 22
+// bits (d (n - 8) has 15, so K and V are exact), and three products, the one of the two small terms left out: 2^-22 of the result.
 #include <type_traits>
 
 #include "tsrc_fa4.cuh"
@@ -61,15 +61,14 @@ template <class T, int D, bool MASK, uint32_t RG> struct TcShape {              
     static_assert(O_COL + RG * D <= COLUMNS && SUM_COL + (TOTAL ? D : 0) <= COLUMNS && (RG == 1 || !TOTAL), "tensor memory");
 };
 
+constexpr int kOperandExp = 7;       // K and V operands are 2^7 of the values
 // What the dequant warps tell of a tile: each of its own cells, 64 / DW in a row.
-struct __align__(16) TileInfo {
-    float k_unscale[8];      // the K operand times this is K
-    float v_log[8], v_inv[8];    // log2 of what the V operand lacks, and 2 to minus that
+struct __align__(8) TileInfo {
     uint8_t flags[8];        // kBad, kFar
 };
 constexpr uint32_t kBad = 1;         // a scale of V that is no number or infinite is there (its block is 0 in the operand)
 constexpr uint32_t kFar = 2;         // a scale above the common ones is there: the cells' own powers of two count
-constexpr uint32_t kFarExp = 19;     // exponent field of scales of 16 to 32, the largest that the common powers follow
+constexpr uint32_t kFarExp = 19;     // exponent field of scales of 16 to 32, the largest common ones
 
 struct Control {                     // at most 4 KB
     uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
@@ -161,9 +160,9 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 __device__ __forceinline__ __half2 as_h2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
-// 2^(15 - e) in fp16: a scale with exponent field e goes to [1, 2)
-__device__ __forceinline__ __half2 to_one(uint32_t e) {
-    return __half2half2(__ushort_as_half(e < 30u ? (unsigned short)((30u - e) << 10) : (unsigned short)0x0200u));
+// What a cell's scales are times, e (kFarExp to 30) the exponent field of the largest: 2^7, or what takes that to below 2^12.
+__device__ __forceinline__ __half2 operand_factor(uint32_t e) {
+    return __half2half2(__ushort_as_half((unsigned short)((15u + kOperandExp + kFarExp - e) << 10)));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
@@ -192,41 +191,21 @@ __device__ __forceinline__ uint32_t finite_most(uint32_t u) {
 __device__ __forceinline__ uint32_t finite_only(uint32_t u) {
     return ((u & 0x7C00u) == 0x7C00u ? 0u : u & 0xFFFFu) | ((u & 0x7C000000u) == 0x7C000000u ? 0u : u & 0xFFFF0000u);
 }
-// Codes i = 0..3 of two halves side by side (four bits each) times d, that is d (n - 8), as operand words.
-//   Two terms: n - 8 without rounding from the fp16 whose last bits are n (1024 + n, or 1024 + 16 n with the code in
-// the next four bits), then the rounded product and what it lacks.
-//   One term: a code in the last bits of an fp16 is the subnormal number n 2^-24 (n 2^-20 in the next four), so one
-// fused step with 2^14 d (2^10 d) and -8 2^-10 d gives d (n - 8) 2^-10, rounded once; d is below 2, so 2^14 d fits.
-template <bool PRECISE> struct Scaled;
-template <> struct Scaled<true> {
-    static constexpr int UNDO = 0;               // log2 of what the operand lacks
-    __half2 d;
-    __device__ __forceinline__ explicit Scaled(__half2 s) : d(s) {}
-    __device__ __forceinline__ void words(uint32_t x, uint32_t (&h)[4], uint32_t (&l)[4]) const {
+// Codes i = 0..3 of two halves side by side (four bits each) times d, that is d (n - 8), as operand words: n - 8 without
+// rounding from the fp16 whose last bits are n (1024 + n, or 1024 + 16 n with the code in the next four bits), then the rounded
+// product and, of two terms, what it lacks.
+template <bool PRECISE>
+__device__ __forceinline__ void scaled(__half2 d, uint32_t x, uint32_t (&h)[4], uint32_t (&l)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t y = j & 2 ? x >> 8 : x;
-            const __half2 n = j & 1 ? __hfma2(as_h2((y & 0x00F000F0u) | 0x64006400u), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f))
-                                    : __hsub2(as_h2((y & 0x000F000Fu) | 0x64006400u), __float2half2_rn(1032.0f));
-            const __half2 w = __hmul2(n, d);
-            h[j] = as_u32(w);
-            l[j] = as_u32(__hfma2(n, d, __hneg2(w)));
-        }
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t y = j & 2 ? x >> 8 : x;
+        const __half2 n = j & 1 ? __hfma2(as_h2((y & 0x00F000F0u) | 0x64006400u), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f))
+                                : __hsub2(as_h2((y & 0x000F000Fu) | 0x64006400u), __float2half2_rn(1032.0f));
+        const __half2 w = __hmul2(n, d);
+        h[j] = as_u32(w);
+        if (PRECISE) l[j] = as_u32(__hfma2(n, d, __hneg2(w)));
     }
-};
-template <> struct Scaled<false> {
-    static constexpr int UNDO = 10;
-    __half2 a, b, c;
-    __device__ __forceinline__ explicit Scaled(__half2 s)
-        : a(__hmul2(s, __float2half2_rn(16384.0f))), b(__hmul2(s, __float2half2_rn(1024.0f))), c(__hmul2(s, __float2half2_rn(-0.0078125f))) {}
-    __device__ __forceinline__ void words(uint32_t x, uint32_t (&h)[4], uint32_t (&)[4]) const {
-        const uint32_t y = x >> 8;
-        h[0] = as_u32(__hfma2(as_h2(x & 0x000F000Fu), a, c));
-        h[1] = as_u32(__hfma2(as_h2(x & 0x00F000F0u), b, c));
-        h[2] = as_u32(__hfma2(as_h2(y & 0x000F000Fu), a, c));
-        h[3] = as_u32(__hfma2(as_h2(y & 0x00F000F0u), b, c));
-    }
-};
+}
 
 // Eight cells of a row's mask from `cell` on, -inf where `seen` lacks the cell's bit (the mask there may hold anything).
 // wide: the row holds all of the tile in aligned memory, and the load stands outside any branch, so that a tile's eight are
@@ -371,7 +350,7 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
         const int e2 = min(12 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
         const float f = copysignf(pow2(e2), a.scale);        // the factor that scores get is positive
-        if (lane < 8) c.q_unscale[r] = fabsf(a.scale) * 1.4426950408889634f * pow2(-e2);
+        if (lane < 8) c.q_unscale[r] = fabsf(a.scale) * 1.4426950408889634f * pow2(-e2 - kOperandExp);
 #pragma unroll
         for (uint32_t j = 0; j < D / 32; ++j) {
             uint32_t h[4], l[4];
@@ -522,56 +501,45 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                 for (uint32_t b = 0; b < NB / 2; ++b) mk = __hmax2_nan(mk, __habs2(as_h2(ks[u][b])));
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k) mv = __hmax2_nan(mv, __habs2(as_h2(vs[k])));
-            uint32_t xk = max(as_u32(mk) & 0xFFFFu, as_u32(mk) >> 16), xv = max(as_u32(mv) & 0xFFFFu, as_u32(mv) >> 16);
-            xk = __reduce_max_sync(0xFFFFFFFFu, xk);
-            xv = __reduce_max_sync(0xFFFFFFFFu, xv);
-            bool bad = false;
-            if (xk >= 0x7C00u) {
-                uint32_t x = 0;
+            const __half2 both = __hmax2_nan(mk, mv);
+            bool bad = false, far = false;
+            __half2 k_one[KU], v_one[4];             // powers of two that the scales are times
+#pragma unroll
+            for (uint32_t u = 0; u < KU; ++u) k_one[u] = operand_factor(kFarExp);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) v_one[k] = operand_factor(kFarExp);
+            if (__any_sync(0xFFFFFFFFu, max(as_u32(both) & 0xFFFFu, as_u32(both) >> 16) >= (kFarExp + 1u) << 10)) {        // seldom
+                uint32_t x = 0, odd = 0;
 #pragma unroll
                 for (uint32_t u = 0; u < KU; ++u)
 #pragma unroll
                     for (uint32_t b = 0; b < NB / 2; ++b) x = max(x, finite_most(ks[u][b]));
-                xk = __reduce_max_sync(0xFFFFFFFFu, x);
-            }
-            if (xv >= 0x7C00u) {
-                uint32_t x = 0;
 #pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) x = max(x, finite_most(vs[k]));
-                xv = __reduce_max_sync(0xFFFFFFFFu, x);
-                bad = true;
+                for (uint32_t k = 0; k < 8; ++k) {
+                    x = max(x, finite_most(vs[k]));
+                    odd |= vs[k] ^ finite_only(vs[k]);
+                }
+                far = __any_sync(0xFFFFFFFFu, x >> 10 > kFarExp);
+                bad = __any_sync(0xFFFFFFFFu, odd != 0);
             }
-            const uint32_t k_exp = min(max(xk >> 10, 1u), kFarExp), v_exp = min(max(xv >> 10, 1u), kFarExp);
-            const bool far = max(xk, xv) >> 10 > kFarExp;
-            if (lane == 0) {
-                TileInfo& info = c.info[i & 3u];
-                info.k_unscale[dw] = pow2((int)k_exp - 15 + Scaled<PRECISE>::UNDO);
-                info.v_log[dw] = (float)((int)v_exp - 15 + Scaled<PRECISE>::UNDO);
-                info.v_inv[dw] = pow2(15 - Scaled<PRECISE>::UNDO - (int)v_exp);
-                info.flags[dw] = (uint8_t)((bad ? kBad : 0u) | (far ? kFar : 0u));
-            }
-            __half2 k_one[KU], v_one[4];             // powers of two that take the scales to [1, 2) at most
-#pragma unroll
-            for (uint32_t u = 0; u < KU; ++u) k_one[u] = to_one(k_exp);
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) v_one[k] = to_one(v_exp);
+            if (lane == 0) c.info[i & 3u].flags[dw] = (uint8_t)((bad ? kBad : 0u) | (far ? kFar : 0u));
             if (far) {
 #pragma unroll
                 for (uint32_t u = 0; u < KU; ++u) {
-                    uint32_t own = k_exp;
+                    uint32_t own = kFarExp;
 #pragma unroll
                     for (uint32_t b = 0; b < NB / 2; ++b) own = max(own, finite_most(ks[u][b]) >> 10);
-                    k_one[u] = to_one(own);
-                    if (kt == 0) c.cell_k[i & 3u][kc + 8u * u] = pow2((int)(own - k_exp));
+                    k_one[u] = operand_factor(own);
+                    if (kt == 0) c.cell_k[i & 3u][kc + 8u * u] = pow2((int)(own - kFarExp));
                 }
 #pragma unroll
                 for (uint32_t k = 0; k < 8; ++k) {
                     uint32_t x = finite_most(vs[k]);
 #pragma unroll
                     for (uint32_t o = 8; o < (BV == 2 ? 16u : 32u); o <<= 1) x = max(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
-                    const uint32_t own = max(v_exp, x >> 10);
-                    if (g == 0 && vb == 0) c.cell_v[i & 3u][8u * vg + k] = (float)(own - v_exp);
-                    const __half2 one = to_one(own);
+                    const uint32_t own = max(kFarExp, x >> 10);
+                    if (g == 0 && vb == 0) c.cell_v[i & 3u][8u * vg + k] = (float)(own - kFarExp);
+                    const __half2 one = operand_factor(own);
                     v_one[k / 2] = k & 1u ? __lows2half2(v_one[k / 2], one) : __lows2half2(one, one);
                 }
             }
@@ -591,7 +559,7 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                     const uint32_t s = ks[u][b / 2];
                     const __half2 d = __hmul2(as_h2(__byte_perm(s, s, b & 1u ? 0x3232 : 0x1010)), k_one[u]);
                     uint32_t h[4], l[4];
-                    Scaled<PRECISE>(d).words(x, h, l);
+                    scaled<PRECISE>(d, x, h, l);
                     uint8_t* p = kb + (4u * b + kt) * (kTile * 16u) + (kc + 8u * u) * 16u;
                     *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
                     if (PRECISE) *reinterpret_cast<uint4*>(p + S::KV_TERM) = make_uint4(l[0], l[1], l[2], l[3]);
@@ -619,7 +587,7 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                     for (uint32_t k = 0; k < 4; ++k) {
                         const uint32_t x = __byte_perm(cw[2 * k], cw[2 * k + 1], b ? 0x7632 : 0x5410);
                         const __half2 d = __hmul2(as_h2(__byte_perm(cs[2 * k], cs[2 * k + 1], b ? 0x7632 : 0x5410)), v_one[k]);
-                        Scaled<PRECISE>(d).words(x, h[k], l[k]);
+                        scaled<PRECISE>(d, x, h[k], l[k]);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -642,7 +610,6 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
         float off = MASK ? -INFINITY : 0.0f;         // the mask's maximum so far: scores and m are relative to it
         // a thread without a row may load the last token's, and sees nothing of it
         const __half* mrow = MASK ? a.mask + (size_t)min(tok, a.T - 1u) * a.mask_stride : nullptr;
-        float v_ref = -14.0f + Scaled<PRECISE>::UNDO;    // log2 of what outputs lack: the largest v_log so far
         uint32_t lost = 0;                           // blocks of V in which the row sees a scale that is no number
         bool ok = true;
         // the cells that all rows of the warp see; rows behind the group's last lose nothing
@@ -658,27 +625,21 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
             fence_after();
             constexpr uint32_t GC = kTile / S::DW;   // cells of a dequant warp
             const TileInfo& info = c.info[i & 3u];
-            float f[S::DW], v_log[S::DW];            // factors of scores
+            float f = qs;                            // what scores are times
             uint32_t flags = 0;
 #pragma unroll
-            for (uint32_t w = 0; w < S::DW; w += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(info.k_unscale + w), y = *reinterpret_cast<const float4*>(info.v_log + w);
-                f[w] = qs * x.x; f[w + 1] = qs * x.y; f[w + 2] = qs * x.z; f[w + 3] = qs * x.w;
-                v_log[w] = y.x; v_log[w + 1] = y.y; v_log[w + 2] = y.z; v_log[w + 3] = y.w;
-                flags |= *reinterpret_cast<const uint32_t*>(info.flags + w);
-            }
+            for (uint32_t w = 0; w < S::DW; w += 4) flags |= *reinterpret_cast<const uint32_t*>(info.flags + w);
             const bool open = c0 >= all_lo && c0 + (int32_t)kTile <= all_hi, far = flags & kFar * 0x01010101u, bad = flags & kBad * 0x01010101u;
             if (far) {                               // seldom: scores with the cells' own powers of two, put back for what follows
 #pragma unroll 1
                 for (uint32_t k = 0; k < kTile; k += 8) {
-                    const float fk = qs * info.k_unscale[k / GC];
                     const bool own = info.flags[k / GC] & kFar;
                     uint32_t x[8];
                     tmem_ld8(at + k, x);
                     tmem_wait_ld8(x);
 #pragma unroll
                     for (uint32_t j = 0; j < 8; ++j) {
-                        const float z = __uint_as_float(x[j]) * fk;
+                        const float z = __uint_as_float(x[j]) * qs;
                         x[j] = __float_as_uint(own ? fmaf(z, c.cell_k[i & 3u][k + j], c.cell_v[i & 3u][k + j]) : z);
                     }
                     tmem_st8(at + k, x);
@@ -694,10 +655,9 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
             if (MASK || !open || far) {              // then these are the scores, elsewhere their factors wait for the exponent
                 if (!far) {
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * f[j / GC]);
+                    for (int j = 0; j < 64; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * qs);
                 }
-#pragma unroll
-                for (uint32_t w = 0; w < S::DW; ++w) f[w] = 1.0f;
+                f = 1.0f;
             }
             if (!open) {
                 const int32_t from = min(max(lo - c0, 0), 64), to = min(max(hi - c0, from), 64);
@@ -739,16 +699,16 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                 if (a.mask_wide && c0 + (int32_t)kTile <= (int32_t)a.n_kv) pass(std::true_type{});
                 else pass(std::false_type{});
             }
-            float most = -INFINITY, v_now = v_ref;
+            float most = -INFINITY;
 #pragma unroll
-            for (uint32_t w = 0; w < S::DW; ++w) {
-                float top = max3(__uint_as_float(raw[GC * w]), __uint_as_float(raw[GC * w + 1]), __uint_as_float(raw[GC * w + 2]));
+            for (uint32_t w = 0; w < 4; ++w) {
+                float top = max3(__uint_as_float(raw[16 * w]), __uint_as_float(raw[16 * w + 1]), __uint_as_float(raw[16 * w + 2]));
 #pragma unroll
-                for (uint32_t j = 3; j + 1 < GC; j += 2) top = max3(top, __uint_as_float(raw[GC * w + j]), __uint_as_float(raw[GC * w + j + 1]));
-                most = fmaxf(most, fmaxf(top, __uint_as_float(raw[GC * w + GC - 1])) * f[w]);
-                v_now = fmaxf(v_now, v_log[w]);
+                for (uint32_t j = 3; j + 1 < 16; j += 2) top = max3(top, __uint_as_float(raw[16 * w + j]), __uint_as_float(raw[16 * w + j + 1]));
+                most = max3(most, top, __uint_as_float(raw[16 * w + 15]));
             }
-            const bool raise = __any_sync(0xFFFFFFFFu, most > m + 8.0f || v_now != v_ref);
+            most *= f;
+            const bool raise = __any_sync(0xFFFFFFFFu, most > m + 8.0f);
             const bool flush = TOTAL && i > 0 && i % S::FLUSH == 0u;
             if (raise || flush) {
                 float both = 1.0f;
@@ -756,8 +716,7 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                     const float now = fmaxf(m, most), base = now == -INFINITY ? 0.0f : now, down = ex2(m - base);
                     l *= down;
                     m = now;
-                    both = down * pow2((int)(v_ref - v_now));
-                    v_ref = v_now;
+                    both = down;
                 }
                 if (i > 0) {
                     // the products so far have to be there
@@ -789,25 +748,16 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                     __syncwarp();
                 }
             }
-            // The weights times what their cells' V lacks beside v_ref. Sums are of these, each dequant warp's cells for
-            // themselves, and then made good.
-            float near_sum = 0.0f;
-            float2 sum[2];
+            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {            // sixteen cells at a time: eight words of each term
                 uint32_t hw[8], lw[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const uint32_t e = 16 * k + 2 * j, w = e / GC;
-                    const float uw = up + (v_log[w] - v_ref);
-                    const float2 z = fma2(make_float2(__uint_as_float(raw[e]), __uint_as_float(raw[e + 1])), make_float2(f[w], f[w]), make_float2(uw, uw));
+                    const uint32_t e = 16 * k + 2 * j;
+                    const float2 z = fma2(make_float2(__uint_as_float(raw[e]), __uint_as_float(raw[e + 1])), make_float2(f, f), make_float2(up, up));
                     const float2 p = make_float2(ex2(z.x), ex2(z.y));
-                    if (e % GC < 4) sum[e / 2 & 1u] = p;
-                    else sum[e / 2 & 1u] = add2(sum[e / 2 & 1u], p);
-                    if (e % GC == GC - 2u) {
-                        const float2 both = add2(sum[0], sum[1]);
-                        near_sum = fmaf(both.x + both.y, info.v_inv[w], near_sum);
-                    }
+                    sum[j & 1] = add2(sum[j & 1], p);
                     const __half2 h = __floats2half2_rn(p.x, p.y);
                     hw[j] = as_u32(h);
                     if (PRECISE) {
@@ -818,7 +768,8 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                 tmem_st8(at + 8u * k, hw);
                 if (PRECISE) tmem_st8(at + kTile / 2u + 8u * k, lw);
             }
-            l += far ? far_sum : near_sum * pow2((int)v_ref);
+            const float2 total = add2(sum[0], sum[1]);
+            l += far ? far_sum : total.x + total.y;
             tmem_wait_st();
             fence_before();
             __syncwarp();
@@ -839,7 +790,7 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
         if (ok) {
             fence_after();
             // l and O are in units of 2^6 p: a split's share names 2^-6 of its reference
-            const float unit = pow2((int)v_ref), f = a.splits > 1u ? unit : l == 0.0f ? 0.0f : unit / l;
+            const float unit = pow2(-kOperandExp), f = a.splits > 1u ? unit : l == 0.0f ? 0.0f : unit / l;
             T* out = static_cast<T*>(a.out) + (size_t)tok * a.out_stride + (size_t)head * D;
             const size_t part = ((((size_t)grp * a.row_tiles + rt) * a.n_head_kv + hk) * a.splits + split) * (kRows * RG) + tid;
             if (a.splits > 1u && row < rows) *reinterpret_cast<float4*>(a.part_ml + part * 4u) = make_float4(off, m - 6.0f, l, 0.0f);
