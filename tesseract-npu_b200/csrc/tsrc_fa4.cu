@@ -266,6 +266,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
 
     float o[NT][NB][2][4] = {}, wsum[NT][NB][2] = {}, m[NT][2], l[NT][2], off[NT][2];
     uint32_t vexp = 1;
+    uint32_t lost = 0;       // bit 4 (2 n + i) + b: the row sees a scale of V in block b that is infinite or no number
 #pragma unroll
     for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
@@ -393,20 +394,37 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
                 dv[e][b] = as_h2(__byte_perm(x[b / 2], y[b / 2], b & 1u ? 0x7632 : 0x5410));
-                most = __hmax2(most, __habs2(dv[e][b]));          // a NaN is passed over
+                most = __hmax2_nan(most, __habs2(dv[e][b]));
             }
         }
         uint32_t big = __reduce_max_sync(0xFFFFFFFFu, max(as_u32(most) & 0xFFFFu, as_u32(most) >> 16));
-        if (big >= 0x7C00u) {                                     // an infinity among them (seldom): the largest finite one
+        if (big >= 0x7C00u) {
+            // Seldom: such a scale counts as 0 in the products, and its block is marked for the rows that see the cell,
+            // whatever weight they give it.
             uint32_t x = 0;
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e)
 #pragma unroll
                 for (uint32_t b = 0; b < NB; ++b) {
-                    const uint32_t u = as_u32(dv[e][b]) & 0x7FFF7FFFu, u0 = u & 0xFFFFu, u1 = u >> 16;
-                    x = max(x, max(u0 < 0x7C00u ? u0 : 0u, u1 < 0x7C00u ? u1 : 0u));
+                    uint32_t u = as_u32(dv[e][b]);
+                    u = ((u & 0x7C00u) == 0x7C00u ? 0u : u & 0xFFFFu) | ((u & 0x7C000000u) == 0x7C000000u ? 0u : u & 0xFFFF0000u);
+                    dv[e][b] = as_h2(u);
+                    x = max(x, max(u & 0x7FFFu, u >> 16 & 0x7FFFu));
                 }
             big = __reduce_max_sync(0xFFFFFFFFu, x);
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint16_t* pd = reinterpret_cast<const uint16_t*>(sk + S::VD_AT + (pg + 8u * j) * S::DS);
+                const int32_t c = (int32_t)(c0 + pg + 8u * j);
+                uint32_t bad = 0;
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) bad |= (pd[b] & 0x7C00u) == 0x7C00u ? 1u << b : 0u;
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i)
+                        if (open || (MASK ? mk[n][i][j] != -INFINITY : c >= lo[n][i] && c < hi[n][i])) lost |= bad << (4u * (2u * n + i));
+            }
         }
         bool moved = false;
         float rescale = 1.0f;
@@ -499,17 +517,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
                     const float2 back = __half22float2(h);
                     pl = as_h2(transpose8(pack2(s[n][0][e] - back.x, s[n][1][e] - back.y)));
                 }
-                // a cell whose weight is 0 has no part in the outputs, whatever its scale is
-                const uint32_t keep = open ? 0xFFFFFFFFu : __hne2_mask(ph, __float2half2_rn(0.0f));
 #pragma unroll
                 for (uint32_t b = 0; b < NB; ++b) {
                     const __half2 x = __hmul2(ph, dv[e][b]);
                     wb[n][0][e][b] = as_u32(x);
                     if (SPLIT) wb[n][SPLIT ? 1 : 0][e][b] = as_u32(__hfma2(pl, dv[e][b], __hfma2(ph, dv[e][b], __hneg2(x))));
-                    if (!open) {
-                        wb[n][0][e][b] &= keep;
-                        if (SPLIT) wb[n][SPLIT ? 1 : 0][e][b] &= keep;
-                    }
                 }
             }
 #pragma unroll
@@ -567,6 +579,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
 
     // the warp's results in its ring: [R][W] outputs without their scales; maxima and sums beside the rings
     float* wo = reinterpret_cast<float*>(ringp);
+#pragma unroll
+    for (uint32_t x = 4; x < 32; x <<= 1) lost |= __shfl_xor_sync(0xFFFFFFFFu, lost, x);
     const float unscale = pow2((WHOLE ? 0 : 24) - value_exp(vexp)), pinv = pow2(-weight_exp(vexp));
 #pragma unroll
     for (uint32_t n = 0; n < NT; ++n) {
@@ -577,8 +591,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
 #pragma unroll
                 for (uint32_t i = 0; i < 2; ++i) {
                     float* p = wo + (8u * n + 2u * t + i) * S::W + 32u * b + 4u * g + 2u * k;
-                    p[0] = (o[n][b][k][i] - wsum[n][b][i]) * (unscale * pinv);
-                    p[1] = (o[n][b][k][2 + i] * kOdd - wsum[n][b][i]) * (unscale * pinv);
+                    const bool none = lost >> (4u * (2u * n + i) + b) & 1u;
+                    p[0] = none ? NAN : (o[n][b][k][i] - wsum[n][b][i]) * (unscale * pinv);
+                    p[1] = none ? NAN : (o[n][b][k][2 + i] * kOdd - wsum[n][b][i]) * (unscale * pinv);
                 }
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
@@ -621,8 +636,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (uint32_t j = 0; j < S::TEAMS; ++j) {
-            const float f = red[j * S::NG * 16u + r].w;
-            if (f == 0.0f) continue;
+            const float f = red[j * S::NG * 16u + r].w;          // outputs are finite or marked by NaN, which a factor of 0 keeps
             const float4 x = *result(j, r, d);
             acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
         }
@@ -687,7 +701,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
             if (k < a.splits) x[k] = remote_f32x4(result(0, r, d), k);
 #pragma unroll
         for (uint32_t k = 0; k < kMaxCluster; ++k)
-            if (k < a.splits && f[k] != 0.0f) {
+            if (k < a.splits) {
                 acc.x += f[k] * x[k].x; acc.y += f[k] * x[k].y; acc.z += f[k] * x[k].z; acc.w += f[k] * x[k].w;
             }
         put(r, d, acc, f[kMaxCluster]);

@@ -116,3 +116,34 @@ def test_blocks_of_very_different_scales(dev, dtype, T, H, Hk, D):
         _set(rows, Hk, D, 4 * _scales(rows, Hk, D).astype(np.float64) * 2.0 ** -by)
     ranges = [[t % n, t % n + 1] if t % 3 == 0 else [t % (n - 5), t % (n - 5) + 3] if t % 3 == 1 else [0, n] for t in range(T)]
     _check(dev, q, kb, vb, Hk, dtype, ranges)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("T,H,Hk,D,n", [(1, 8, 2, 128, 200), (3, 8, 2, 64, 200), (3, 4, 2, 256, 77), (2, 2, 1, 512, 90), (1, 8, 2, 128, 5000),
+                                        (1, 4, 1, 64, 40000), (1, 2, 1, 256, 40000), (300, 32, 8, 64, 200), (1300, 32, 8, 128, 200)])
+@pytest.mark.parametrize("bits", [0x7C00, 0xFC00, 0x7E01])
+def test_scale_of_v_that_is_not_finite_shows_at_any_weight(dev, dtype, T, H, Hk, D, n, bits):
+    """A visible cell whose weight is 0 in any arithmetic, by its score or by a mask of the type's lowest value, in tiles that
+    all rows see whole and in others: its block is not finite, and no other output changes."""
+    low = np.float16(np.finfo(np.float16).min)
+    for masked in (False, True):
+        rng, q, kb, vb = _inputs(T + D, T, H, Hk, D, n, dtype)
+        q[:] = 1.0
+        at = n // 2 + 1
+        mask = None
+        b = kb.reshape(n, Hk, D // 32, 18)
+        b[..., 2:] = 0x88                                             # scores of 0
+        if masked:
+            mask = np.zeros((T, n), np.float16)
+            mask[:, at] = low
+        else:
+            b[at, ..., 2:] = 0x00                                     # n - 8 = -8, 32 times a block
+            _set(kb, Hk, D, np.where((np.arange(n) == at)[:, None, None], 1.0, _scales(kb, Hk, D)))
+        ranges = [[0, n - 3] if t % 2 == 0 else [3, n // 2] for t in range(T)]
+        clean = _run(dev, q, kb, vb, Hk, 0.5, ranges, mask)
+        vb.reshape(n, Hk, D // 32, 18)[at, Hk - 1, 1, :2] = np.array([bits & 255, bits >> 8], np.uint8)
+        got = _run(dev, q, kb, vb, Hk, 0.5, ranges, mask)
+        lost = np.zeros(got.shape, bool)
+        lost[::2, H - H // Hk:, 32:64] = True
+        assert not np.isfinite(got[lost]).any()
+        np.testing.assert_array_equal(got[~lost], clean[~lost])
