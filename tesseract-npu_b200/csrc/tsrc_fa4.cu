@@ -84,10 +84,14 @@ template <int D, int MODE> __host__ __device__ constexpr uint32_t dec_smem() {
     return WARPS * S::RING + (WARPS + 1u) * 16u * 16u + (S::NG > 1 ? 2u * WARPS * 32u : kMaxCluster + 4u) * kRowsOf<MODE> * 4u;
 }
 
-// The weights' scale, by the exponent field v of the largest |dV| met: p is taken times 2^weight_exp(v) and, where
-// all dV are tiny, dV times 2^10, so that w = p dV stays below 2^15 and keeps its digits above fp16's last, 2^-24.
-__device__ __forceinline__ int weight_exp(uint32_t v) { return v >= 15u ? 29 - (int)v : 15; }
-__device__ __forceinline__ int value_exp(uint32_t v) { return v < 5u ? 10 : 0; }
+// Weights go in as 2^10 p dV: below 2^15 for scales of V below 32, with digits down to fp16's last, 2^-24. Where all scales
+// that a warp has met are below 2^-10, they are taken times 2^10. A cell with a scale of 32 and above (no row of ordinary
+// size has one) has its scales divided by 2^x, x that scale's exponent field above kFarExp, and x added to its scores for the
+// weights (not for their sum): the rows that see it follow by their running maximum, those that do not keep their digits.
+constexpr float kWeightUp = 10.0f;
+constexpr int kTinyUp = 10;
+constexpr uint32_t kFarExp = 19;           // exponent field of scales of 16 to 32
+constexpr uint32_t kTinyExp = 5;           // ... and of 2^-10 to 2^-9
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // Decode attention, one pass over the cells.
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
     }
 
     float o[NT][NB][2][4] = {}, wsum[NT][NB][2] = {}, m[NT][2], l[NT][2], off[NT][2];
-    uint32_t vexp = 1;
+    bool tiny = true;        // no scale of V of 2^-10 and above was met
     uint32_t lost = 0;       // bit 4 (2 n + i) + b: the row sees a scale of V in block b that is infinite or no number
 #pragma unroll
     for (uint32_t n = 0; n < NT; ++n)
@@ -428,19 +432,45 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
         }
         bool moved = false;
         float rescale = 1.0f;
-        if ((big >> 10) > vexp) {                                 // the same for the whole warp
-            const uint32_t v = big >> 10;
-            const int p = weight_exp(v) - weight_exp(vexp);
-            rescale = pow2(p + value_exp(v) - value_exp(vexp));
-#pragma unroll
-            for (uint32_t n = 0; n < NT; ++n) {
-                l[n][0] *= pow2(p);
-                l[n][1] *= pow2(p);
-            }
-            vexp = v;
-            moved = rescale != 1.0f;
+        if (tiny && (big >> 10) >= kTinyExp) {                    // the same for the whole warp
+            tiny = false;
+            rescale = pow2(-kTinyUp);
+            moved = true;
         }
-        const float pexp = (float)weight_exp(vexp);
+        const bool far = (big >> 10) > kFarExp;                   // seldom
+        auto above = [&](uint32_t j) {                            // x of the lane's cell pg + 8 j
+            const uint16_t* pd = reinterpret_cast<const uint16_t*>(sk + S::VD_AT + (pg + 8u * j) * S::DS);
+            uint32_t v = kFarExp;
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                const uint32_t u = pd[b] & 0x7FFFu;
+                v = max(v, u < 0x7C00u ? u >> 10 : 0u);
+            }
+            return (int)(v - kFarExp);
+        };
+        if (far) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const float x = (float)above(j);
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n) {
+                    s[n][0][j] += x;
+                    s[n][1][j] += x;
+                }
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                uint32_t va = kFarExp, vb = kFarExp;
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) {
+                    va = max(va, as_u32(dv[e][b]) >> 10 & 31u);
+                    vb = max(vb, as_u32(dv[e][b]) >> 26 & 31u);
+                }
+                const __half2 down = as_h2((15u + kFarExp - va) << 10 | (15u + kFarExp - vb) << 26);
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) dv[e][b] = __hmul2(dv[e][b], down);
+            }
+        }
         // running maximum and sum; what a row does not see is -inf
         float alpha[NT][2];
 #pragma unroll
@@ -473,14 +503,30 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
                 float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
 #pragma unroll
                 for (uint32_t x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-                const float m_new = fmaxf(m_old, top), base = m_new == -INFINITY ? 0.0f : m_new, up = pexp - base;
+                const float m_new = fmaxf(m_old, top), base = m_new == -INFINITY ? 0.0f : m_new, up = kWeightUp - base;
                 alpha[n][i] = ex2(m_old - base);
                 moved |= m_new > m[n][i] || m_old != m[n][i];
                 m[n][i] = m_new;
 #pragma unroll
                 for (uint32_t j = 0; j < 4; ++j) z[j] = ex2(z[j] + up);
-                l[n][i] = fmaf(l[n][i], alpha[n][i], (z[0] + z[1]) + (z[2] + z[3]));
+                if (!far) l[n][i] = fmaf(l[n][i], alpha[n][i], (z[0] + z[1]) + (z[2] + z[3]));
             }
+        if (far) {
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n) {
+                l[n][0] *= alpha[n][0];
+                l[n][1] *= alpha[n][1];
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const float down = pow2(-above(j));
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n) {
+                    l[n][0] = fmaf(s[n][0][j], down, l[n][0]);
+                    l[n][1] = fmaf(s[n][1][j], down, l[n][1]);
+                }
+            }
+        }
         if (__any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
             for (uint32_t n = 0; n < NT; ++n) {
@@ -499,11 +545,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
                 }
             }
         }
-        if (vexp < 5u) {
+        if (tiny) {
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e)
 #pragma unroll
-                for (uint32_t b = 0; b < NB; ++b) dv[e][b] = __hmul2(dv[e][b], __float2half2_rn(1024.0f));
+                for (uint32_t b = 0; b < NB; ++b) dv[e][b] = __hmul2(dv[e][b], __float2half2_rn((float)(1 << kTinyUp)));
         }
         // the weights of each block, cells now along the lane's pairs and row g in the column
         uint32_t wb[NT][SPLIT ? 2 : 1][4][NB];
@@ -581,7 +627,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
     float* wo = reinterpret_cast<float*>(ringp);
 #pragma unroll
     for (uint32_t x = 4; x < 32; x <<= 1) lost |= __shfl_xor_sync(0xFFFFFFFFu, lost, x);
-    const float unscale = pow2((WHOLE ? 0 : 24) - value_exp(vexp)), pinv = pow2(-weight_exp(vexp));
+    const float pinv = pow2(-(int)kWeightUp), unscale = pinv * pow2((WHOLE ? 0 : 24) - (tiny ? kTinyUp : 0));
 #pragma unroll
     for (uint32_t n = 0; n < NT; ++n) {
 #pragma unroll
@@ -592,8 +638,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
                 for (uint32_t i = 0; i < 2; ++i) {
                     float* p = wo + (8u * n + 2u * t + i) * S::W + 32u * b + 4u * g + 2u * k;
                     const bool none = lost >> (4u * (2u * n + i) + b) & 1u;
-                    p[0] = none ? NAN : (o[n][b][k][i] - wsum[n][b][i]) * (unscale * pinv);
-                    p[1] = none ? NAN : (o[n][b][k][2 + i] * kOdd - wsum[n][b][i]) * (unscale * pinv);
+                    p[0] = none ? NAN : (o[n][b][k][i] - wsum[n][b][i]) * unscale;
+                    p[1] = none ? NAN : (o[n][b][k][2 + i] * kOdd - wsum[n][b][i]) * unscale;
                 }
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
@@ -604,8 +650,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
         }
     }
     __syncthreads();
-    // Each team's factor for each row (a thread per row, in order), the CTA's maximum and sum; then the teams' outputs,
-    // four values a thread, into the first team's place.
+    // Each warp's factor for each row (a thread per row, in order; the warps of a team share sums, and maxima but for far scales),
+    // the CTA's maximum and sum; then the teams' outputs, four values a thread, into the first team's place.
     auto result = [&](uint32_t j, uint32_t r, uint32_t d) {
         return reinterpret_cast<float4*>(sm + (j * S::NG + d / S::W) * S::RING) + (r * S::W + d % S::W) / 4u;
     };
@@ -615,18 +661,18 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
         float ot = -INFINITY, mt = -INFINITY, lt = 0.0f;
         if (MASK) {
 #pragma unroll
-            for (uint32_t j = 0; j < S::TEAMS; ++j) ot = fmaxf(ot, red[j * S::NG * 16u + r].x);
+            for (uint32_t j = 0; j < WARPS; ++j) ot = fmaxf(ot, red[j * 16u + r].x);
         }
         auto level = [&](const float4& p) { return !MASK || p.x == ot || p.y == -INFINITY ? p.y : p.y + (p.x - ot) * kLog2e; };
 #pragma unroll
-        for (uint32_t j = 0; j < S::TEAMS; ++j) mt = fmaxf(mt, level(red[j * S::NG * 16u + r]));
+        for (uint32_t j = 0; j < WARPS; ++j) mt = fmaxf(mt, level(red[j * 16u + r]));
         const float base = mt == -INFINITY ? 0.0f : mt;
 #pragma unroll
-        for (uint32_t j = 0; j < S::TEAMS; ++j) {
-            const float4 p = red[j * S::NG * 16u + r];
-            const float f = p.z == 0.0f ? 0.0f : ex2(level(p) - base);       // a team that saw nothing of the row: 0
-            lt += f * p.z;
-            red[j * S::NG * 16u + r].w = f;
+        for (uint32_t j = 0; j < WARPS; ++j) {
+            const float4 p = red[j * 16u + r];
+            const float f = p.z == 0.0f ? 0.0f : ex2(level(p) - base);       // a warp that saw nothing of the row: 0
+            if (j % S::NG == 0) lt += f * p.z;
+            red[j * 16u + r].w = f;
         }
         fin[r] = make_float4(ot, mt, lt, 0.0f);
     }
@@ -636,7 +682,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (uint32_t j = 0; j < S::TEAMS; ++j) {
-            const float f = red[j * S::NG * 16u + r].w;          // outputs are finite or marked by NaN, which a factor of 0 keeps
+            const float f = red[(j * S::NG + d / S::W) * 16u + r].w;         // outputs are finite or marked by NaN, which a factor of 0 keeps
             const float4 x = *result(j, r, d);
             acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
         }

@@ -147,3 +147,29 @@ def test_scale_of_v_that_is_not_finite_shows_at_any_weight(dev, dtype, T, H, Hk,
         lost[::2, H - H // Hk:, 32:64] = True
         assert not np.isfinite(got[lost]).any()
         np.testing.assert_array_equal(got[~lost], clean[~lost])
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("T,H,Hk", SHAPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_size_of_what_is_hidden_has_no_effect(dev, dtype, T, H, Hk, D, masked):
+    """Small cells seen beside hidden cells of large finite scales, each row with cells of its own."""
+    if D == 256 and T == 1300:
+        T = 100
+    n = 160
+    for large in (20.0, 1000.0, 65504.0):
+        rng, q, kb, vb = _inputs(T + D, T, H, Hk, D, n, dtype)
+        q *= 64
+        big = np.arange(n) % 5 == 4
+        for rows in (kb, vb):
+            d = _scales(rows, Hk, D).astype(np.float64) * 2.0 ** -9
+            d[big] = large
+            _set(rows, Hk, D, d)
+        if masked:
+            mask = np.where(rng.random((T, n)) < 0.5, -np.inf, 0.0).astype(np.float16)
+            mask[:, big] = -np.inf
+            _check(dev, q, kb, vb, Hk, dtype, [[0, n]] * T, mask)
+        else:
+            ranges = [[5 * (t % (n // 5)) + t % 3, 5 * (t % (n // 5)) + 4] for t in range(T)]
+            _check(dev, q, kb, vb, Hk, dtype, ranges)
