@@ -1,5 +1,6 @@
 // tsrc_fa4.cu -- attention over the q4_0 KV cache (tsrc_flash_attn_q4). Cache layout: tsrc_kv4.cuh.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdio>
 #include <type_traits>
@@ -238,7 +239,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, MODE == kRows16 ? 3 : 4) fa4_d
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
         // the row's largest value to [2^12, 2^13); rows of tiny values by 2^100 at most
         const int e = min(12 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
-        const float f = pow2(e), mine = a.scale * kLog2e * (pow2(-e) * (WHOLE ? 1.0f : 16777216.0f));
+        // Step by step, so that only a factor that leaves f32 itself does; cut to the largest finite one, scores of 0 stay 0, and
+        // others are as far apart from each other as any exponential can tell (the smallest is 2^-48 of the factor).
+        const float f = pow2(e), mine = fminf(fmaxf(a.scale * pow2(-e) * (kLog2e * (WHOLE ? 1.0f : 16777216.0f)), -FLT_MAX), FLT_MAX);
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) rs[n][i] = __shfl_sync(0xFFFFFFFFu, mine, 8u * t + 4u * i);
 #pragma unroll

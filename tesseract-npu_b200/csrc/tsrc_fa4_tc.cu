@@ -22,6 +22,7 @@
 // see it keep their digits (beside one of 2^15, a block of the same cell keeps all of its own down to 2^-10). Precision:
 // bf16 outputs take one fp16 term (11 bits) of q (exact), K, V and the weights. f32 and f16 outputs take two terms of each, 22
 // bits (d (n - 8) has 15, so K and V are exact), and three products, the one of the two small terms left out: 2^-22 of the result.
+#include <cfloat>
 #include <type_traits>
 
 #include "tsrc_fa4.cuh"
@@ -350,7 +351,8 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
         const int e2 = min(12 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
         const float f = copysignf(pow2(e2), a.scale);        // the factor that scores get is positive
-        if (lane < 8) c.q_unscale[r] = fabsf(a.scale) * 1.4426950408889634f * pow2(-e2 - kOperandExp);
+        // cut to the largest finite factor: scores of 0 stay 0, and others are as far apart as any exponential can tell
+        if (lane < 8) c.q_unscale[r] = fminf(fabsf(a.scale) * pow2(-e2) * (1.4426950408889634f / (1 << kOperandExp)), FLT_MAX);
 #pragma unroll
         for (uint32_t j = 0; j < D / 32; ++j) {
             uint32_t h[4], l[4];

@@ -11,10 +11,13 @@ Tolerance of an output value (e = 2^-24), for few visible cells or long rows ali
            (96 + n / 256 + 64) e or (4 (n / 64 + 2) + 64) e; together and rounded up, C e with C = 160 + n / 16;
            and half a step of `type` for the last rounding.
 All this is relative to sum p |v| of the output's own channel, so nothing that a row does not see, and no other block's scale,
-widens it. 16-bit outputs of the kernel for few rows take codes as subnormal numbers, which costs up to 2^-16 of
-15 sum p |d| besides; bf16 outputs round weights, and in the kernel for many rows K and V, to one fp16: 2^-10 (A + 1) sum p |v|.
+widens it. 16-bit outputs of the kernel for few rows take codes n = 0..15 as subnormal numbers n 2^-24, which the tensor cores
+align as 2^-14, so that a step is cut by 2^-14 2^-24 of the other operand, 2^-18 of a product with n = 15; a block takes two steps
+for each of two terms, and starts from -8 sum q: 2^-16 of 15 sum |q| |d_K| for a score, and likewise up to 2^-16 of 15 sum p |d|
+for an output, besides; bf16 outputs round weights, and in the kernel for many rows K and V, to one fp16: 2^-10 (A + 1) sum p |v|.
 Where a weight is far below the row's largest it is held to 2^-30 of that, which matters only beside scales of
-V that differ by as much: 2^-28 max |d| over the visible cells.
+V that differ by as much: 2^-28 max |d| over the visible cells. However far off the scores are, an output is a mean of the
+visible values, none of them above 8 max |d|: it is never off by more than twice that.
 """
 import numpy as np
 import pytest
@@ -42,6 +45,10 @@ def _attend(q, kb, vb, Hk, scale, ranges, mask, dtype):
         if seen[t].any():
             most[t] = np.repeat(np.repeat(np.nan_to_num(d[seen[t]].max(0), posinf=0.0), 32, -1), H // Hk, 0)
     ds = (2.0 ** -21 + (6 * D / 16 + 16) * E) * A
+    if dtype != "float32":
+        dk = np.repeat(np.nan_to_num(np.abs(_scales(kb, Hk, D).astype(np.float64)), posinf=0.0), 32, -1)
+        for h in range(H):
+            ds[:, h, 0] += 2.0 ** -16 * 15 * np.where(seen, abs(scale) * (np.abs(q[:, h]) @ dk[:, h // (H // Hk)].T), 0.0).max(1)
     tol = (2 * ds + 2.0 ** -20 + 2.0 ** -21 + (160 + n / 16) * E) * pv + 2.0 ** -28 * most
     if mask is not None:
         spread = np.zeros((T, 1, 1))
@@ -53,7 +60,7 @@ def _attend(q, kb, vb, Hk, scale, ranges, mask, dtype):
         tol += 2.0 ** -16 * 15 * pd
     if dtype == "bfloat16":
         tol += 2.0 ** -10 * (A + 1) * pv + 2.0 ** -16 * 15 * pd
-    return want, tol + np.maximum(HALF[dtype] * np.abs(want), 2.0 ** -25 if dtype == "float16" else 0.0) + 1e-30
+    return want, np.minimum(tol, 16 * most) + np.maximum(HALF[dtype] * np.abs(want), 2.0 ** -25 if dtype == "float16" else 0.0) + 1e-30
 
 
 def _run(dev, q, kb, vb, Hk, scale, ranges=None, mask=None, group=0, max_len=0):
@@ -173,3 +180,23 @@ def test_size_of_what_is_hidden_has_no_effect(dev, dtype, T, H, Hk, D, masked):
         else:
             ranges = [[5 * (t % (n // 5)) + t % 3, 5 * (t % (n // 5)) + 4] for t in range(T)]
             _check(dev, q, kb, vb, Hk, dtype, ranges)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("T,H,Hk", SHAPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_largest_and_smallest_queries(dev, dtype, T, H, Hk, D):
+    """Queries near the type's largest and smallest values, with a scale that makes ordinary scores of them, and with keys of 0."""
+    if D == 256 and T == 1300:
+        T = 100
+    n = 90
+    ranges = [[t % 7, n] for t in range(T)]
+    for size, scale in ((2.0 ** 120, 2.0 ** -123), (2.0 ** 124, 2.0 ** -60), (2.0 ** -70, 2.0 ** 66), (2.0 ** -84, 2.0 ** 81)):
+        _, q, kb, vb = _inputs(T + D, T, H, Hk, D, n, dtype)
+        q *= size
+        if scale == 2.0 ** -60:                                      # scores of 0, whatever the factor
+            kb.reshape(n, -1, 18)[..., 2:] = 0x88
+            for s in (scale, 2.0 ** 100, -2.0 ** 100):
+                _check(dev, q, kb, vb, Hk, dtype, ranges, scale=s)
+        else:
+            _check(dev, q, kb, vb, Hk, dtype, ranges, scale=scale)
