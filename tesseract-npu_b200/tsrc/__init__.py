@@ -205,19 +205,46 @@ def _type_of(a, b=None) -> int:
     _torch or _load_torch()
     if a is None:
         a, b = b, None
-    kind = None if a is None else _kinds.get(a.dtype)
-    if kind is None or (b is not None and b.dtype != a.dtype):
+    kind = _kinds.get(getattr(a, "dtype", None))
+    if kind is None or (b is not None and getattr(b, "dtype", None) != a.dtype):
         raise TsrcError(E_ARG, "tensors must be of one type among float32, float16 and bfloat16")
     return kind
 
 
-def _expect(t, dtype: str, what: str):
-    """t's address after a check of its element type and density (None and raw addresses pass)."""
-    if t is None or isinstance(t, int):
+def _expect(t, dtype: str, what: str, index: int = 0, least: int = 0):
+    """t's address after a check of its element type, density, device and size (None and raw addresses pass)."""
+    if t is None or type(t) is int:
         return t
-    if t.dtype is not getattr(_torch or _load_torch(), dtype) or not t.is_contiguous() or not t.is_cuda:
-        raise TsrcError(E_ARG, f"{what} must be a contiguous CUDA tensor of {dtype}")
+    # get_device: -1 where the tensor is not on a GPU
+    if t.dtype is not getattr(_torch or _load_torch(), dtype) or t.get_device() != index or not t.is_contiguous():
+        raise TsrcError(E_ARG, f"{what} must be a contiguous CUDA tensor of {dtype} on device {index}")
+    if t.numel() < least:
+        raise TsrcError(E_ARG, f"{what} holds {t.numel()} values, the call takes {least}")
     return t.data_ptr()
+
+
+def _rows_at(t, what: str, rows: int, width: int, stride: int, index: int):
+    """(address, values from row to row) of the `rows` rows of `width` values that a call takes from t (None and raw addresses
+    pass). A dense tensor is taken as memory in which rows lie `stride` values apart (0: width); another one must be those rows
+    itself, each dense and all equally far apart, and then its own stride counts."""
+    if t is None or type(t) is int:
+        return t, stride
+    if t.get_device() != index:
+        raise TsrcError(E_ARG, f"{what} must be a CUDA tensor on device {index}")
+    if t.is_contiguous():
+        if (rows - 1) * (stride or width) + width > t.numel() and rows > 0:
+            raise TsrcError(E_ARG, f"{what} holds {t.numel()} values, too few for {rows} rows of {width}, {stride or width} apart")
+        return t.data_ptr(), stride
+    step = 0
+    if t.numel() == rows * width:
+        try:
+            r = t.view(rows, width)
+            step = r.stride(0) if r.stride(1) == 1 else 0
+        except RuntimeError:
+            pass
+    if step < width or stride not in (0, step):
+        raise TsrcError(E_ARG, f"{what} is neither dense nor {rows} dense rows of {width} values" + (f", {stride} apart" if stride else ""))
+    return t.data_ptr(), step
 
 
 def _stream_on(index: int, stream):
@@ -233,7 +260,11 @@ def _workspace(like, nbytes: int, given, stream):
     allocator, taken on the call's own stream: a block is free for the stream that it was taken on, while work queued
     there may still use it."""
     if given is not None:
-        return given, _addr(given), nbytes if isinstance(given, int) else given.numel() * given.element_size()
+        if isinstance(given, int):
+            return given, given, nbytes
+        if given.get_device() != like.get_device() or not given.is_contiguous():
+            raise TsrcError(E_ARG, "workspace must be a contiguous CUDA tensor on the call's device")
+        return given, given.data_ptr(), given.numel() * given.element_size()
     if nbytes == 0:
         return None, None, 0
     torch = _torch or _load_torch()
@@ -481,25 +512,33 @@ class Device:
         """out[t][h] = attention of q[t][h] over the cells of kv that token t sees (tsrc_flash_attn_q4).
         q / out: device f32, f16 or bf16 tensors of one type; ranges: device int32 [T][2]; mask: device f16
         [T][mask_stride]; workspace: a device buffer of flash_attn_q4_workspace bytes, or None to take one from
-        torch's allocator."""
+        torch's allocator. Tensors must lie on the handle's device and hold what the call reads and writes; q and out may be
+        rows of a wider matrix, as a tensor of such rows or as its memory with a stride."""
         kind = _type_of(q, out)
+        qp, q_stride = _rows_at(q, "q", T, n_head * kv.head_dim, q_stride, self.index)
+        op, out_stride = _rows_at(out, "out", T, n_head * kv.head_dim, out_stride, self.index)
         if mask is not None and not isinstance(mask, int) and mask_stride == 0:
             mask_stride = mask.shape[-1]
         nbytes = lib().tsrc_flash_attn_q4_workspace(kind, kv.n_head_kv, kv.head_dim, T, n_head, n_kv, group, max_len)
         ws, ptr, size = _workspace(q, nbytes, workspace, stream)
-        _check(lib().tsrc_flash_attn_q4(self.handle, kv.handle, kind, _addr(q), q_stride, T, n_head, n_kv,
-                                        _expect(ranges, "int32", "ranges"), group, max_len, _expect(mask, "float16", "mask"),
-                                        mask_stride, scale, _addr(out), out_stride, ptr, size, _stream_on(self.index, stream)))
+        _check(lib().tsrc_flash_attn_q4(self.handle, kv.handle, kind, qp, q_stride, T, n_head, n_kv,
+                                        _expect(ranges, "int32", "ranges", self.index, 2 * T), group, max_len,
+                                        _expect(mask, "float16", "mask", self.index, (T - 1) * (mask_stride or n_kv) + n_kv if T else 0),
+                                        mask_stride, scale, op, out_stride, ptr, size, _stream_on(self.index, stream)))
 
     def beam_select(self, logits, scores, out_scores, out_beam, out_token, n_group: int, n_beam: int, n_vocab: int,
                     n_out: int, stride: int = 0, workspace=None, stream=None) -> None:
-        """The n_out best continuations of each group's beams (tsrc_beam_select)."""
+        """The n_out best continuations of each group's beams (tsrc_beam_select). logits: n_group * n_beam device rows, dense or
+        of a wider matrix; scores: device f32 [n_group][n_beam] or None; outputs: device tensors of n_group * n_out values."""
         kind = _type_of(logits)
+        x, stride = _rows_at(logits, "logits", n_group * n_beam, n_vocab, stride, self.index)
+        n = n_group * n_out
         nbytes = lib().tsrc_beam_select_workspace(n_group, n_beam, n_vocab, n_out)
         ws, ptr, size = _workspace(logits, nbytes, workspace, stream)
-        _check(lib().tsrc_beam_select(self.handle, kind, _addr(logits), stride, _expect(scores, "float32", "scores"), n_group,
-                                      n_beam, n_vocab, n_out, _expect(out_scores, "float32", "out_scores"),
-                                      _expect(out_beam, "int32", "out_beam"), _expect(out_token, "int32", "out_token"),
+        _check(lib().tsrc_beam_select(self.handle, kind, x, stride, _expect(scores, "float32", "scores", self.index, n_group * n_beam),
+                                      n_group, n_beam, n_vocab, n_out, _expect(out_scores, "float32", "out_scores", self.index, n),
+                                      _expect(out_beam, "int32", "out_beam", self.index, n),
+                                      _expect(out_token, "int32", "out_token", self.index, n),
                                       ptr, size, _stream_on(self.index, stream)))
 
 
@@ -666,28 +705,33 @@ class Kv4Cache:
         return out
 
     def set_rows(self, k, v, n: int | None = None, cells=None, cell0: int = 0, row_stride: int = 0, stream=None) -> None:
-        """Quantizes device rows [n][E] of k and v (f32, f16 or bf16; either may be None) into cells (device int64)
-        or cell0 + i."""
-        n = self._rows(k, v) if n is None else n
-        _check(lib().tsrc_kv4_set_rows(self.dev.handle, self.handle, _type_of(k, v), _addr(k), _addr(v), n, row_stride,
-                                       _expect(cells, "int64", "cells"), cell0, _stream_on(self.dev.index, stream)))
+        """Quantizes device rows [n][E] of k and v (f32, f16 or bf16; either may be None; dense or of a wider matrix, both with
+        the same stride) into cells (device int64) or cell0 + i."""
+        self._move(lib().tsrc_kv4_set_rows, k, v, n, cells, cell0, row_stride, stream)
 
     def get_rows(self, k, v, n: int | None = None, cells=None, cell0: int = 0, row_stride: int = 0, stream=None) -> None:
         """The values of cells (device int64) or cell0 + i into device rows of k and v (either may be None)."""
-        n = self._rows(k, v) if n is None else n
-        _check(lib().tsrc_kv4_get_rows(self.dev.handle, self.handle, _type_of(k, v), _addr(k), _addr(v), n, row_stride,
-                                       _expect(cells, "int64", "cells"), cell0, _stream_on(self.dev.index, stream)))
+        self._move(lib().tsrc_kv4_get_rows, k, v, n, cells, cell0, row_stride, stream)
 
-    @staticmethod
-    def _rows(k, v) -> int:
+    def _move(self, call, k, v, n, cells, cell0: int, row_stride: int, stream) -> None:
         if k is None and v is None:
             raise TsrcError(E_ARG, "neither k nor v rows")
-        return (v if k is None else k).shape[0]
+        kind, index = _type_of(k, v), self.dev.index
+        n = (v if k is None else k).shape[0] if n is None else n
+        kp, stride = _rows_at(k, "k", n, self.E, row_stride, index)
+        vp, other = _rows_at(v, "v", n, self.E, row_stride, index)
+        if k is None:
+            stride = other
+        elif v is not None and (stride or self.E) != (other or self.E):
+            raise TsrcError(E_ARG, f"k's rows lie {stride or self.E} values apart, v's {other or self.E}")
+        _check(call(self.dev.handle, self.handle, kind, kp, vp, n, stride, _expect(cells, "int64", "cells", index, n), cell0,
+                    _stream_on(index, stream)))
 
     def reorder(self, parent, n_group: int, n_beam: int, seq_stride: int, n: int, cell0: int = 0, stream=None) -> None:
-        """Sequence (g, b) takes the first n cells of (g, parent[g][b]) (device int32), in place."""
-        _check(lib().tsrc_kv4_reorder(self.dev.handle, self.handle, _expect(parent, "int32", "parent"), n_group, n_beam, cell0,
-                                      seq_stride, n, _stream_on(self.dev.index, stream)))
+        """Sequence (g, b) takes the first n cells of (g, parent[g][b]) (device int32 [n_group][n_beam]), in place."""
+        at = _expect(parent, "int32", "parent", self.dev.index, n_group * n_beam)
+        _check(lib().tsrc_kv4_reorder(self.dev.handle, self.handle, at, n_group, n_beam, cell0, seq_stride, n,
+                                      _stream_on(self.dev.index, stream)))
 
     def free(self) -> None:
         if self.handle and self.dev.handle:
