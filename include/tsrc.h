@@ -306,9 +306,10 @@ TSRC_API int tsrc_kv4_set_bytes(tsrc_kv4 * kv, uint32_t which, const void * ggml
 TSRC_API int tsrc_kv4_get_bytes(const tsrc_kv4 * kv, uint32_t which, void * ggml_rows, uint32_t cell0, uint32_t n);
 // Beam search's reordering of its states: n_group groups of n_beam (1..32) sequences, sequence s = g * n_beam + b
 // holding cells [cell0 + s * seq_stride, + n). Afterwards sequence (g, b) holds what (g, parent[g * n_beam + b])
-// held before, K and V, in place (parent: device int32, any values in [0, n_beam), as tsrc_beam_select writes
-// them; -1: the sequence keeps its cells). Another parent keeps them too and makes the next tsrc_sync return
-// TSRC_E_ARG. seq_stride >= n. On `stream`.
+// held before, K and V, in place (parent: device int32 [n_group][n_beam], any values in [0, n_beam); -1: the sequence
+// keeps its cells). Another parent keeps them too and makes the next tsrc_sync return TSRC_E_ARG. seq_stride >= n.
+// tsrc_beam_select's out_beam is such an array where its n_out is n_beam; of a wider one the caller first gathers the n_beam
+// entries that go on (its rows are n_out long). Selection takes up to 64 beams, reordering 32. On `stream`.
 TSRC_API int tsrc_kv4_reorder(tsrc_ctx * ctx, tsrc_kv4 * kv, const int32_t * parent, uint32_t n_group, uint32_t n_beam,
                               uint32_t cell0, uint32_t seq_stride, uint32_t n, void * stream);
 

@@ -728,7 +728,10 @@ class Kv4Cache:
                     _stream_on(index, stream)))
 
     def reorder(self, parent, n_group: int, n_beam: int, seq_stride: int, n: int, cell0: int = 0, stream=None) -> None:
-        """Sequence (g, b) takes the first n cells of (g, parent[g][b]) (device int32 [n_group][n_beam]), in place."""
+        """Sequence (g, b) takes the first n cells of (g, parent[g][b]) (device int32 [n_group][n_beam]), in place. Of a selection with
+        n_out above n_beam, that is the n_beam chosen of each group, made contiguous: not out_beam itself."""
+        if n_group and hasattr(parent, "numel") and parent.numel() != n_group * n_beam:
+            raise TsrcError(E_ARG, f"parent holds {parent.numel()} values, not one for each of {n_group} x {n_beam} sequences")
         at = _expect(parent, "int32", "parent", self.dev.index, n_group * n_beam)
         _check(lib().tsrc_kv4_reorder(self.dev.handle, self.handle, at, n_group, n_beam, cell0, seq_stride, n,
                                       _stream_on(self.dev.index, stream)))

@@ -133,3 +133,14 @@ def test_rows_refuse_tensors_that_do_not_hold_the_call(stub, name):
                            (_on(fused[:, 1]), None, dict(row_stride=128), "k "), (_on(x), None, dict(cells=_on(cells[:4])), "cells"),
                            (_on(x), None, dict(cells=cells), "cells"), (_on(x[:1].expand(5, 128)), None, {}, "k "), (None, None, {}, "neither")):
         _refused(lambda: move(k, v, **kw), what)
+
+
+def test_reorder_refuses_a_selection_that_was_not_gathered(stub):
+    """out_beam of n_out = 2 n_beam: rows twice as long as the parents', whose entries would be read as other groups'."""
+    import torch
+    _, kv = stub
+    wide = torch.zeros(3, 8, dtype=torch.int32)
+    _refused(lambda: kv.reorder(_on(wide[:, :4].contiguous()), 3, 4, 8, 8), "NULL")
+    for parent in (wide, wide.flatten(), wide[:, :4], wide[:2, :4].contiguous()):
+        _refused(lambda: kv.reorder(_on(parent), 3, 4, 8, 8), "parent")
+    _refused(lambda: kv.reorder(wide[:, :4].contiguous(), 3, 4, 8, 8), "parent")

@@ -40,3 +40,27 @@ def test_rows_of_a_fused_projection(dev, dtype, T):
             kv.free()
     for a, b in zip(*res):
         assert torch.equal(a, b)
+
+
+def test_reorder_by_a_selection_of_twice_the_beams(dev):
+    """Several groups, n_out = 2 n_beam: the first n_beam entries of each group go on, gathered."""
+    import torch
+    rng = np.random.default_rng(8)
+    G, B, V, cap = 3, 4, 500, 8
+    kv = dev.kv4_create(1, 64, G * B * cap)
+    try:
+        img = rng.integers(0, 256, (G * B * cap, kv.row_bytes), dtype=np.uint8)
+        kv.set_bytes(tsrc.KV_K, img)
+        x = torch.from_numpy(rng.standard_normal((G, B, V)).astype(np.float32)).cuda()
+        s = torch.empty(G, 2 * B, device="cuda")
+        b, t = (torch.empty(G, 2 * B, dtype=torch.int32, device="cuda") for _ in range(2))
+        dev.beam_select(x, None, s, b, t, n_group=G, n_beam=B, n_vocab=V, n_out=2 * B)
+        with pytest.raises(tsrc.TsrcError):
+            kv.reorder(b, G, B, cap, cap)
+        kv.reorder(b[:, :B].contiguous(), G, B, cap, cap)
+        dev.sync()
+        parent = P.beam(x.double().cpu().numpy(), np.zeros((G, B)), 2 * B)[1][:, :B]
+        want = img.reshape(G, B, -1)[np.arange(G)[:, None], parent].reshape(img.shape)
+        np.testing.assert_array_equal(kv.get_bytes(tsrc.KV_K), want)
+    finally:
+        kv.free()
