@@ -74,6 +74,7 @@ constexpr uint32_t kFarExp = 19;     // exponent field of scales of 16 to 32, th
 struct Control {                     // at most 4 KB
     uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
     uint64_t s_full[2][4], p_full[2][4], o_done[2][2];    // of a lot of rows
+    uint64_t drained;        // the products in flight when a wait ran out
     TileInfo info[4];
     // far tiles: what a cell's scores are times, and what the log2 of its weights is raised by. Of four tiles, as info:
     // the dequant warps are up to two tiles ahead of the softmax when they write these.
@@ -310,6 +311,7 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                 bar_init(&c.p_full[i / 4][i % 4], 4);
             }
             for (uint32_t i = 0; i < 2 * RG; ++i) bar_init(&c.o_done[i / 2][i % 2], 1);
+            bar_init(&c.drained, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
     }
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                         mma_ss(to, qa + ((k == 1 ? S::Q_TERM : 0u) + s * 2u * kRows * 16u >> 4), kb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * kTile * 16u >> 4),
                                instruction(kTile), k != (PRECISE ? 2u : 0u) || s != 0u);
                 }
-                if (rg + 1u == RG) commit(&c.k_free[buf]);
+                if (rg + 1u == RG && i + 2u < tiles) commit(&c.k_free[buf]);      // only where a tile comes that waits for it:
                 commit(&c.s_full[rg][sb]);
                 bar_arrive(&c.s_full[rg][sb]);
                 return true;
@@ -430,13 +432,18 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                         mma_ts(tmem + S::O_COL + rg * D, pa + (k == 1 ? kTile / 2u : 0u) + 8u * s, vb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * D * 16u >> 4),
                                instruction(D), k == (PRECISE ? 2u : 0u) && s == 0u ? (TOTAL ? i % S::FLUSH : i) : 1u);
                 commit(&c.o_done[rg][buf]);
-                if (rg + 1u == RG) commit(&c.v_free[buf]);
+                if (rg + 1u == RG && i + 2u < tiles) commit(&c.v_free[buf]);      // the CTA leaves when the last o_done is there
                 return true;
             };
             bool ok = true;
             for (uint32_t rg = 0; ok && tiles && rg < RG; ++rg) ok = scores(0, rg);
             for (uint32_t i = 0; ok && i < tiles; ++i)
                 for (uint32_t rg = 0; ok && rg < RG; ++rg) ok = (i + 1u == tiles || scores(i + 1u, rg)) && outputs(i, rg);
+            if (!ok) {                                       // given up: what is in flight ends before the CTA leaves
+                uint32_t none = 0;
+                commit(&c.drained);
+                bar_wait(&c.drained, 0, &none);
+            }
         }
         __syncwarp();
     } else if (warp >= S::SW) {
