@@ -12,7 +12,6 @@
 // A candidate is one 64-bit key, the logit's bits made monotone above the complement of its index, so that equal
 // logits go to the lowest index and no two keys are equal. Key 0 stands for none.
 #include <cmath>
-#include <cstdio>
 #include <type_traits>
 
 #include "tsrc_kv4.cuh"
@@ -452,13 +451,6 @@ cudaError_t launch_beam(const void* logits, size_t stride, const float* scores, 
                               scores, n_beam, n_out, out_scores, out_beam, out_token);
 }
 
-template <class... A>
-int refuse(int code, const char* fmt, A... a) {
-    char msg[256];
-    snprintf(msg, sizeof msg, fmt, a...);
-    return set_error(code, msg);
-}
-
 }  // namespace
 
 }  // namespace tsrc
@@ -506,8 +498,7 @@ int tsrc_beam_select(tsrc_ctx* ctx, uint32_t type, const void* logits, uint32_t 
     if (type == TSRC_TYPE_F32) e = launch_beam<float>(logits, stride, scores, n_group, n_beam, n_vocab, n_out, out_scores, out_beam, out_token, parts, maxima, st);
     else if (type == TSRC_TYPE_F16) e = launch_beam<__half>(logits, stride, scores, n_group, n_beam, n_vocab, n_out, out_scores, out_beam, out_token, parts, maxima, st);
     else e = launch_beam<__nv_bfloat16>(logits, stride, scores, n_group, n_beam, n_vocab, n_out, out_scores, out_beam, out_token, parts, maxima, st);
-    if (e != cudaSuccess) return refuse(TSRC_E_CUDA, "tsrc_beam_select: %s (%s)", cudaGetErrorString(e), cudaGetErrorName(e));
-    return TSRC_OK;
+    return e == cudaSuccess ? TSRC_OK : cuda_refuse(e, "tsrc_beam_select");
 }
 
 }  // extern "C"

@@ -2,7 +2,6 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
-#include <cstdio>
 #include <type_traits>
 
 #include "tsrc_fa4.cuh"
@@ -936,13 +935,6 @@ cudaError_t dec_launch_d(const Fa4Args& a, uint32_t D, uint32_t units, cudaStrea
     }
 }
 
-template <class... A>
-int refuse(int code, const char* fmt, A... a) {
-    char msg[256];
-    snprintf(msg, sizeof msg, fmt, a...);
-    return set_error(code, msg);
-}
-
 }  // namespace
 
 }  // namespace tsrc
@@ -1034,8 +1026,7 @@ int tsrc_flash_attn_q4(tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, const v
     else if (type == TSRC_TYPE_F32) e = dec_launch_d<float, kRows8Split>(a, kv->D, p.units, st);
     else if (type == TSRC_TYPE_F16) e = dec_launch_d<__half, kRows8Split>(a, kv->D, p.units, st);
     else e = p.mode == kRows8 ? dec_launch_d<__nv_bfloat16, kRows8>(a, kv->D, p.units, st) : dec_launch_d<__nv_bfloat16, kRows16>(a, kv->D, p.units, st);
-    if (e != cudaSuccess) return refuse(TSRC_E_CUDA, "tsrc_flash_attn_q4: %s (%s)", cudaGetErrorString(e), cudaGetErrorName(e));
-    return TSRC_OK;
+    return e == cudaSuccess ? TSRC_OK : cuda_refuse(e, "tsrc_flash_attn_q4");
 }
 
 }  // extern "C"

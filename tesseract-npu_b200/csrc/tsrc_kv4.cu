@@ -1,6 +1,5 @@
 // tsrc_kv4.cu -- the q4_0 KV cache: storing rows (quantizing them), reading them back, the ggml image, and beam
 // search's reordering, with the cache's C ABI entry points. Layout: tsrc_kv4.cuh.
-#include <cstdio>
 #include <new>
 
 #include "tsrc_kv4.cuh"
@@ -357,17 +356,6 @@ cudaError_t rows_io(bool store, void* k, void* v, uint32_t n, size_t stride, con
     return cudaGetLastError();
 }
 
-template <class... A>
-int refuse(int code, const char* fmt, A... a) {
-    char msg[256];
-    snprintf(msg, sizeof msg, fmt, a...);
-    return set_error(code, msg);
-}
-
-int cuda_refuse(cudaError_t e, const char* what) {
-    return refuse(TSRC_E_CUDA, "%s: %s (%s)", what, cudaGetErrorString(e), cudaGetErrorName(e));
-}
-
 // set_rows and get_rows: the same checks and geometry.
 int kv4_rows(const char* who, bool store, tsrc_ctx* ctx, const tsrc_kv4* kv, uint32_t type, void* k, void* v, uint32_t n,
              uint32_t row_stride, const int64_t* cells, uint32_t cell0, void* stream) {
@@ -408,7 +396,10 @@ int kv4_bytes(const char* who, const tsrc_kv4* kv, uint32_t which, void* rows, u
     const uint32_t part = (uint32_t)(n < 1u + (64u << 20) / row ? n : 1u + (64u << 20) / row);
     uint8_t* stage = nullptr;
     cudaError_t e = cudaMalloc(&stage, part * row);
-    if (e != cudaSuccess) return refuse(TSRC_E_NOMEM, "%s: cudaMalloc of %zu staging bytes", who, part * row);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return refuse(TSRC_E_NOMEM, "%s: cudaMalloc of %zu staging bytes: %s", who, part * row, cudaGetErrorString(e));
+    }
     e = cudaDeviceSynchronize();
     for (uint32_t at = 0; at < n && e == cudaSuccess; at += part) {
         const uint32_t m = n - at < part ? n - at : part;

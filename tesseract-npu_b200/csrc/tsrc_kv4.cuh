@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <stdio.h>
 
 #include <type_traits>
 
@@ -59,6 +60,19 @@ public:
 private:
     int was_ = -1;
 };
+
+template <class... A>
+inline int refuse(int code, const char* fmt, A... a) {
+    char msg[256];
+    snprintf(msg, sizeof msg, fmt, a...);
+    return set_error(code, msg);
+}
+// A CUDA call's error as the entry point's. The runtime keeps it as the thread's last error, which the next launch would take
+// for its own, so it is taken from there.
+inline int cuda_refuse(cudaError_t e, const char* who) {
+    (void)cudaGetLastError();
+    return refuse(TSRC_E_CUDA, "%s: %s (%s)", who, cudaGetErrorString(e), cudaGetErrorName(e));
+}
 
 inline bool kv4_type_ok(uint32_t type) { return type == TSRC_TYPE_F32 || type == TSRC_TYPE_F16 || type == TSRC_TYPE_BF16; }
 inline uint32_t kv4_type_size(uint32_t type) { return type == TSRC_TYPE_F32 ? 4u : 2u; }
