@@ -429,9 +429,11 @@ int tsrc_sync(tsrc_ctx* ctx, void* stream) {
     if (!ctx->kv4_used) return TSRC_OK;
     e = tsrc::kv4_error(&code, true);
     if (e != cudaSuccess) return cuda_fail(e, "reading the q4_0 cache error word");
-    if (code & tsrc::kKv4ErrSet) return fail(TSRC_E_ARG, "tsrc_kv4_set_rows: a cell index outside the cache (those rows were not stored)");
-    if (code & tsrc::kKv4ErrGet) return fail(TSRC_E_ARG, "tsrc_kv4_get_rows: a cell index outside the cache (those rows were not written)");
-    if (code & tsrc::kKv4ErrParent) return fail(TSRC_E_ARG, "tsrc_kv4_reorder: a parent outside [0, n_beam) (those sequences kept their cells)");
+    if (code)                                            // the word is cleared: all that it holds is reported
+        return fail(TSRC_E_ARG, "%s%s%s",
+                    code & tsrc::kKv4ErrSet ? "tsrc_kv4_set_rows: a cell index outside the cache (those rows were not stored); " : "",
+                    code & tsrc::kKv4ErrGet ? "tsrc_kv4_get_rows: a cell index outside the cache (those rows were not written); " : "",
+                    code & tsrc::kKv4ErrParent ? "tsrc_kv4_reorder: a parent outside [0, n_beam) (those sequences kept their cells); " : "");
     e = tsrc::fa4_error(&code, true);
     if (e != cudaSuccess) return cuda_fail(e, "reading the q4_0 attention error word");
     if (code) return fail(TSRC_E_DEVICE, "a q4_0 attention kernel gave up a bounded wait (code %u)", code);
