@@ -271,7 +271,7 @@ TSRC_API int tsrc_flash_attn(tsrc_ctx * ctx, const tsrc_kv * kv, const float * q
 // No counterpart in the reference, whose cache is q8_0 only and whose outputs end at the logits. The cache
 // holds ggml's q4_0 blocks (llama.cpp's q4_0 cache type): per 32 values {fp16 d; 32 codes n of 4 bits}, each
 // value standing for d (n - 8). Values in device memory are f32, f16 or bf16, named by ggml's type numbers.
-// Arithmetic is in f32 or better with rounding to nearest, not the reference's flushing f32 rules. Nothing here
+// Arithmetic is not the reference's flushing f32 rules; each call below says what its own keeps. Nothing here
 // allocates device memory after tsrc_kv4_create (set_bytes / get_bytes stage through a temporary buffer) or
 // synchronises, except where noted, so every queued call may be captured into a CUDA graph; workspaces are the
 // caller's, and calls (or graphs) that may run at the same time need one each. The calling thread's current
@@ -316,18 +316,28 @@ TSRC_API int tsrc_kv4_reorder(tsrc_ctx * ctx, tsrc_kv4 * kv, const int32_t * par
 // Attention over the cache. For token t < T and query head h < n_head (a multiple of n_head_kv; head h reads KV
 // head h / (n_head / n_head_kv)), over the cells c that t sees:
 //   out[t][h][:] = sum_c p_c V[c] / sum_c p_c,   p_c = exp(s_c - max_c s_c),   s_c = scale * q[t][h] . K[c] + mask[t][c]
-// with K and V the values the codes stand for, products and sums in f32 or better, and one rounding to `type` (of
-// q and out) at the end. Token t sees cells [ranges[2t], ranges[2t + 1]) (device int32, cut to [0, n_kv); NULL: all
-// n_kv) whose mask (device f16 [T][mask_stride], mask_stride >= n_kv or 0 = n_kv, cells from 0; NULL: none) is not
-// -inf; what other cells hold, NaN or infinities included, has no effect. A token that sees no cell gets zeros. A NaN score makes its row NaN; a
-// scale of V that is infinite or no number leaves no finite value in its 32 outputs for the tokens that see its cell.
+// with K and V the values the codes stand for and one rounding to `type` (of q and out) at the end. Maxima, sums and
+// outputs are f32; products run on the tensor cores in fp16 terms. Before that rounding, with A = max_c scale |q| . |K[c]|, B = the
+// same with a block's |d| for |K|, an output is off by
+//   f32   two terms of q and p (22 bits), K and V exact: 4e-5 (1 + A) sum_c p_c |V[c]| at most up to 10000 cells; 1e-6
+//         of it where measured;
+//   f16   the same; calls with few rows on a stretch of cells take codes as subnormal operands: 2^-12 (B sum_c p_c |V[c]| + sum_c
+//         p_c |d[c]|) besides (1.4e-5 of a row where measured);
+//   bf16  one term: p to 11 bits, for many rows K and V too: 2^-10 (1 + A) sum_c p_c |V[c]| and what f16 has.
+// A block keeps its digits whatever the scales of other blocks and cells, seen or not: p |d| down to 2^-35 (few rows), p
+// to 2^-31 of the row's largest (many rows); beside a scale of 2^(5 + x) in its own cell, down to 2^x times that.
+// Token t sees cells [ranges[2t], ranges[2t + 1]) (device int32, cut to [0, n_kv); NULL: all n_kv) whose mask (device f16
+// [T][mask_stride], mask_stride >= n_kv or 0 = n_kv, cells from 0; NULL: none) is not -inf; what other cells hold, NaN or
+// infinities included, has no effect. A token that sees no cell gets zeros. A NaN score makes its row NaN; a scale of V that is
+// infinite or no number leaves no finite value in its 32 outputs for the tokens that see its cell, whatever their weight.
 // So a decode step of many sequences, a causal or windowed prompt and a drafted tree are one call each; the ranges
 // may be rewritten on the device between replays of a captured call.
 // group (0 = T): consecutive tokens that read about the same cells (a sequence's); T must be a multiple of it.
 // max_len (0 = n_kv): about how many cells one group's tokens span. Both choose how the work is split, never what
-// is computed. q and out: device, token rows q_stride / out_stride values apart (0 = n_head * head_dim), heads dense.
+// is computed beyond the last digits. q and out: device, token rows q_stride / out_stride values apart (0 = n_head * head_dim), heads dense.
 // ws: ws_bytes of device memory (256-byte aligned), at least tsrc_flash_attn_q4_workspace's (NULL when that is 0);
-// its content needs no initialisation. out must not overlap q. On `stream`.
+// its content needs no initialisation. out must not overlap q. A kernel for many rows bounds its waits (about a second); where one
+// runs out, tsrc_sync returns TSRC_E_DEVICE and what that call left in out is not defined. On `stream`.
 TSRC_API int tsrc_flash_attn_q4(tsrc_ctx * ctx, const tsrc_kv4 * kv, uint32_t type, const void * q, uint32_t q_stride,
                                 uint32_t T, uint32_t n_head, uint32_t n_kv, const int32_t * ranges, uint32_t group,
                                 uint32_t max_len, const uint16_t * mask, uint32_t mask_stride, float scale, void * out,
@@ -343,7 +353,9 @@ TSRC_API const char * tsrc_flash_attn_q4_unsupported(uint32_t type, uint32_t n_h
 // `stride` values apart, 0 = n_vocab; row g * n_beam + b),
 //   s[b][v] = scores[g][b] + x[b][v] - log(sum_u exp(x[b][u]))       (scores: device f32, NULL = zeros)
 // and the n_out largest over all (b, v) of the group, in descending order, equal ones by ascending (b, v):
-// out_scores (f32), out_beam and out_token (int32), each [n_group][n_out]. Comparisons are on s in f64. A candidate
+// out_scores (f32), out_beam and out_token (int32), each [n_group][n_out]. s is made in f64 from the logit, the row's maximum and
+// a normaliser of f32 sums, within 2^-18 of its value and the same for alike rows wherever they lie; inside a row the
+// order is that of the logits themselves. A candidate
 // whose s is -inf or NaN is never chosen (banned tokens, dead beams; a row with a NaN or +inf logit loses every
 // candidate); where too few are left the rest of the row is (-inf, -1, -1). n_out 1..64, n_beam 1..64.
 // ws as above, tsrc_beam_select_workspace bytes. On `stream`.
