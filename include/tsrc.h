@@ -321,8 +321,8 @@ TSRC_API int tsrc_kv4_reorder(tsrc_ctx * ctx, tsrc_kv4 * kv, const int32_t * par
 // same with a block's |d| for |K|, an output is off by
 //   f32   two terms of q and p (22 bits), K and V exact: 4e-5 (1 + A) sum_c p_c |V[c]| at most up to 10000 cells; 1e-6
 //         of it where measured;
-//   f16   the same; calls with few rows on a stretch of cells take codes as subnormal operands: 2^-12 (B sum_c p_c |V[c]| + sum_c
-//         p_c |d[c]|) besides (1.4e-5 of a row where measured);
+//   f16   the same; calls with few rows on a stretch of cells take codes as subnormal operands: 2^-11 B sum_c p_c |V[c]| + 2^-12 sum_c
+//         p_c |d[c]| besides (1.4e-5 of a row where measured);
 //   bf16  one term: p to 11 bits, for many rows K and V too: 2^-10 (1 + A) sum_c p_c |V[c]| and what f16 has.
 // A block keeps its digits whatever the scales of other blocks and cells, seen or not: p |d| down to 2^-35 (few rows), p
 // to 2^-31 of the row's largest (many rows); beside a scale of 2^(5 + x) in its own cell, down to 2^x times that.

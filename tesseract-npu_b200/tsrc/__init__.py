@@ -14,6 +14,7 @@ device is present, every call raises ``TsrcError``.
 from __future__ import annotations
 
 import ctypes as ct
+import functools
 import os
 
 import numpy as np
@@ -205,8 +206,13 @@ def _type_of(a, b=None) -> int:
     _torch or _load_torch()
     if a is None:
         a, b = b, None
-    kind = _kinds.get(getattr(a, "dtype", None))
-    if kind is None or (b is not None and getattr(b, "dtype", None) != a.dtype):
+    try:
+        kind = _kinds.get(a.dtype)
+        if b is not None and b.dtype is not a.dtype:
+            kind = None
+    except AttributeError:
+        kind = None
+    if kind is None:
         raise TsrcError(E_ARG, "tensors must be of one type among float32, float16 and bfloat16")
     return kind
 
@@ -274,6 +280,17 @@ def _workspace(like, nbytes: int, given, stream):
         with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=like.device) if isinstance(stream, int) else stream):
             ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
     return ws, ws.data_ptr(), nbytes
+
+
+@functools.lru_cache(maxsize=1024)
+def _attn_workspace(*sizes) -> int:
+    """tsrc_flash_attn_q4_workspace, a function of the call's sizes alone, without a call into the library each time."""
+    return lib().tsrc_flash_attn_q4_workspace(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _beam_workspace(*sizes) -> int:
+    return lib().tsrc_beam_select_workspace(*sizes)
 
 
 def flash_attn_q4_unsupported(type_: int, n_head_kv: int, head_dim: int, n_head: int) -> str | None:
@@ -519,7 +536,7 @@ class Device:
         op, out_stride = _rows_at(out, "out", T, n_head * kv.head_dim, out_stride, self.index)
         if mask is not None and not isinstance(mask, int) and mask_stride == 0:
             mask_stride = mask.shape[-1]
-        nbytes = lib().tsrc_flash_attn_q4_workspace(kind, kv.n_head_kv, kv.head_dim, T, n_head, n_kv, group, max_len)
+        nbytes = _attn_workspace(kind, kv.n_head_kv, kv.head_dim, T, n_head, n_kv, group, max_len)
         ws, ptr, size = _workspace(q, nbytes, workspace, stream)
         _check(lib().tsrc_flash_attn_q4(self.handle, kv.handle, kind, qp, q_stride, T, n_head, n_kv,
                                         _expect(ranges, "int32", "ranges", self.index, 2 * T), group, max_len,
@@ -533,7 +550,7 @@ class Device:
         kind = _type_of(logits)
         x, stride = _rows_at(logits, "logits", n_group * n_beam, n_vocab, stride, self.index)
         n = n_group * n_out
-        nbytes = lib().tsrc_beam_select_workspace(n_group, n_beam, n_vocab, n_out)
+        nbytes = _beam_workspace(n_group, n_beam, n_vocab, n_out)
         ws, ptr, size = _workspace(logits, nbytes, workspace, stream)
         _check(lib().tsrc_beam_select(self.handle, kind, x, stride, _expect(scores, "float32", "scores", self.index, n_group * n_beam),
                                       n_group, n_beam, n_vocab, n_out, _expect(out_scores, "float32", "out_scores", self.index, n),
