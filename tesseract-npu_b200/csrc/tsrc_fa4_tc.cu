@@ -74,7 +74,6 @@ constexpr uint32_t kFarExp = 19;     // exponent field of scales of 16 to 32, th
 struct Control {                     // at most 4 KB
     uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
     uint64_t s_full[2][4], p_full[2][4], o_done[2][2];    // of a lot of rows
-    uint64_t drained;        // the products in flight when a wait ran out
     TileInfo info[4];
     // far tiles: what a cell's scores are times, and what the log2 of its weights is raised by. Of four tiles, as info:
     // the dequant warps are up to two tiles ahead of the softmax when they write these.
@@ -82,6 +81,8 @@ struct Control {                     // at most 4 KB
     uint32_t tmem, abort;
     int32_t span[8][2];      // the softmax warps' first and last cell
     float q_unscale[2 * kRows];
+    uint64_t drained;        // the products in flight when a wait ran out
+    uint32_t never;          // stays 0
 };
 
 static_assert(sizeof(Control) <= 4096, "room behind the operands");
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)), "n"(S::COLUMNS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         if (lane == 0) {
-            c.abort = 0;
+            c.abort = c.never = 0;
             for (int i = 0; i < 2; ++i) {
                 bar_init(&c.k_full[i], S::DW);
                 bar_init(&c.k_free[i], 1);
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                         mma_ss(to, qa + ((k == 1 ? S::Q_TERM : 0u) + s * 2u * kRows * 16u >> 4), kb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * kTile * 16u >> 4),
                                instruction(kTile), k != (PRECISE ? 2u : 0u) || s != 0u);
                 }
-                if (rg + 1u == RG && i + 2u < tiles) commit(&c.k_free[buf]);      // only where a tile comes that waits for it:
+                if (rg + 1u == RG) commit(&c.k_free[buf]);
                 commit(&c.s_full[rg][sb]);
                 bar_arrive(&c.s_full[rg][sb]);
                 return true;
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
                         mma_ts(tmem + S::O_COL + rg * D, pa + (k == 1 ? kTile / 2u : 0u) + 8u * s, vb + ((k == 2 ? S::KV_TERM : 0u) + s * 2u * D * 16u >> 4),
                                instruction(D), k == (PRECISE ? 2u : 0u) && s == 0u ? (TOTAL ? i % S::FLUSH : i) : 1u);
                 commit(&c.o_done[rg][buf]);
-                if (rg + 1u == RG && i + 2u < tiles) commit(&c.v_free[buf]);      // the CTA leaves when the last o_done is there
+                if (rg + 1u == RG) commit(&c.v_free[buf]);
                 return true;
             };
             bool ok = true;
@@ -440,9 +441,8 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
             for (uint32_t i = 0; ok && i < tiles; ++i)
                 for (uint32_t rg = 0; ok && rg < RG; ++rg) ok = (i + 1u == tiles || scores(i + 1u, rg)) && outputs(i, rg);
             if (!ok) {                                       // given up: what is in flight ends before the CTA leaves
-                uint32_t none = 0;
                 commit(&c.drained);
-                bar_wait(&c.drained, 0, &none);
+                bar_wait(&c.drained, 0, &c.never);
             }
         }
         __syncwarp();
@@ -611,6 +611,12 @@ __global__ void __launch_bounds__(TcShape<T, D, MASK, RG>::THREADS, TcShape<T, D
             __syncwarp();
             if (lane == 0) bar_arrive(&c.v_full[buf]);
         }
+        // the last tiles' buffers come free too before the CTA leaves, so that no arrival comes after it
+        for (uint32_t b = 0; ok && dw == 0 && b < 2; ++b) {
+            const uint32_t n = (tiles + 1u - b) >> 1;            // phases of buffer b
+            if (n) ok = bar_wait(&c.k_free[b], (n - 1u) & 1u, &c.abort) && bar_wait(&c.v_free[b], (n - 1u) & 1u, &c.abort);
+        }
+        __syncwarp();
     } else {
         // ---- softmax: this thread's row
         const uint32_t rg = warp / 4u, mine = tmem + ((warp % 4u * 32u) << 16), o_at = mine + S::O_COL + rg * D;
