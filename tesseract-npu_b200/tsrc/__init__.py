@@ -233,6 +233,8 @@ def _rows_at(t, what: str, rows: int, width: int, stride: int, index: int):
     """(address, values from row to row) of the `rows` rows of `width` values that a call takes from t (None and raw addresses
     pass). A dense tensor is taken as memory in which rows lie `stride` values apart (0: width); another one must be those rows
     itself, each dense and all equally far apart, and then its own stride counts."""
+    if rows < 0 or stride < 0:
+        raise TsrcError(E_ARG, f"{what}: {rows} rows, {stride} apart")
     if t is None or type(t) is int:
         return t, stride
     if t.get_device() != index:
@@ -536,6 +538,8 @@ class Device:
         op, out_stride = _rows_at(out, "out", T, n_head * kv.head_dim, out_stride, self.index)
         if mask is not None and not isinstance(mask, int) and mask_stride == 0:
             mask_stride = mask.shape[-1]
+        if mask_stride < 0:
+            raise TsrcError(E_ARG, f"mask_stride {mask_stride}")
         nbytes = _attn_workspace(kind, kv.n_head_kv, kv.head_dim, T, n_head, n_kv, group, max_len)
         ws, ptr, size = _workspace(q, nbytes, workspace, stream)
         _check(lib().tsrc_flash_attn_q4(self.handle, kv.handle, kind, qp, q_stride, T, n_head, n_kv,

@@ -91,7 +91,8 @@ def test_attention_refuses_tensors_that_do_not_hold_the_call(stub):
            (dict(ranges=_on(torch.zeros(5, 2, dtype=i32))), "ranges"), (dict(ranges=torch.zeros(6, 2, dtype=i32)), "ranges"),
            (dict(mask=_on(torch.zeros(5, 100, dtype=f16))), "mask"), (dict(mask=_on(torch.zeros(6, 200, dtype=f16)[:, :100])), "mask"),
            (dict(mask=_on(torch.zeros(6, 100, dtype=f16), 1)), "mask"), (dict(workspace=torch.zeros(64, dtype=torch.uint8)), "workspace"),
-           (dict(q=4096), "type")]
+           (dict(q=4096), "type"), (dict(q_stride=-256), "q"), (dict(out_stride=-1), "out"), (dict(T=-1), "q"),
+           (dict(mask=_on(torch.zeros(6, 100, dtype=f16)), mask_stride=-100), "mask_stride")]
     for kw, what in bad:
         _refused(lambda: call(**kw), what)
 
@@ -131,7 +132,8 @@ def test_rows_refuse_tensors_that_do_not_hold_the_call(stub, name):
     for k, v, kw, what in ((x, None, {}, "k "), (None, x, {}, "v "), (_on(x, 1), None, {}, "k "), (_on(x), _on(x[:4]), {}, "v "),
                            (_on(x), None, dict(n=6), "k "), (_on(torch.zeros(128, 5).t()), None, {}, "k "), (_on(x), _on(fused[:, 1]), {}, "apart"),
                            (_on(fused[:, 1]), None, dict(row_stride=128), "k "), (_on(x), None, dict(cells=_on(cells[:4])), "cells"),
-                           (_on(x), None, dict(cells=cells), "cells"), (_on(x[:1].expand(5, 128)), None, {}, "k "), (None, None, {}, "neither")):
+                           (_on(x), None, dict(cells=cells), "cells"), (_on(x[:1].expand(5, 128)), None, {}, "k "), (None, None, {}, "neither"),
+                           (_on(x), None, dict(row_stride=-128), "k"), (None, _on(x), dict(n=-1, cells=_on(cells)), "-1 rows")):
         _refused(lambda: move(k, v, **kw), what)
 
 
